@@ -59,6 +59,30 @@ class MMStaticArgs(ctypes.Structure):
         ('timeout_ms', ctypes.c_float), ('device_status_out', ctypes.c_void_p)]
 
 
+class MMBlockNormArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ('residual', 'y', 'gate', 'pre_weight', 'post_weight', 'residual_out', 'normed')] + \
+               [(n, ctypes.c_int64) for n in ('tokens', 'residual_stride', 'y_stride', 'gate_stride', 'residual_out_stride', 'normed_stride')] + \
+               [(n, ctypes.c_int32) for n in ('hidden', 'dtype', 'stream_dtype', 'weight_dtype', 'gate_dtype', 'gate_mode')] + \
+               [(n, ctypes.c_float) for n in ('scale', 'eps', 'weight_offset')]
+
+
+class MMBlockNormGrads(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ('d_residual_out', 'd_normed', 'd_residual', 'd_y', 'd_gate', 'd_pre_weight', 'd_post_weight')] + \
+               [(n, ctypes.c_int64) for n in ('d_residual_out_stride', 'd_normed_stride', 'd_residual_stride', 'd_y_stride', 'd_gate_stride')] + \
+               [('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_int64)]
+
+
+class MMRouterArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ('logits', 'topk_idx', 'topk_weights')] + [('logits_stride', ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ('tokens', 'num_experts', 'topk', 'dtype', 'score_mode')] + [('route_scale', ctypes.c_float)]
+
+
+class MMBalanceArgs(ctypes.Structure):
+    _fields_ = [('cu_seqlens', ctypes.c_void_p), ('num_sequences', ctypes.c_int32), ('balance_coef', ctypes.c_float), ('z_coef', ctypes.c_float)] + \
+               [(n, ctypes.c_void_p) for n in ('counts', 'seq_tokens', 'mean_probs', 'losses')]
+
+
+GATE = {'none': 0, 'channel': 1, 'token': 2, 'element': 3}
 STATIC_SCRATCH_BYTES = 24 * 1024 * 1024 + 128 * 1024
 TUNE = {'knobs': 0, 'stages': 1, 'prefetch_w1_experts': 2, 'prefetch_w2_experts': 3, 'row_cache': 4}
 KNOB_PREFETCH, KNOB_OWN_ROWS, KNOB_EARLY_COMBINE = 1, 2, 4
@@ -67,7 +91,9 @@ WINDOW_HANDLE_BYTES = 64
 EXPORTS = ('mm_get_layout', 'mm_get_weight_geometry', 'mm_get_token_alignment', 'mm_mega_moe_launch',
            'mm_frontend_launch', 'mm_frontend_workspace_bytes', 'mm_mega_moe_from_hidden_launch', 'mm_reset',
            'mm_read_device_status', 'mm_read_phase_stamps', 'mm_status_string', 'mm_last_cuda_error',
-           'mm_mega_moe_launch_static_scratch', 'mm_set_tuning', 'mm_get_tuning', 'mm_read_sm_phases', 'mm_fe_forward', 'mm_fe_workspace_bytes', 'mm_fe_router_ctas', 'mm_transform_weights', 'mm_cast_rows_to_fp4', 'mm_tensor_absmax', 'mm_window_alloc', 'mm_window_open', 'mm_window_close')
+           'mm_mega_moe_launch_static_scratch', 'mm_set_tuning', 'mm_get_tuning', 'mm_read_sm_phases', 'mm_fe_forward', 'mm_fe_workspace_bytes', 'mm_fe_router_ctas', 'mm_transform_weights', 'mm_cast_rows_to_fp4', 'mm_tensor_absmax', 'mm_window_alloc', 'mm_window_open', 'mm_window_close',
+           'mm_block_norm', 'mm_block_norm_workspace_bytes', 'mm_block_norm_backward', 'mm_route_tokens', 'mm_balance_workspace_bytes', 'mm_balance_loss',
+           'mm_router_backward')
 
 _libs = {}
 
@@ -112,6 +138,16 @@ def load(check: bool = False) -> ctypes.CDLL:
     lib.mm_window_alloc.argtypes = [ctypes.c_int64, P(ctypes.c_void_p), ctypes.c_char_p]
     lib.mm_window_open.argtypes = [ctypes.c_char_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, P(ctypes.c_void_p)]
     lib.mm_window_close.argtypes = [P(ctypes.c_void_p), ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
+    # (the Python side hands these structures over as packed bytes)
+    lib.mm_block_norm.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    lib.mm_block_norm_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32]
+    lib.mm_block_norm_workspace_bytes.restype = ctypes.c_int64
+    lib.mm_block_norm_backward.argtypes = [ctypes.c_void_p] * 3
+    lib.mm_route_tokens.argtypes = [ctypes.c_void_p] * 4
+    lib.mm_balance_workspace_bytes.argtypes = [ctypes.c_int32, ctypes.c_int32]
+    lib.mm_balance_workspace_bytes.restype = ctypes.c_int64
+    lib.mm_balance_loss.argtypes = [ctypes.c_void_p] * 3 + [ctypes.c_int64, ctypes.c_void_p]
+    lib.mm_router_backward.argtypes = [ctypes.c_void_p] * 3 + [ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
     lib.mm_status_string.argtypes = [ctypes.c_int]
     lib.mm_status_string.restype = ctypes.c_char_p
     lib.mm_last_cuda_error.restype = ctypes.c_char_p

@@ -12,16 +12,23 @@
 #include "mm_batch.cuh"
 #include "mm_decode.cuh"
 #include "mm_device_attribute.h"
+#include "mm_error.h"
 
-namespace {
+namespace mm {
 
-thread_local char g_cuda_error[256] = "";
+thread_local char g_cuda_error[kErrorBytes] = "";
 
 int cuda_fail(cudaError_t e, const char* what) {
     snprintf(g_cuda_error, sizeof(g_cuda_error), "%s: %s", what, cudaGetErrorString(e));
     return MM_ERR_CUDA;
 }
-#define MM_CUDA(call) do { cudaError_t e_ = (call); if (e_ != cudaSuccess) return cuda_fail(e_, #call); } while (0)
+
+}  // namespace mm
+
+namespace {
+
+using mm::cuda_fail;
+using mm::g_cuda_error;
 
 inline int64_t align_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 

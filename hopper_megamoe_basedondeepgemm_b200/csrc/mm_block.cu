@@ -1,0 +1,363 @@
+// C ABI of the operators around the layer: a block's norms, routing from logits, the balance loss. Argument checks and launches; no torch types, no exceptions.
+#include <cuda_runtime.h>
+#include <cmath>
+#include <cstring>
+
+#include "../../include/megamoe_b200.h"
+#include "mm_block_norm.cuh"
+#include "mm_router.cuh"
+#include "mm_error.h"
+
+namespace {
+
+int sm_count(int* out) {
+    int dev = 0;
+    MM_CUDA(cudaGetDevice(&dev));
+    MM_CUDA(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev));
+    return MM_OK;
+}
+
+int dtype_bytes(int dtype) { return dtype == MM_DTYPE_FP32 ? 4 : 2; }
+bool known_dtype(int dtype) { return dtype == MM_DTYPE_BF16 || dtype == MM_DTYPE_FP16 || dtype == MM_DTYPE_FP32; }
+
+// ----------------------------------------------------------------------------- norms
+// Rows of a tensor in memory: what two of them share decides whether one may be written while the other is read.
+struct Rows {
+    const void* p;
+    int64_t ld, width;                       // bytes between rows, bytes of a row
+    int64_t n;
+};
+
+bool share_memory(const Rows& a, const Rows& b) {
+    if (a.p == nullptr || b.p == nullptr || a.n == 0 || b.n == 0) return false;
+    const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+    const uintptr_t ea = pa + (a.n - 1) * a.ld + a.width, eb = pb + (b.n - 1) * b.ld + b.width;
+    if (ea <= pb || eb <= pa) return false;
+    if (a.ld != b.ld || a.ld == 0) return true;
+    const int64_t d = pa > pb ? static_cast<int64_t>((pa - pb) % a.ld) : static_cast<int64_t>((pb - pa) % a.ld);
+    const int64_t first = pa > pb ? b.width : a.width, second = pa > pb ? a.width : b.width;       // columns of one buffer lie beside each other
+    return !(d >= first && a.ld - d >= second);
+}
+
+// An output may be the very rows of an input that is read by the thread which writes them, and nothing else of any tensor of the call.
+bool writes_safely(const Rows& out, const Rows* others, int n, bool in_place) {
+    for (int i = 0; i < n; ++i)
+        if (share_memory(out, others[i]) && !(in_place && out.p == others[i].p && out.ld == others[i].ld && out.width == others[i].width)) return false;
+    return true;
+}
+
+struct NormShape {
+    bool vec;
+    int chunks, threads;
+};
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }
+
+int norm_check(const mm_block_norm_args_t* a) {
+    if (a == nullptr || a->tokens < 0 || a->tokens > 0x7fffffffll || a->hidden < 1) return MM_ERR_INVALID_ARGUMENT;
+    if (!known_dtype(a->dtype) || !known_dtype(a->stream_dtype) || !known_dtype(a->weight_dtype) || !known_dtype(a->gate_dtype)) return MM_ERR_INVALID_ARGUMENT;
+    if (a->hidden > mm::kBnMaxHidden) return MM_ERR_UNSUPPORTED;
+    if (a->stream_dtype != a->dtype && a->stream_dtype != MM_DTYPE_FP32) return MM_ERR_UNSUPPORTED;
+    if (a->weight_dtype != a->dtype && a->weight_dtype != MM_DTYPE_FP32) return MM_ERR_UNSUPPORTED;
+    if (a->gate_dtype != a->dtype && a->gate_dtype != MM_DTYPE_FP32) return MM_ERR_UNSUPPORTED;
+    if (a->gate_mode < MM_GATE_NONE || a->gate_mode > MM_GATE_ELEMENT) return MM_ERR_INVALID_ARGUMENT;
+    if (a->tokens > 0) {                     // (tensors of no rows have no address)
+        if ((a->gate_mode != MM_GATE_NONE) != (a->gate != nullptr) || (a->gate != nullptr && a->y == nullptr)) return MM_ERR_INVALID_ARGUMENT;
+        if (a->y == nullptr && (a->post_weight != nullptr || a->pre_weight == nullptr)) return MM_ERR_INVALID_ARGUMENT;
+    }
+    if (!(a->eps > 0.f) || !std::isfinite(a->eps) || !std::isfinite(a->scale) || !std::isfinite(a->weight_offset)) return MM_ERR_INVALID_ARGUMENT;
+    return MM_OK;
+}
+
+// Rows of a tensor as the call gives them; a single row needs no distance to the next.
+Rows rows_of(const void* p, int64_t ld, int64_t n, int32_t hidden, int dtype) {
+    return Rows{p, ld * dtype_bytes(dtype), static_cast<int64_t>(hidden) * dtype_bytes(dtype), n};
+}
+
+NormShape norm_shape(const mm_block_norm_args_t* a, const Rows* rows, int n) {
+    NormShape s;
+    s.vec = a->hidden % 8 == 0;
+    for (int i = 0; i < n; ++i)
+        if (rows[i].p != nullptr && (!aligned16(rows[i].p) || (rows[i].ld & 15) != 0)) s.vec = false;
+    s.chunks = a->hidden <= 8 * mm::kBnMaxThreads ? 1 : 2;
+    const int per = 8 * s.chunks;
+    s.threads = ((a->hidden + per - 1) / per + 31) / 32 * 32;
+    return s;
+}
+
+mm::BnParams norm_params(const mm_block_norm_args_t* a) {
+    mm::BnParams q;
+    memset(&q, 0, sizeof(q));
+    q.residual = a->residual; q.y = a->y; q.gate = a->gate; q.pre_w = a->pre_weight; q.post_w = a->post_weight;
+    q.residual_out = a->residual_out; q.normed = a->normed;
+    q.tokens = a->tokens;
+    q.residual_ld = a->residual_stride; q.y_ld = a->y_stride; q.gate_ld = a->gate_stride;
+    q.residual_out_ld = a->residual_out_stride; q.normed_ld = a->normed_stride;
+    q.hidden = a->hidden; q.gate_mode = a->gate_mode;
+    q.weight32 = a->weight_dtype == MM_DTYPE_FP32; q.gate32 = a->gate_dtype == MM_DTYPE_FP32;
+    q.scale = a->scale; q.eps = a->eps; q.offset = a->weight_offset;
+    return q;
+}
+
+#define MM_NORM_CASE(X, R, C, V, KERNEL) KERNEL<X, R, C, V><<<grid, s.threads, 0, stream>>>(q)
+#define MM_NORM_SHAPE(X, R, KERNEL)                                                     \
+    do {                                                                                \
+        if (s.vec) { if (s.chunks == 1) MM_NORM_CASE(X, R, 1, true, KERNEL); else MM_NORM_CASE(X, R, 2, true, KERNEL); }   \
+        else { if (s.chunks == 1) MM_NORM_CASE(X, R, 1, false, KERNEL); else MM_NORM_CASE(X, R, 2, false, KERNEL); }       \
+    } while (0)
+#define MM_NORM_LAUNCH(KERNEL)                                                                                              \
+    do {                                                                                                                    \
+        if (a->dtype == MM_DTYPE_FP32) MM_NORM_SHAPE(float, float, KERNEL);                                                 \
+        else if (a->dtype == MM_DTYPE_BF16 && a->stream_dtype == MM_DTYPE_BF16) MM_NORM_SHAPE(__nv_bfloat16, __nv_bfloat16, KERNEL);     \
+        else if (a->dtype == MM_DTYPE_BF16) MM_NORM_SHAPE(__nv_bfloat16, float, KERNEL);                                    \
+        else if (a->stream_dtype == MM_DTYPE_FP16) MM_NORM_SHAPE(__half, __half, KERNEL);                                   \
+        else MM_NORM_SHAPE(__half, float, KERNEL);                                                                          \
+    } while (0)
+
+// Rows that the CTAs of a backward pass share out: each leaves one row of partial sums.
+int64_t norm_backward_ctas(int64_t tokens) {
+    const int64_t most = 296;
+    return tokens < most ? tokens : most;
+}
+
+// ----------------------------------------------------------------------------- router
+int router_check(const mm_router_args_t* a) {
+    if (a == nullptr || a->tokens < 0 || a->num_experts < 1 || a->topk < 1) return MM_ERR_INVALID_ARGUMENT;
+    if (!known_dtype(a->dtype) || (a->score_mode != 0 && a->score_mode != 1)) return MM_ERR_INVALID_ARGUMENT;
+    if (a->num_experts > mm::kRtMaxExperts || a->topk > mm::kRtMaxTopk || a->tokens > (1 << 27)) return MM_ERR_UNSUPPORTED;
+    if (a->topk > a->num_experts) return MM_ERR_INVALID_ARGUMENT;
+    if (a->tokens > 0 && (a->logits == nullptr || a->topk_idx == nullptr)) return MM_ERR_INVALID_ARGUMENT;
+    if (a->tokens > 1 && a->logits_stride < a->num_experts) return MM_ERR_INVALID_ARGUMENT;
+    return MM_OK;
+}
+
+mm::RtParams router_params(const mm_router_args_t* a) {
+    mm::RtParams q;
+    memset(&q, 0, sizeof(q));
+    q.logits = a->logits; q.logits_ld = a->logits_stride;
+    q.idx = reinterpret_cast<long long*>(a->topk_idx); q.weights = a->topk_weights;
+    q.T = a->tokens; q.E = a->num_experts; q.K = a->topk; q.S = 1; q.mode = a->score_mode;
+    q.route_scale = a->route_scale;
+    return q;
+}
+
+void balance_params(const mm_balance_args_t* b, mm::RtParams& q) {
+    q.cu = b->cu_seqlens; q.S = b->num_sequences;
+    q.balance_coef = b->balance_coef; q.z_coef = b->z_coef;
+    q.counts = b->counts; q.tokens = b->seq_tokens; q.mean = b->mean_probs; q.losses = b->losses;
+}
+
+int balance_check(const mm_balance_args_t* b) {
+    if (b == nullptr || b->num_sequences < 1 || (b->cu_seqlens == nullptr && b->num_sequences != 1)) return MM_ERR_INVALID_ARGUMENT;
+    if (b->counts == nullptr || b->seq_tokens == nullptr) return MM_ERR_INVALID_ARGUMENT;
+    if (!std::isfinite(b->balance_coef) || !std::isfinite(b->z_coef)) return MM_ERR_INVALID_ARGUMENT;
+    return MM_OK;
+}
+
+#define MM_ROUTER_EXPERTS(L, KERNEL)                                                              \
+    do {                                                                                          \
+        const int v = (q.E + 31) / 32;                                                            \
+        if (v <= 1) KERNEL<L, 1><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);                      \
+        else if (v <= 2) KERNEL<L, 2><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);                 \
+        else if (v <= 4) KERNEL<L, 4><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);                 \
+        else if (v <= 8) KERNEL<L, 8><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);                 \
+        else if (v <= 12) KERNEL<L, 12><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);               \
+        else if (v <= 16) KERNEL<L, 16><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);               \
+        else KERNEL<L, 32><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);                            \
+    } while (0)
+#define MM_ROUTER_LAUNCH(KERNEL)                                                                  \
+    do {                                                                                          \
+        if (a->dtype == MM_DTYPE_FP32) MM_ROUTER_EXPERTS(float, KERNEL);                          \
+        else if (a->dtype == MM_DTYPE_BF16) MM_ROUTER_EXPERTS(__nv_bfloat16, KERNEL);             \
+        else MM_ROUTER_EXPERTS(__half, KERNEL);                                                   \
+    } while (0)
+
+int router_grid(int tokens, int sms) {
+    const int blocks = (tokens + mm::kRtWarps - 1) / mm::kRtWarps, most = sms * 8;
+    return blocks < most ? (blocks > 0 ? blocks : 1) : most;
+}
+
+constexpr int kBalanceGrid = 1184;           // CTAs of the balance kernel at most (eight per SM of 148): the workspace does not depend on the device
+
+int balance_grid(int tokens) {
+    const int blocks = (tokens + mm::kRtWarps - 1) / mm::kRtWarps;
+    return blocks < kBalanceGrid ? (blocks > 0 ? blocks : 1) : kBalanceGrid;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mm_block_norm(const mm_block_norm_args_t* a, void* stream_ptr) {
+    int st = norm_check(a);
+    if (st != MM_OK) return st;
+    if (a->tokens == 0) return MM_OK;
+    if (a->residual == nullptr || (a->y != nullptr) != (a->residual_out != nullptr) || (a->pre_weight != nullptr) != (a->normed != nullptr)) return MM_ERR_INVALID_ARGUMENT;
+    const bool element = a->gate_mode == MM_GATE_ELEMENT;
+    const int64_t t = a->tokens;
+    Rows rows[7] = {rows_of(a->residual_out, a->residual_out_stride, t, a->hidden, a->stream_dtype), rows_of(a->normed, a->normed_stride, t, a->hidden, a->dtype),
+                    rows_of(a->residual, a->residual_stride, t, a->hidden, a->stream_dtype), rows_of(a->y, a->y_stride, t, a->hidden, a->dtype),
+                    element ? rows_of(a->gate, a->gate_stride, t, a->hidden, a->gate_dtype)
+                            : rows_of(a->gate, a->gate_mode == MM_GATE_TOKEN ? a->gate_stride : 0, a->gate_mode == MM_GATE_TOKEN ? t : 1,
+                                      a->gate_mode == MM_GATE_TOKEN ? 1 : a->hidden, a->gate_dtype),
+                    rows_of(a->pre_weight, 0, 1, a->hidden, a->weight_dtype), rows_of(a->post_weight, 0, 1, a->hidden, a->weight_dtype)};
+    for (int i = 0; i < 2; ++i)
+        if (t > 1 && rows[i].p != nullptr && rows[i].ld < rows[i].width) return MM_ERR_INVALID_ARGUMENT;
+    if (!writes_safely(rows[0], rows + 1, 1, false) || !writes_safely(rows[0], rows + 2, 2, true) || !writes_safely(rows[0], rows + 4, 3, false) ||
+        !writes_safely(rows[1], rows + 2, 2, true) || !writes_safely(rows[1], rows + 4, 3, false)) return MM_ERR_INVALID_ARGUMENT;
+    if (t == 1) for (Rows& r : rows) r.ld = 0;
+    if (a->gate_mode == MM_GATE_TOKEN) rows[4].p = nullptr;                 // (read one by one)
+    const NormShape s = norm_shape(a, rows, 7);
+    int sms = 0;
+    st = sm_count(&sms);
+    if (st != MM_OK) return st;
+    const mm::BnParams q = norm_params(a);
+    const int64_t most = static_cast<int64_t>(sms) * (2048 / s.threads < 32 ? 2048 / s.threads : 32);
+    const unsigned grid = static_cast<unsigned>(t < most ? t : most);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    MM_NORM_LAUNCH(mm::block_norm_kernel);
+    MM_CUDA(cudaGetLastError());
+    return MM_OK;
+}
+
+int64_t mm_block_norm_workspace_bytes(int64_t tokens, int32_t hidden) {
+    if (tokens < 0 || hidden < 1 || hidden > mm::kBnMaxHidden) return -1;
+    return norm_backward_ctas(tokens) * hidden * 3 * 4;
+}
+
+int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_grads_t* g, void* stream_ptr) {
+    int st = norm_check(a);
+    if (st != MM_OK) return st;
+    if (g == nullptr) return MM_ERR_INVALID_ARGUMENT;
+    const bool channel = a->gate_mode == MM_GATE_CHANNEL, element = a->gate_mode == MM_GATE_ELEMENT, token = a->gate_mode == MM_GATE_TOKEN;
+    if ((a->pre_weight != nullptr) != (g->d_pre_weight != nullptr) || (a->post_weight != nullptr) != (g->d_post_weight != nullptr)) return MM_ERR_INVALID_ARGUMENT;
+    const int sums = (a->pre_weight != nullptr) + (a->post_weight != nullptr) + channel;
+    const int64_t t = a->tokens;
+    if (channel && g->d_gate == nullptr) return MM_ERR_INVALID_ARGUMENT;
+    if (t > 0) {
+        if ((a->pre_weight != nullptr) != (g->d_normed != nullptr) || (a->y != nullptr) != (g->d_y != nullptr) || g->d_residual == nullptr) return MM_ERR_INVALID_ARGUMENT;
+        if ((a->pre_weight != nullptr && a->residual == nullptr) || (a->gate != nullptr && g->d_gate == nullptr)) return MM_ERR_INVALID_ARGUMENT;
+        if (sums > 0 && (g->workspace == nullptr || g->workspace_bytes < mm_block_norm_workspace_bytes(t, a->hidden) || !aligned16(g->workspace))) return MM_ERR_INVALID_ARGUMENT;
+    }
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    const int64_t ctas = norm_backward_ctas(t);
+    if (t > 0) {
+        const Rows none = {nullptr, 0, 0, 0};
+        Rows rows[10] = {rows_of(g->d_residual, g->d_residual_stride, t, a->hidden, a->stream_dtype), rows_of(g->d_y, g->d_y_stride, t, a->hidden, a->dtype),
+                         element ? rows_of(g->d_gate, g->d_gate_stride, t, a->hidden, a->gate_dtype) : (token ? rows_of(g->d_gate, g->d_gate_stride, t, 1, a->gate_dtype) : none),
+                         rows_of(g->d_residual_out, g->d_residual_out_stride, t, a->hidden, a->stream_dtype), rows_of(g->d_normed, g->d_normed_stride, t, a->hidden, a->dtype),
+                         rows_of(a->residual, a->residual_stride, t, a->hidden, a->stream_dtype), rows_of(a->y, a->y_stride, t, a->hidden, a->dtype),
+                         element ? rows_of(a->gate, a->gate_stride, t, a->hidden, a->gate_dtype) : (token ? rows_of(a->gate, a->gate_stride, t, 1, a->gate_dtype) : rows_of(a->gate, 0, 1, a->hidden, a->gate_dtype)),
+                         rows_of(a->pre_weight, 0, 1, a->hidden, a->weight_dtype), rows_of(a->post_weight, 0, 1, a->hidden, a->weight_dtype)};
+        for (int i = 0; i < 3; ++i) {
+            if (t > 1 && rows[i].p != nullptr && rows[i].ld < rows[i].width) return MM_ERR_INVALID_ARGUMENT;
+            for (int k = 0; k < 10; ++k)         // gradients are written apart from everything else
+                if (k != i && share_memory(rows[i], rows[k])) return MM_ERR_INVALID_ARGUMENT;
+        }
+        if (t == 1) for (Rows& r : rows) r.ld = 0;
+        if (token) rows[2].p = rows[7].p = nullptr;
+        const NormShape s = norm_shape(a, rows, 10);
+        mm::BnParams q = norm_params(a);
+        q.d_residual_out = g->d_residual_out; q.d_residual_out_ld = g->d_residual_out_stride;
+        q.d_normed = g->d_normed; q.d_normed_ld = g->d_normed_stride;
+        q.d_residual = g->d_residual; q.d_residual_ld = g->d_residual_stride;
+        q.d_y = g->d_y; q.d_y_ld = g->d_y_stride;
+        q.d_gate = g->d_gate; q.d_gate_ld = g->d_gate_stride;
+        q.partial = static_cast<float*>(g->workspace);
+        const unsigned grid = static_cast<unsigned>(ctas);
+        MM_NORM_LAUNCH(mm::block_norm_backward_kernel);
+        MM_CUDA(cudaGetLastError());
+    }
+    if (sums > 0) {
+        mm::BnSumsParams q;
+        memset(&q, 0, sizeof(q));
+        q.partial = static_cast<const float*>(g->workspace);
+        q.rows = static_cast<int>(ctas); q.hidden = a->hidden;
+        int n = 0;
+        if (a->pre_weight != nullptr) { q.out[n] = g->d_pre_weight; q.is32[n++] = a->weight_dtype == MM_DTYPE_FP32; }
+        if (a->post_weight != nullptr) { q.out[n] = g->d_post_weight; q.is32[n++] = a->weight_dtype == MM_DTYPE_FP32; }
+        if (channel) { q.out[n] = g->d_gate; q.is32[n++] = a->gate_dtype == MM_DTYPE_FP32; }
+        const dim3 grid((a->hidden + 31) / 32, n);
+        if (a->dtype == MM_DTYPE_FP32) mm::block_norm_sums_kernel<float><<<grid, 256, 0, stream>>>(q);
+        else if (a->dtype == MM_DTYPE_BF16) mm::block_norm_sums_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(q);
+        else mm::block_norm_sums_kernel<__half><<<grid, 256, 0, stream>>>(q);
+        MM_CUDA(cudaGetLastError());
+    }
+    return MM_OK;
+}
+
+int mm_route_tokens(const mm_router_args_t* a, const float* expert_bias, const uint8_t* valid, void* stream_ptr) {
+    int st = router_check(a);
+    if (st != MM_OK) return st;
+    if ((expert_bias != nullptr && a->score_mode != 1) || !std::isfinite(a->route_scale)) return MM_ERR_INVALID_ARGUMENT;
+    if (a->tokens == 0) return MM_OK;
+    if (a->topk_weights == nullptr) return MM_ERR_INVALID_ARGUMENT;
+    mm::RtParams q = router_params(a);
+    q.bias = expert_bias; q.valid = valid;
+    int sms = 0;
+    st = sm_count(&sms);
+    if (st != MM_OK) return st;
+    const int grid = router_grid(a->tokens, sms);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    MM_ROUTER_LAUNCH(mm::route_kernel);
+    MM_CUDA(cudaGetLastError());
+    return MM_OK;
+}
+
+int64_t mm_balance_workspace_bytes(int32_t num_experts, int32_t num_sequences) {
+    if (num_experts < 1 || num_experts > mm::kRtMaxExperts || num_sequences < 1) return -1;
+    return static_cast<int64_t>(num_sequences) * num_experts * 8 + static_cast<int64_t>(kBalanceGrid) * mm::kRtWarps * 8;
+}
+
+int mm_balance_loss(const mm_router_args_t* a, const mm_balance_args_t* b, void* workspace, int64_t workspace_bytes, void* stream_ptr) {
+    int st = router_check(a);
+    if (st == MM_OK) st = balance_check(b);
+    if (st != MM_OK) return st;
+    if (b->mean_probs == nullptr || b->losses == nullptr || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 7u) != 0u ||
+        workspace_bytes < mm_balance_workspace_bytes(a->num_experts, b->num_sequences)) return MM_ERR_INVALID_ARGUMENT;
+    mm::RtParams q = router_params(a);
+    balance_params(b, q);
+    const int grid = balance_grid(a->tokens);
+    const int64_t cells = static_cast<int64_t>(q.S) * q.E;
+    q.sums = static_cast<unsigned long long*>(workspace);
+    q.z_part = reinterpret_cast<double*>(q.sums + cells);
+    q.z_parts = grid * mm::kRtWarps;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    MM_CUDA(cudaMemsetAsync(q.sums, 0, cells * 8, stream));
+    MM_CUDA(cudaMemsetAsync(q.counts, 0, cells * 4, stream));
+    MM_CUDA(cudaMemsetAsync(q.tokens, 0, static_cast<size_t>(q.S) * 4, stream));
+    MM_ROUTER_LAUNCH(mm::balance_kernel);
+    MM_CUDA(cudaGetLastError());
+    mm::balance_end_kernel<<<1, 1024, 0, stream>>>(q);
+    MM_CUDA(cudaGetLastError());
+    return MM_OK;
+}
+
+int mm_router_backward(const mm_router_args_t* a, const float* d_topk_weights, const mm_balance_args_t* b, float d_loss, const float* d_loss_ptr,
+                       void* d_logits, int64_t d_logits_stride, void* stream_ptr) {
+    int st = router_check(a);
+    if (st == MM_OK && b != nullptr) st = balance_check(b);
+    if (st != MM_OK) return st;
+    if ((d_topk_weights == nullptr && b == nullptr) || !std::isfinite(a->route_scale)) return MM_ERR_INVALID_ARGUMENT;
+    if (a->tokens == 0) return MM_OK;
+    if (d_logits == nullptr || (a->tokens > 1 && d_logits_stride < a->num_experts)) return MM_ERR_INVALID_ARGUMENT;
+    const int bytes = dtype_bytes(a->dtype);
+    const Rows logits = {a->logits, a->logits_stride * bytes, static_cast<int64_t>(a->num_experts) * bytes, a->tokens};
+    const Rows grads = {d_logits, d_logits_stride * bytes, static_cast<int64_t>(a->num_experts) * bytes, a->tokens};
+    if (!writes_safely(grads, &logits, 1, true)) return MM_ERR_INVALID_ARGUMENT;
+    mm::RtParams q = router_params(a);
+    if (b != nullptr) balance_params(b, q);
+    q.balance = b != nullptr;
+    q.d_weights = d_topk_weights; q.d_loss = d_loss; q.d_loss_ptr = d_loss_ptr;
+    q.d_logits = d_logits; q.d_logits_ld = d_logits_stride;
+    int sms = 0;
+    st = sm_count(&sms);
+    if (st != MM_OK) return st;
+    const int grid = router_grid(a->tokens, sms);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+    MM_ROUTER_LAUNCH(mm::router_backward_kernel);
+    MM_CUDA(cudaGetLastError());
+    return MM_OK;
+}
+
+}  // extern "C"

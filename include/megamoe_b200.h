@@ -246,6 +246,87 @@ int mm_mega_moe_launch_static_scratch(const mm_config_t* cfg, const mm_static_ar
 const char* mm_status_string(int status);
 const char* mm_last_cuda_error(void);
 
+/* ---- Operators around the layer: a block's norms, routing from logits, the balance loss over the experts. The reference has
+ * none of them: a program brings its own between the attention and `mega_moe`, and in training around the router. All calls are
+ * asynchronous on `stream`, allocate nothing and keep nothing from one call for the next; what they need beyond inputs and outputs is a
+ * workspace of the caller's, which two calls may share only if they do not overlap on the GPU. Strides count elements. */
+enum mm_dtype { MM_DTYPE_BF16 = 0, MM_DTYPE_FP16 = 1, MM_DTYPE_FP32 = 2 };
+enum mm_gate_mode { MM_GATE_NONE = 0, MM_GATE_CHANNEL = 1 /* [hidden] */, MM_GATE_TOKEN = 2 /* [tokens], gate_stride apart */, MM_GATE_ELEMENT = 3 /* [tokens][hidden] */ };
+
+/* u = y, or RMS norm of y with post_weight; residual_out = residual + scale * gate * u; normed = RMS norm of that sum (before it is
+ * rounded) with pre_weight. Weights count as weight_offset + w. Rows of hidden <= 8192 channels that lie next to each other. */
+typedef struct mm_block_norm_args {
+    const void* residual;            /* stream_dtype [tokens][hidden] */
+    const void* y;                   /* dtype [tokens][hidden]: the block's output, or NULL: only the norm of `residual` */
+    const void* gate;                /* gate_dtype, by gate_mode; NULL with MM_GATE_NONE */
+    const void* pre_weight;          /* weight_dtype [hidden], or NULL: no norm of the stream, no `normed` */
+    const void* post_weight;         /* weight_dtype [hidden], or NULL: y as it is */
+    void* residual_out;              /* stream_dtype [tokens][hidden]; NULL if y is; may be `residual` itself */
+    void* normed;                    /* dtype [tokens][hidden]; NULL if pre_weight is; may be `y` or `residual` itself */
+    int64_t tokens;
+    int64_t residual_stride, y_stride, gate_stride, residual_out_stride, normed_stride;
+    int32_t hidden;
+    int32_t dtype;                   /* enum mm_dtype, of y and normed */
+    int32_t stream_dtype, weight_dtype, gate_dtype;      /* each `dtype` or MM_DTYPE_FP32 */
+    int32_t gate_mode;
+    float scale, eps, weight_offset; /* eps > 0 */
+} mm_block_norm_args_t;
+
+/* The gradients' side of mm_block_norm_backward. No output shares memory with anything else of the call. */
+typedef struct mm_block_norm_grads {
+    const void* d_residual_out;      /* stream_dtype [tokens][hidden], or NULL: zero */
+    const void* d_normed;            /* dtype [tokens][hidden]; NULL if pre_weight is */
+    void* d_residual;                /* stream_dtype [tokens][hidden] */
+    void* d_y;                       /* dtype [tokens][hidden]; NULL if y is */
+    void* d_gate;                    /* like the gate */
+    void* d_pre_weight;              /* weight_dtype [hidden] */
+    void* d_post_weight;
+    int64_t d_residual_out_stride, d_normed_stride, d_residual_stride, d_y_stride, d_gate_stride;
+    void* workspace;                 /* mm_block_norm_workspace_bytes(), 16-byte aligned; needed for weights' and a channel gate's gradients */
+    int64_t workspace_bytes;
+} mm_block_norm_grads_t;
+
+int mm_block_norm(const mm_block_norm_args_t* args, void* stream);
+int64_t mm_block_norm_workspace_bytes(int64_t tokens, int32_t hidden);
+/* Gradients of mm_block_norm from its inputs (residual_out and normed of `args` are not looked at). Sums over the tokens are always added in the
+ * same order. */
+int mm_block_norm_backward(const mm_block_norm_args_t* args, const mm_block_norm_grads_t* grads, void* stream);
+
+/* A token's scores over the experts: score_mode 0 softmax, 1 sigmoid of its logits, as in mm_frontend_args. A logit that is -inf or NaN
+ * switches the expert off for the token. At most 1024 experts, 32 routes per token, 2^27 tokens. */
+typedef struct mm_router_args {
+    const void* logits;              /* dtype [tokens][num_experts] */
+    int64_t* topk_idx;               /* [tokens][topk]: written by mm_route_tokens, read by the others; outside 0..num_experts-1: no route */
+    float* topk_weights;             /* [tokens][topk]: written by mm_route_tokens, not looked at by the others */
+    int64_t logits_stride;
+    int32_t tokens, num_experts, topk;
+    int32_t dtype, score_mode;
+    float route_scale;               /* the routing weights are scores / sum of the selected scores, times this */
+} mm_router_args_t;
+
+typedef struct mm_balance_args {
+    const int32_t* cu_seqlens;       /* [num_sequences + 1] ascending, sequence s is tokens cu[s] .. cu[s+1]-1; NULL: one sequence of all tokens */
+    int32_t num_sequences;
+    float balance_coef, z_coef;
+    int32_t* counts;                 /* [num_sequences][num_experts] routing slots per expert */
+    int32_t* seq_tokens;             /* [num_sequences] tokens with a route */
+    float* mean_probs;               /* [num_sequences][num_experts] mean probabilities over those tokens */
+    float* losses;                   /* [3]: balance_coef * balance + z_coef * z, balance, z */
+} mm_balance_args_t;
+
+/* The topk experts with the largest keys (logits; or sigmoid + expert_bias, compared as in 64 bits), ties to the lower expert, and their
+ * weights: what mm_fe_forward and mm_frontend_launch work out from hidden states, from logits that the caller has. Tokens whose `valid` is
+ * 0, and slots for which no expert is left, get -1 and weight 0. */
+int mm_route_tokens(const mm_router_args_t* args, const float* expert_bias, const uint8_t* valid, void* stream);
+int64_t mm_balance_workspace_bytes(int32_t num_experts, int32_t num_sequences);
+/* balance = mean over the sequences with tokens of sum_e (E c_e / (topk n)) P_e (c counts, n seq_tokens, P mean_probs), z = mean over those
+ * tokens of log(sum exp logits)^2. Whole-number sums: the same in every call. */
+int mm_balance_loss(const mm_router_args_t* args, const mm_balance_args_t* balance, void* workspace, int64_t workspace_bytes, void* stream);
+/* d_logits (dtype, may be `logits` itself) = gradient of  sum(d_topk_weights * topk_weights) + d_loss * loss.  Either part may be NULL. Of
+ * `balance` counts, seq_tokens, cu_seqlens and the coefficients are read; d_loss comes from d_loss_ptr (device) if that is given. */
+int mm_router_backward(const mm_router_args_t* args, const float* d_topk_weights, const mm_balance_args_t* balance, float d_loss,
+                       const float* d_loss_ptr, void* d_logits, int64_t d_logits_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
