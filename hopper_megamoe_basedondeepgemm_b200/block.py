@@ -113,13 +113,13 @@ def block_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, pre_
     out_ptr = out_ld = normed_ptr = normed_ld = 0
     if y is not None:
         if residual_out is None:
-            residual_out = torch.empty(shape, dtype=residual.dtype, device=residual.device)
+            residual_out = torch.empty_like(residual)
         out_ptr, out_ld = _rows(residual_out, 'residual_out', shape, residual.dtype, device)
     elif residual_out is not None:
         raise RuntimeError('without y the stream stays as it is: no residual_out')
     if pre_weight is not None:
         if normed is None:
-            normed = torch.empty(shape, dtype=dtype, device=residual.device)
+            normed = torch.empty_like(residual) if y is None else torch.empty_like(y)
         normed_ptr, normed_ld = _rows(normed, 'normed', shape, dtype, device)
     elif normed is not None:
         raise RuntimeError('normed needs pre_weight')
@@ -149,18 +149,17 @@ def block_norm_backward(d_residual_out: Optional[torch.Tensor], d_normed: Option
     dtype = y.dtype if y is not None else (d_normed.dtype if d_normed is not None else residual.dtype)
     shape, device, ptrs, lds, types = _block(residual, y, pre_weight, post_weight, gate, dtype)
     tokens, hidden = shape
-    dev = residual.device
     dro_ptr, dro_ld = _rows(d_residual_out, 'd_residual_out', shape, residual.dtype, device) if d_residual_out is not None else (0, 0)
     dn_ptr, dn_ld = _rows(d_normed, 'd_normed', shape, dtype, device) if d_normed is not None else (0, 0)
-    d_residual = torch.empty(shape, dtype=residual.dtype, device=dev)
-    d_y = torch.empty(shape, dtype=dtype, device=dev) if y is not None else None
-    d_gate = torch.empty(gate.shape, dtype=gate.dtype, device=dev) if gate is not None else None
-    d_pre = torch.empty(hidden, dtype=pre_weight.dtype, device=dev) if pre_weight is not None else None
-    d_post = torch.empty(hidden, dtype=post_weight.dtype, device=dev) if post_weight is not None else None
+    d_residual = torch.empty_like(residual)
+    d_y = torch.empty_like(y) if y is not None else None
+    d_gate = torch.empty_like(gate) if gate is not None else None
+    d_pre = torch.empty_like(pre_weight) if pre_weight is not None else None
+    d_post = torch.empty_like(post_weight) if post_weight is not None else None
     ws_ptr = ws_bytes = 0
     if tokens and (d_pre is not None or d_post is not None or types[4] == 1):
         ws_bytes = _lib.load().mm_block_norm_workspace_bytes(tokens, hidden)
-        workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        workspace = residual.new_empty(ws_bytes, dtype=torch.uint8)
         ws_ptr = workspace.data_ptr()
     args = _NORM_ARGS.pack(*ptrs, 0, 0, tokens, *lds, 0, 0, hidden, *types, scale, eps, weight_offset)
     grads = _GRAD_ARGS.pack(dro_ptr, dn_ptr, d_residual.data_ptr(), d_y.data_ptr() if d_y is not None else 0, d_gate.data_ptr() if d_gate is not None else 0,

@@ -4,7 +4,7 @@
 #include <cstring>
 
 #include "../../include/megamoe_b200.h"
-#include "mm_block_norm.cuh"
+#include "mm_block_norm.h"
 #include "mm_router.cuh"
 #include "mm_error.h"
 
@@ -46,13 +46,6 @@ bool writes_safely(const Rows& out, const Rows* others, int n, bool in_place) {
     return true;
 }
 
-struct NormShape {
-    bool vec;
-    int chunks, threads;
-};
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0u; }
-
 int norm_check(const mm_block_norm_args_t* a) {
     if (a == nullptr || a->tokens < 0 || a->tokens > 0x7fffffffll || a->hidden < 1) return MM_ERR_INVALID_ARGUMENT;
     if (!known_dtype(a->dtype) || !known_dtype(a->stream_dtype) || !known_dtype(a->weight_dtype) || !known_dtype(a->gate_dtype)) return MM_ERR_INVALID_ARGUMENT;
@@ -74,15 +67,14 @@ Rows rows_of(const void* p, int64_t ld, int64_t n, int32_t hidden, int dtype) {
     return Rows{p, ld * dtype_bytes(dtype), static_cast<int64_t>(hidden) * dtype_bytes(dtype), n};
 }
 
-NormShape norm_shape(const mm_block_norm_args_t* a, const Rows* rows, int n) {
-    NormShape s;
-    s.vec = a->hidden % 8 == 0;
-    for (int i = 0; i < n; ++i)
-        if (rows[i].p != nullptr && (!aligned16(rows[i].p) || (rows[i].ld & 15) != 0)) s.vec = false;
-    s.chunks = a->hidden <= 8 * mm::kBnMaxThreads ? 1 : 2;
-    const int per = 8 * s.chunks;
-    s.threads = ((a->hidden + per - 1) / per + 31) / 32 * 32;
-    return s;
+// Whether every row starts on 16 bytes, one of 32-bit elements on 32, and is made of whole groups of eight elements.
+bool norm_rows_aligned(int hidden, const Rows* rows, int n) {
+    if (hidden % 8 != 0) return false;
+    for (int i = 0; i < n; ++i) {
+        const int unit = rows[i].width == static_cast<int64_t>(hidden) * 4 ? 32 : 16;
+        if (rows[i].p != nullptr && (reinterpret_cast<uintptr_t>(rows[i].p) % unit != 0 || rows[i].ld % unit != 0)) return false;
+    }
+    return true;
 }
 
 mm::BnParams norm_params(const mm_block_norm_args_t* a) {
@@ -99,25 +91,9 @@ mm::BnParams norm_params(const mm_block_norm_args_t* a) {
     return q;
 }
 
-#define MM_NORM_CASE(X, R, C, V, KERNEL) KERNEL<X, R, C, V><<<grid, s.threads, 0, stream>>>(q)
-#define MM_NORM_SHAPE(X, R, KERNEL)                                                     \
-    do {                                                                                \
-        if (s.vec) { if (s.chunks == 1) MM_NORM_CASE(X, R, 1, true, KERNEL); else MM_NORM_CASE(X, R, 2, true, KERNEL); }   \
-        else { if (s.chunks == 1) MM_NORM_CASE(X, R, 1, false, KERNEL); else MM_NORM_CASE(X, R, 2, false, KERNEL); }       \
-    } while (0)
-#define MM_NORM_LAUNCH(KERNEL)                                                                                              \
-    do {                                                                                                                    \
-        if (a->dtype == MM_DTYPE_FP32) MM_NORM_SHAPE(float, float, KERNEL);                                                 \
-        else if (a->dtype == MM_DTYPE_BF16 && a->stream_dtype == MM_DTYPE_BF16) MM_NORM_SHAPE(__nv_bfloat16, __nv_bfloat16, KERNEL);     \
-        else if (a->dtype == MM_DTYPE_BF16) MM_NORM_SHAPE(__nv_bfloat16, float, KERNEL);                                    \
-        else if (a->stream_dtype == MM_DTYPE_FP16) MM_NORM_SHAPE(__half, __half, KERNEL);                                   \
-        else MM_NORM_SHAPE(__half, float, KERNEL);                                                                          \
-    } while (0)
-
-// Rows that the CTAs of a backward pass share out: each leaves one row of partial sums.
-int64_t norm_backward_ctas(int64_t tokens) {
-    const int64_t most = 296;
-    return tokens < most ? tokens : most;
+int launch_norm(int dtype, const mm::BnParams& q, const mm::BnLaunch& how, cudaStream_t stream) {
+    return dtype == MM_DTYPE_BF16 ? mm::launch_block_norm_bf16(q, how, stream)
+                                  : (dtype == MM_DTYPE_FP16 ? mm::launch_block_norm_fp16(q, how, stream) : mm::launch_block_norm_fp32(q, how, stream));
 }
 
 // ----------------------------------------------------------------------------- router
@@ -207,22 +183,14 @@ int mm_block_norm(const mm_block_norm_args_t* a, void* stream_ptr) {
         !writes_safely(rows[1], rows + 2, 2, true) || !writes_safely(rows[1], rows + 4, 3, false)) return MM_ERR_INVALID_ARGUMENT;
     if (t == 1) for (Rows& r : rows) r.ld = 0;
     if (a->gate_mode == MM_GATE_TOKEN) rows[4].p = nullptr;                 // (read one by one)
-    const NormShape s = norm_shape(a, rows, 7);
-    int sms = 0;
-    st = sm_count(&sms);
-    if (st != MM_OK) return st;
-    const mm::BnParams q = norm_params(a);
-    const int64_t most = static_cast<int64_t>(sms) * (2048 / s.threads < 32 ? 2048 / s.threads : 32);
-    const unsigned grid = static_cast<unsigned>(t < most ? t : most);
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-    MM_NORM_LAUNCH(mm::block_norm_kernel);
-    MM_CUDA(cudaGetLastError());
-    return MM_OK;
+    mm::BnLaunch how = {false, a->stream_dtype == MM_DTYPE_FP32, norm_rows_aligned(a->hidden, rows, 7), 0, 0};
+    st = sm_count(&how.sms);
+    return st != MM_OK ? st : launch_norm(a->dtype, norm_params(a), how, static_cast<cudaStream_t>(stream_ptr));
 }
 
 int64_t mm_block_norm_workspace_bytes(int64_t tokens, int32_t hidden) {
     if (tokens < 0 || hidden < 1 || hidden > mm::kBnMaxHidden) return -1;
-    return norm_backward_ctas(tokens) * hidden * 3 * 4;
+    return mm::bn_backward_ctas(tokens, hidden) * hidden * 2 * 4;
 }
 
 int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_grads_t* g, void* stream_ptr) {
@@ -231,16 +199,16 @@ int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_gr
     if (g == nullptr) return MM_ERR_INVALID_ARGUMENT;
     const bool channel = a->gate_mode == MM_GATE_CHANNEL, element = a->gate_mode == MM_GATE_ELEMENT, token = a->gate_mode == MM_GATE_TOKEN;
     if ((a->pre_weight != nullptr) != (g->d_pre_weight != nullptr) || (a->post_weight != nullptr) != (g->d_post_weight != nullptr)) return MM_ERR_INVALID_ARGUMENT;
-    const int sums = (a->pre_weight != nullptr) + (a->post_weight != nullptr) + channel;
+    const int sums = (a->pre_weight != nullptr) + (a->post_weight != nullptr || channel);
     const int64_t t = a->tokens;
     if (channel && g->d_gate == nullptr) return MM_ERR_INVALID_ARGUMENT;
     if (t > 0) {
         if ((a->pre_weight != nullptr) != (g->d_normed != nullptr) || (a->y != nullptr) != (g->d_y != nullptr) || g->d_residual == nullptr) return MM_ERR_INVALID_ARGUMENT;
         if ((a->pre_weight != nullptr && a->residual == nullptr) || (a->gate != nullptr && g->d_gate == nullptr)) return MM_ERR_INVALID_ARGUMENT;
-        if (sums > 0 && (g->workspace == nullptr || g->workspace_bytes < mm_block_norm_workspace_bytes(t, a->hidden) || !aligned16(g->workspace))) return MM_ERR_INVALID_ARGUMENT;
+        if (sums > 0 && (g->workspace == nullptr || g->workspace_bytes < mm_block_norm_workspace_bytes(t, a->hidden) || (reinterpret_cast<uintptr_t>(g->workspace) & 31u) != 0u)) return MM_ERR_INVALID_ARGUMENT;
     }
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-    const int64_t ctas = norm_backward_ctas(t);
+    const int64_t ctas = mm::bn_backward_ctas(t, a->hidden);
     if (t > 0) {
         const Rows none = {nullptr, 0, 0, 0};
         Rows rows[10] = {rows_of(g->d_residual, g->d_residual_stride, t, a->hidden, a->stream_dtype), rows_of(g->d_y, g->d_y_stride, t, a->hidden, a->dtype),
@@ -256,7 +224,6 @@ int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_gr
         }
         if (t == 1) for (Rows& r : rows) r.ld = 0;
         if (token) rows[2].p = rows[7].p = nullptr;
-        const NormShape s = norm_shape(a, rows, 10);
         mm::BnParams q = norm_params(a);
         q.d_residual_out = g->d_residual_out; q.d_residual_out_ld = g->d_residual_out_stride;
         q.d_normed = g->d_normed; q.d_normed_ld = g->d_normed_stride;
@@ -264,24 +231,21 @@ int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_gr
         q.d_y = g->d_y; q.d_y_ld = g->d_y_stride;
         q.d_gate = g->d_gate; q.d_gate_ld = g->d_gate_stride;
         q.partial = static_cast<float*>(g->workspace);
-        const unsigned grid = static_cast<unsigned>(ctas);
-        MM_NORM_LAUNCH(mm::block_norm_backward_kernel);
-        MM_CUDA(cudaGetLastError());
+        st = launch_norm(a->dtype, q, {true, a->stream_dtype == MM_DTYPE_FP32, norm_rows_aligned(a->hidden, rows, 10), 0, static_cast<int>(ctas)}, stream);
+        if (st != MM_OK) return st;
     }
     if (sums > 0) {
         mm::BnSumsParams q;
         memset(&q, 0, sizeof(q));
         q.partial = static_cast<const float*>(g->workspace);
         q.rows = static_cast<int>(ctas); q.hidden = a->hidden;
-        int n = 0;
-        if (a->pre_weight != nullptr) { q.out[n] = g->d_pre_weight; q.is32[n++] = a->weight_dtype == MM_DTYPE_FP32; }
-        if (a->post_weight != nullptr) { q.out[n] = g->d_post_weight; q.is32[n++] = a->weight_dtype == MM_DTYPE_FP32; }
-        if (channel) { q.out[n] = g->d_gate; q.is32[n++] = a->gate_dtype == MM_DTYPE_FP32; }
-        const dim3 grid((a->hidden + 31) / 32, n);
-        if (a->dtype == MM_DTYPE_FP32) mm::block_norm_sums_kernel<float><<<grid, 256, 0, stream>>>(q);
-        else if (a->dtype == MM_DTYPE_BF16) mm::block_norm_sums_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(q);
-        else mm::block_norm_sums_kernel<__half><<<grid, 256, 0, stream>>>(q);
-        MM_CUDA(cudaGetLastError());
+        q.gate = channel ? a->gate : nullptr; q.post_w = a->post_weight;
+        q.d_pre_w = g->d_pre_weight; q.d_post_w = g->d_post_weight; q.d_gate = channel ? g->d_gate : nullptr;
+        q.weight32 = a->weight_dtype == MM_DTYPE_FP32; q.gate32 = a->gate_dtype == MM_DTYPE_FP32;
+        q.scale = a->scale; q.offset = a->weight_offset;
+        q.sums = sums;
+        return a->dtype == MM_DTYPE_BF16 ? mm::launch_block_norm_sums_bf16(q, stream)
+                                         : (a->dtype == MM_DTYPE_FP16 ? mm::launch_block_norm_sums_fp16(q, stream) : mm::launch_block_norm_sums_fp32(q, stream));
     }
     return MM_OK;
 }

@@ -11,30 +11,28 @@
 //   dv = scale * dr,  dg = dv u (summed over what the gate is broadcast to),  du = dv g
 //   dy = i1 (du w1 - n1 mean(du w1 n1)),  or du       dw_post = sum over the rows of du n1
 //
-// A row belongs to one CTA, which holds it in registers: eight neighbouring elements per thread and chunk.
+// In the backward pass everything that goes through y is written with the coefficient a = scale * (gate of the channel) * (offset + w_post) and
+// v = y i1 a (times the token's or element's gate): then the sum that the norm of y needs is sum of v dr, which with
+// dr = d_r' + i2 dh w2 - k r',  k = i2^3 / H * sum of dh w2 r',  falls apart into sums of v d_r', v dh w2 and v r'. They are taken together with
+// those of the norm of r', so that a row needs one exchange between its threads. The gradients of a channel's gate and of w_post are one sum over
+// the rows, of dr n1 (token's or element's gate), times the other's factor.
+//
+// A row belongs to one CTA, eight channels to a thread, up to 4096 channels. Bound by memory: the bytes of the rows, in and out. CTAs stay and walk over the rows; a
+// thread asks for its part of the next row before it works on the one it has, and while a row's sums are exchanged, the sum of squares of the next row's
+// y goes with them: one barrier a row.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
+#include <type_traits>
+
+#include "../../include/megamoe_b200.h"
+#include "mm_block_norm.h"
+#include "mm_error.h"
 
 namespace mm {
-
-constexpr int kBnMaxHidden = 8192;
-constexpr int kBnMaxThreads = 512;
-enum BnGate { kBnGateNone = 0, kBnGateChannel = 1, kBnGateToken = 2, kBnGateElement = 3 };
-
-struct BnParams {
-    const void *residual, *y, *gate, *pre_w, *post_w;        // y, gate and either weight may be missing
-    void *residual_out, *normed;
-    const void *d_residual_out, *d_normed;                   // backward
-    void *d_residual, *d_y, *d_gate;
-    float* partial;                                          // backward: [sums][CTAs][hidden]
-    long long tokens;
-    long long residual_ld, y_ld, gate_ld, residual_out_ld, normed_ld, d_residual_out_ld, d_normed_ld, d_residual_ld, d_y_ld, d_gate_ld;
-    int hidden, gate_mode, weight32, gate32;
-    float scale, eps, offset;
-};
 
 template <typename T> __device__ __forceinline__ float bn_float(T v);
 template <> __device__ __forceinline__ float bn_float<float>(float v) { return v; }
@@ -45,119 +43,117 @@ template <> __device__ __forceinline__ float bn_round<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 bn_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half bn_round<__half>(float v) { return __float2half_rn(v); }
 
-// Eight elements of a row as this thread sees them in chunk c. Rows that start on 16 bytes and hold a multiple of eight elements (`Vec`): eight
-// neighbours, in 16 B accesses. Others: elements a CTA's width apart, one by one, so that neighbouring threads still read neighbouring elements.
-template <bool Vec>
-__device__ __forceinline__ int bn_at(int c, int j) {
-    return Vec ? (c * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8 + j
-               : (c * 8 + j) * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x);
-}
+// Eight elements of a row, a CTA's width apart, so that neighbouring threads read neighbouring elements wherever the row starts.
+__device__ __forceinline__ int bn_at(int c, int j) { return (c * 8 + j) * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x); }
 
-template <typename T, bool Vec>
+template <typename T>
 __device__ __forceinline__ void bn_load(const T* row, int hidden, int c, float (&v)[8]) {
-    if constexpr (Vec) {
-        const int at = bn_at<true>(c, 0);
-        alignas(16) T e[8];
-        if (at < hidden) {
-            #pragma unroll
-            for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q)
-                reinterpret_cast<uint4*>(e)[q] = *reinterpret_cast<const uint4*>(row + at + q * (16 / static_cast<int>(sizeof(T))));
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = bn_float<T>(e[j]);
-        } else {
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = 0.f;
-        }
-    } else {
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int at = bn_at<false>(c, j);
-            v[j] = at < hidden ? bn_float<T>(row[at]) : 0.f;
-        }
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int at = bn_at(c, j);
+        v[j] = at < hidden ? bn_float<T>(row[at]) : 0.f;
     }
 }
 
-template <typename T, bool Vec>
+template <typename T>
 __device__ __forceinline__ void bn_store(T* row, int hidden, int c, const float (&v)[8]) {
-    if constexpr (Vec) {
-        const int at = bn_at<true>(c, 0);
-        if (at >= hidden) return;
-        alignas(16) T e[8];
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = bn_round<T>(v[j]);
-        #pragma unroll
-        for (int q = 0; q < static_cast<int>(sizeof(T)) / 2; ++q)
-            *reinterpret_cast<uint4*>(row + at + q * (16 / static_cast<int>(sizeof(T)))) = reinterpret_cast<const uint4*>(e)[q];
-    } else {
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int at = bn_at<false>(c, j);
-            if (at < hidden) row[at] = bn_round<T>(v[j]);
-        }
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int at = bn_at(c, j);
+        if (at < hidden) row[at] = bn_round<T>(v[j]);
     }
 }
 
 // a weight or gate row that is 32 bits wide or of the activations' type
-template <typename X, bool Vec>
+template <typename X>
 __device__ __forceinline__ void bn_load_either(const void* row, int is32, long long at_row, int hidden, int c, float (&v)[8]) {
-    if (is32) bn_load<float, Vec>(static_cast<const float*>(row) + at_row, hidden, c, v);
-    else bn_load<X, Vec>(static_cast<const X*>(row) + at_row, hidden, c, v);
+    if (is32) bn_load<float>(static_cast<const float*>(row) + at_row, hidden, c, v);
+    else bn_load<X>(static_cast<const X*>(row) + at_row, hidden, c, v);
 }
 
-// Sums of N values over the CTA, the same in every thread: shuffles, then each warp's sums through shared memory. `part` is used by turns
-// (`turn`), so that a sum needs one barrier: the next one's values go where no thread can still be reading.
+template <typename X>
+__device__ __forceinline__ float bn_token_gate(const BnParams& q, long long row) {
+    return q.gate32 ? static_cast<const float*>(q.gate)[row * q.gate_ld] : bn_float<X>(static_cast<const X*>(q.gate)[row * q.gate_ld]);
+}
+
+// Sums of N values (a power of two) over the CTA, the same in every thread. In a warp the values are dealt out while they are added: each step
+// halves both the values of a lane and the lanes of a value. Each warp's sums go through shared memory (`part`, all zero at first, of which a turn
+// is used at a time: the next sums' values go where no thread can still be reading, so one barrier does), and four lanes add up one value.
+constexpr int kBnSumWarps = kBnMaxThreads / 32;
 template <int N>
-__device__ __forceinline__ void bn_sum(float (&v)[N], float (*part)[kBnMaxThreads / 32][4], int& turn) {
+__device__ __forceinline__ void bn_sum(float (&v)[N], float (*part)[8][kBnSumWarps], int& turn) {
+    const uint32_t lane = threadIdx.x & 31u;
+    float s[N];
     #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
-    }
-    const int warps = blockDim.x >> 5;
-    if (warps == 1) return;
-    float (*p)[4] = part[turn];
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0) {
-        #pragma unroll
-        for (int n = 0; n < N; ++n) p[threadIdx.x >> 5][n] = v[n];
-    }
-    __syncthreads();
+    for (int n = 0; n < N; ++n) s[n] = v[n];
+    int o = 16;
     #pragma unroll
-    for (int n = 0; n < N; ++n) v[n] = 0.f;
-    for (int w = 0; w < warps; ++w) {
+    for (int half = N / 2; half > 0; half /= 2, o /= 2) {
         #pragma unroll
-        for (int n = 0; n < N; ++n) v[n] += p[w][n];
+        for (int n = 0; n < half; ++n) {
+            const bool up = (lane & o) != 0u;
+            const float keep = up ? s[n + half] : s[n], send = up ? s[n] : s[n + half];
+            s[n] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    }
+    #pragma unroll
+    for (; o > 0; o /= 2) s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+    const uint32_t mine = lane * N / 32;                     // the value that this lane has the warp's sum of
+    if (blockDim.x > 32) {
+        float (*p)[kBnSumWarps] = part[turn];
+        turn ^= 1;
+        if (lane % (32 / N) == 0) p[mine][threadIdx.x >> 5] = s[0];
+        __syncthreads();
+        const float4 w = *reinterpret_cast<const float4*>(&p[(lane >> 2) % N][(lane & 3u) * 4u]);
+        float t = (w.x + w.y) + (w.z + w.w);
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        #pragma unroll
+        for (int n = 0; n < N; ++n) v[n] = __shfl_sync(0xffffffffu, t, n * 4);
+    } else {
+        #pragma unroll
+        for (int n = 0; n < N; ++n) v[n] = __shfl_sync(0xffffffffu, s[0], n * (32 / N));
+    }
+}
+static_assert(kBnSumWarps == 16, "four lanes read four warps' sums each");
+
+__device__ __forceinline__ void bn_sum_init(float (*part)[8][kBnSumWarps]) {
+    if (blockDim.x > 32) {
+        for (int i = threadIdx.x; i < 2 * 8 * kBnSumWarps; i += blockDim.x) (&part[0][0][0])[i] = 0.f;
+        __syncthreads();
     }
 }
 
-// scale * gate of a chunk
-template <typename X, bool Vec>
+// ----------------------------------------------------------------------------- rows of more than 4096 channels
+// Sixteen channels a thread, one by one, a row at a time: as it comes, without anything in flight ahead (half the memory's rate; the layer's rows end at 4096).
+// gate of a chunk
+template <typename X>
 __device__ __forceinline__ void bn_gate(const BnParams& q, long long row, int c, float (&g)[8]) {
     if (q.gate_mode == kBnGateNone || q.gate_mode == kBnGateToken) {
-        float s = 1.f;
-        if (q.gate_mode == kBnGateToken)
-            s = q.gate32 ? static_cast<const float*>(q.gate)[row * q.gate_ld] : bn_float<X>(static_cast<const X*>(q.gate)[row * q.gate_ld]);
+        const float s = q.gate_mode == kBnGateToken ? bn_token_gate<X>(q, row) : 1.f;
         #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] = s;
     } else {
-        bn_load_either<X, Vec>(q.gate, q.gate32, q.gate_mode == kBnGateElement ? row * q.gate_ld : 0, q.hidden, c, g);
+        bn_load_either<X>(q.gate, q.gate32, q.gate_mode == kBnGateElement ? row * q.gate_ld : 0, q.hidden, c, g);
     }
 }
 
-template <typename X, typename R, int C, bool Vec>
-__global__ void __launch_bounds__(kBnMaxThreads) block_norm_kernel(const BnParams q) {
-    __shared__ float part[2][kBnMaxThreads / 32][4];
+template <typename X, typename R>
+__global__ void __launch_bounds__(kBnMaxThreads) block_norm_wide_kernel(const BnParams q) {
+    __shared__ __align__(16) float part[2][8][kBnSumWarps];
+    constexpr int C = 2;
+    bn_sum_init(part);
     int turn = 0;
     const float inv_h = 1.f / static_cast<float>(q.hidden);
     for (long long row = blockIdx.x; row < q.tokens; row += gridDim.x) {
         float r[C][8], u[C][8];
         #pragma unroll
-        for (int c = 0; c < C; ++c) bn_load<R, Vec>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, c, r[c]);
+        for (int c = 0; c < C; ++c) bn_load<R>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, c, r[c]);
         if (q.y != nullptr) {
             float sum[1] = {0.f};
             #pragma unroll
             for (int c = 0; c < C; ++c) {
-                bn_load<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, c, u[c]);
+                bn_load<X>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, c, u[c]);
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) sum[0] += u[c][j] * u[c][j];
             }
@@ -169,15 +165,15 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_kernel(const BnParam
             #pragma unroll
             for (int c = 0; c < C; ++c) {
                 float g[8], w[8];
-                bn_gate<X, Vec>(q, row, c, g);
+                bn_gate<X>(q, row, c, g);
                 if (q.post_w != nullptr) {
-                    bn_load_either<X, Vec>(q.post_w, q.weight32, 0, q.hidden, c, w);
+                    bn_load_either<X>(q.post_w, q.weight32, 0, q.hidden, c, w);
                     #pragma unroll
                     for (int j = 0; j < 8; ++j) u[c][j] = u[c][j] * i1 * (w[j] + q.offset);
                 }
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[c][j] += q.scale * (u[c][j] * g[j]);
-                bn_store<R, Vec>(static_cast<R*>(q.residual_out) + row * q.residual_out_ld, q.hidden, c, r[c]);
+                bn_store<R>(static_cast<R*>(q.residual_out) + row * q.residual_out_ld, q.hidden, c, r[c]);
             }
         }
         if (q.pre_w != nullptr) {
@@ -192,31 +188,33 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_kernel(const BnParam
             #pragma unroll
             for (int c = 0; c < C; ++c) {
                 float w[8];
-                bn_load_either<X, Vec>(q.pre_w, q.weight32, 0, q.hidden, c, w);
+                bn_load_either<X>(q.pre_w, q.weight32, 0, q.hidden, c, w);
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[c][j] = r[c][j] * i2 * (w[j] + q.offset);
-                bn_store<X, Vec>(static_cast<X*>(q.normed) + row * q.normed_ld, q.hidden, c, r[c]);
+                bn_store<X>(static_cast<X*>(q.normed) + row * q.normed_ld, q.hidden, c, r[c]);
             }
         }
     }
 }
 
-// Rows are dealt to the CTAs in turn; a thread sums the gradients of its channels' weights over the CTA's rows and leaves them in `partial`,
-// which `block_norm_sums_kernel` adds up: always in the same order.
-template <typename X, typename R, int C, bool Vec>
-__global__ void __launch_bounds__(kBnMaxThreads) block_norm_backward_kernel(const BnParams q) {
-    __shared__ float part[2][kBnMaxThreads / 32][4];
+// Rows are dealt to the CTAs in turn; a thread sums over the CTA's rows what the gradients of its channels' weights are made of and leaves it in
+// `partial`, which `block_norm_sums_kernel` adds up: always in the same order.
+template <typename X, typename R>
+__global__ void __launch_bounds__(kBnMaxThreads) block_norm_backward_wide_kernel(const BnParams q) {
+    __shared__ __align__(16) float part[2][8][kBnSumWarps];
+    constexpr int C = 2;
+    bn_sum_init(part);
     int turn = 0;
     const float inv_h = 1.f / static_cast<float>(q.hidden);
     const bool post = q.post_w != nullptr, pre = q.pre_w != nullptr;
-    float acc_pre[C][8] = {}, acc_post[C][8] = {}, acc_gate[C][8] = {};
+    float acc_pre[C][8] = {}, acc_y[C][8] = {};
     for (long long row = blockIdx.x; row < q.tokens; row += gridDim.x) {
         float y[C][8], i1 = 1.f;
         if (q.y != nullptr) {
             float sum[1] = {0.f};
             #pragma unroll
             for (int c = 0; c < C; ++c) {
-                bn_load<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, c, y[c]);
+                bn_load<X>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, c, y[c]);
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) sum[0] += y[c][j] * y[c][j];
             }
@@ -229,7 +227,7 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_backward_kernel(cons
         #pragma unroll
         for (int c = 0; c < C; ++c) {
             if (q.d_residual_out != nullptr) {
-                bn_load<R, Vec>(static_cast<const R*>(q.d_residual_out) + row * q.d_residual_out_ld, q.hidden, c, d[c]);
+                bn_load<R>(static_cast<const R*>(q.d_residual_out) + row * q.d_residual_out_ld, q.hidden, c, d[c]);
             } else {
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) d[c][j] = 0.f;
@@ -239,14 +237,14 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_backward_kernel(cons
             float n[C][8], dh[C][8], sum[2] = {0.f, 0.f};
             #pragma unroll
             for (int c = 0; c < C; ++c) {
-                bn_load<R, Vec>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, c, n[c]);
-                bn_load<X, Vec>(static_cast<const X*>(q.d_normed) + row * q.d_normed_ld, q.hidden, c, dh[c]);
+                bn_load<R>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, c, n[c]);
+                bn_load<X>(static_cast<const X*>(q.d_normed) + row * q.d_normed_ld, q.hidden, c, dh[c]);
                 float w[8];
                 if (q.y != nullptr) {
                     float g[8];
-                    bn_gate<X, Vec>(q, row, c, g);
+                    bn_gate<X>(q, row, c, g);
                     if (post) {
-                        bn_load_either<X, Vec>(q.post_w, q.weight32, 0, q.hidden, c, w);
+                        bn_load_either<X>(q.post_w, q.weight32, 0, q.hidden, c, w);
                         #pragma unroll
                         for (int j = 0; j < 8; ++j) n[c][j] += q.scale * (y[c][j] * i1 * (w[j] + q.offset) * g[j]);
                     } else {
@@ -254,7 +252,7 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_backward_kernel(cons
                         for (int j = 0; j < 8; ++j) n[c][j] += q.scale * (y[c][j] * g[j]);
                     }
                 }
-                bn_load_either<X, Vec>(q.pre_w, q.weight32, 0, q.hidden, c, w);
+                bn_load_either<X>(q.pre_w, q.weight32, 0, q.hidden, c, w);
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     sum[0] += n[c][j] * n[c][j];
@@ -266,7 +264,7 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_backward_kernel(cons
             #pragma unroll
             for (int c = 0; c < C; ++c) {
                 float w[8];
-                bn_load_either<X, Vec>(q.pre_w, q.weight32, 0, q.hidden, c, w);
+                bn_load_either<X>(q.pre_w, q.weight32, 0, q.hidden, c, w);
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float n2 = n[c][j] * i2;
@@ -275,34 +273,27 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_backward_kernel(cons
                 }
             }
         }
-        if (q.d_residual != nullptr) {
-            #pragma unroll
-            for (int c = 0; c < C; ++c) bn_store<R, Vec>(static_cast<R*>(q.d_residual) + row * q.d_residual_ld, q.hidden, c, d[c]);
-        }
+        #pragma unroll
+        for (int c = 0; c < C; ++c) bn_store<R>(static_cast<R*>(q.d_residual) + row * q.d_residual_ld, q.hidden, c, d[c]);
         if (q.y == nullptr) continue;
         float sum[2] = {0.f, 0.f};
         #pragma unroll
         for (int c = 0; c < C; ++c) {
-            float g[8], w[8];
-            bn_gate<X, Vec>(q, row, c, g);
-            if (post) bn_load_either<X, Vec>(q.post_w, q.weight32, 0, q.hidden, c, w);
-            float dg[8];
+            float g[8], w[8], dg[8];
+            bn_gate<X>(q, row, c, g);
+            if (post) bn_load_either<X>(q.post_w, q.weight32, 0, q.hidden, c, w);
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float n1 = y[c][j] * i1, w1 = post ? w[j] + q.offset : 1.f, dv = q.scale * d[c][j];
+                acc_y[c][j] += d[c][j] * n1 * (q.gate_mode == kBnGateChannel ? 1.f : g[j]);
                 dg[j] = dv * (n1 * w1);
-                const float du = dv * g[j];
-                acc_post[c][j] += du * n1;
-                d[c][j] = du * w1;
+                d[c][j] = dv * g[j] * w1;
                 sum[0] += d[c][j] * n1;
                 sum[1] += dg[j];
             }
-            if (q.gate_mode == kBnGateChannel) {
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) acc_gate[c][j] += dg[j];
-            } else if (q.gate_mode == kBnGateElement) {
-                if (q.gate32) bn_store<float, Vec>(static_cast<float*>(q.d_gate) + row * q.d_gate_ld, q.hidden, c, dg);
-                else bn_store<X, Vec>(static_cast<X*>(q.d_gate) + row * q.d_gate_ld, q.hidden, c, dg);
+            if (q.gate_mode == kBnGateElement) {
+                if (q.gate32) bn_store<float>(static_cast<float*>(q.d_gate) + row * q.d_gate_ld, q.hidden, c, dg);
+                else bn_store<X>(static_cast<X*>(q.d_gate) + row * q.d_gate_ld, q.hidden, c, dg);
             }
         }
         if (post || q.gate_mode == kBnGateToken) bn_sum<2>(sum, part, turn);
@@ -317,44 +308,545 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_backward_kernel(cons
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) d[c][j] = i1 * (d[c][j] - y[c][j] * i1 * mean);
             }
-            bn_store<X, Vec>(static_cast<X*>(q.d_y) + row * q.d_y_ld, q.hidden, c, d[c]);
+            bn_store<X>(static_cast<X*>(q.d_y) + row * q.d_y_ld, q.hidden, c, d[c]);
         }
     }
     float* p = q.partial + static_cast<long long>(blockIdx.x) * q.hidden;
     const long long stride = static_cast<long long>(gridDim.x) * q.hidden;
+    const bool sum_y = post || q.gate_mode == kBnGateChannel;
     #pragma unroll
     for (int c = 0; c < C; ++c) {
-        float* to = p;
-        if (pre) { bn_store<float, Vec>(to, q.hidden, c, acc_pre[c]); to += stride; }
-        if (post) { bn_store<float, Vec>(to, q.hidden, c, acc_post[c]); to += stride; }
-        if (q.gate_mode == kBnGateChannel) bn_store<float, Vec>(to, q.hidden, c, acc_gate[c]);
+        if (pre) bn_store<float>(p, q.hidden, c, acc_pre[c]);
+        if (sum_y) bn_store<float>(pre ? p + stride : p, q.hidden, c, acc_y[c]);
     }
 }
 
-struct BnSumsParams {
-    const float* partial;                                    // [sums][rows][hidden]
-    void* out[3];
-    int is32[3];
-    int rows, hidden;
-};
+// ----------------------------------------------------------------------------- rows of up to 4096 channels
+// Two 32-bit numbers in one register pair: one instruction adds or multiplies both.
+__device__ __forceinline__ unsigned long long bn_bits(float2 v) { return *reinterpret_cast<unsigned long long*>(&v); }
+__device__ __forceinline__ float2 bn_pair(unsigned long long b) { return *reinterpret_cast<float2*>(&b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bn_bits(a)), "l"(bn_bits(b)), "l"(bn_bits(c)));
+    return bn_pair(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bn_bits(a)), "l"(bn_bits(b)));
+    return bn_pair(d);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// Column sums: a block takes 32 channels of one of the (up to three) gradients, a warp every eighth row; added up in shared memory in order.
+// Eight elements as they lie in memory. Loads of them are written down where they are to be issued (volatile), a row ahead of their use.
+template <typename T> struct Bn8 { uint32_t w[sizeof(T) * 2]; };
+
+__device__ __forceinline__ void bn_unpack(const Bn8<float>& r, float2 (&v)[4]) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+}
+__device__ __forceinline__ void bn_unpack(const Bn8<__nv_bfloat16>& r, float2 (&v)[4]) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(r.w[i] << 16), __uint_as_float(r.w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void bn_unpack(const Bn8<__half>& r, float2 (&v)[4]) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+}
+__device__ __forceinline__ Bn8<float> bn_pack(const float2 (&v)[4], float) {
+    Bn8<float> r;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) { r.w[2 * i] = __float_as_uint(v[i].x); r.w[2 * i + 1] = __float_as_uint(v[i].y); }
+    return r;
+}
+__device__ __forceinline__ Bn8<__nv_bfloat16> bn_pack(const float2 (&v)[4], __nv_bfloat16) {
+    Bn8<__nv_bfloat16> r;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) { const __nv_bfloat162 p = __float22bfloat162_rn(v[i]); r.w[i] = *reinterpret_cast<const uint32_t*>(&p); }
+    return r;
+}
+__device__ __forceinline__ Bn8<__half> bn_pack(const float2 (&v)[4], __half) {
+    Bn8<__half> r;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) { const __half2 p = __float22half2_rn(v[i]); r.w[i] = *reinterpret_cast<const uint32_t*>(&p); }
+    return r;
+}
+
+// The eight channels of this thread in a row. `Vec`: eight neighbours, in one access (of 32 bytes for 32-bit elements: two of 16 would each move half of
+// every 32-byte sector). Otherwise channels a CTA's width apart, one by one: neighbouring threads still read neighbours.
+template <typename T, bool Vec>
+__device__ __forceinline__ void bn_fetch(const T* row, int hidden, Bn8<T>& r) {
+    if constexpr (Vec) {
+        const T* p = row + static_cast<int>(threadIdx.x) * 8;
+        if constexpr (sizeof(T) == 4)
+            asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]),
+                         "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7]) : "l"(p) : "memory");
+        else
+            asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "l"(p) : "memory");
+    } else {
+        const int at = static_cast<int>(threadIdx.x), width = static_cast<int>(blockDim.x);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int a = at + 2 * i * width, b = a + width;
+            if constexpr (sizeof(T) == 4) {
+                r.w[2 * i] = a < hidden ? reinterpret_cast<const uint32_t*>(row)[a] : 0u;
+                r.w[2 * i + 1] = b < hidden ? reinterpret_cast<const uint32_t*>(row)[b] : 0u;
+            } else {
+                const uint32_t lo = a < hidden ? reinterpret_cast<const uint16_t*>(row)[a] : 0u, hi = b < hidden ? reinterpret_cast<const uint16_t*>(row)[b] : 0u;
+                r.w[i] = lo | hi << 16;
+            }
+        }
+    }
+}
+template <typename T, bool Vec>
+__device__ __forceinline__ void bn_put(T* row, int hidden, const float2 (&v)[4]) {
+    const Bn8<T> r = bn_pack(v, T());
+    if constexpr (Vec) {
+        T* p = row + static_cast<int>(threadIdx.x) * 8;
+        if constexpr (sizeof(T) == 4)
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]),
+                         "r"(r.w[7]) : "memory");
+        else
+            asm volatile("st.global.v4.b32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]) : "memory");
+    } else {
+        const int at = static_cast<int>(threadIdx.x), width = static_cast<int>(blockDim.x);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int a = at + 2 * i * width, b = a + width;
+            if constexpr (sizeof(T) == 4) {
+                if (a < hidden) reinterpret_cast<uint32_t*>(row)[a] = r.w[2 * i];
+                if (b < hidden) reinterpret_cast<uint32_t*>(row)[b] = r.w[2 * i + 1];
+            } else {
+                if (a < hidden) reinterpret_cast<uint16_t*>(row)[a] = static_cast<uint16_t>(r.w[i]);
+                if (b < hidden) reinterpret_cast<uint16_t*>(row)[b] = static_cast<uint16_t>(r.w[i] >> 16);
+            }
+        }
+    }
+}
+
+// weights and gates of the channels
+template <typename X, bool Vec>
+__device__ __forceinline__ void bn_weight(const void* w, int is32, int hidden, float2 (&v)[4]) {
+    if (is32) { Bn8<float> r; bn_fetch<float, Vec>(static_cast<const float*>(w), hidden, r); bn_unpack(r, v); }
+    else { Bn8<X> r; bn_fetch<X, Vec>(static_cast<const X*>(w), hidden, r); bn_unpack(r, v); }
+}
+// scale * (channel's gate) * (offset + w_post): the factor of y
+template <typename X, bool Vec>
+__device__ __forceinline__ void bn_y_factor(const BnParams& q, float2 (&a)[4]) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = both(q.scale);
+    if (q.post_w != nullptr) {
+        float2 w[4];
+        bn_weight<X, Vec>(q.post_w, q.weight32, q.hidden, w);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = make_float2(q.scale * (w[i].x + q.offset), q.scale * (w[i].y + q.offset));
+    }
+    if (q.gate_mode == kBnGateChannel) {
+        float2 g[4];
+        bn_weight<X, Vec>(q.gate, q.gate32, q.hidden, g);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = mul2(a[i], g[i]);
+    }
+}
+template <typename X, bool Vec>
+__device__ __forceinline__ void bn_pre_factor(const BnParams& q, float2 (&w)[4]) {
+    bn_weight<X, Vec>(q.pre_w, q.weight32, q.hidden, w);
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = make_float2(w[i].x + q.offset, w[i].y + q.offset);
+}
+
+// A token's gate is asked for a row ahead as it lies in memory, and turned into a number when its row comes: a conversion at the load would wait for it.
+template <typename X>
+__device__ __forceinline__ uint32_t bn_gate_bits(const BnParams& q, long long row) {
+    if (sizeof(X) == 4 || q.gate32) return static_cast<const uint32_t*>(q.gate)[row * q.gate_ld];
+    return static_cast<const uint16_t*>(q.gate)[row * q.gate_ld];
+}
+template <typename X>
+__device__ __forceinline__ float bn_gate_value(const BnParams& q, uint32_t bits) {
+    if (sizeof(X) == 4 || q.gate32) return __uint_as_float(bits);
+    const uint16_t half = static_cast<uint16_t>(bits);
+    return bn_float<X>(*reinterpret_cast<const X*>(&half));
+}
+// an element's gate: of the activations' type or 32 bits, held in room for the latter
+template <typename X, bool Vec>
+__device__ __forceinline__ void bn_fetch_gate(const BnParams& q, long long row, Bn8<float>& r) {
+    if (sizeof(X) == 4 || q.gate32) {
+        bn_fetch<float, Vec>(static_cast<const float*>(q.gate) + row * q.gate_ld, q.hidden, r);
+    } else {
+        Bn8<X> h;
+        bn_fetch<X, Vec>(static_cast<const X*>(q.gate) + row * q.gate_ld, q.hidden, h);
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i] = h.w[i];
+    }
+}
+template <typename X>
+__device__ __forceinline__ void bn_unpack_gate(const BnParams& q, const Bn8<float>& r, float2 (&g)[4]) {
+    if (sizeof(X) == 4 || q.gate32) {
+        bn_unpack(r, g);
+    } else {
+        Bn8<X> h;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) h.w[i] = r.w[i];
+        bn_unpack(h, g);
+    }
+}
+
+__device__ __forceinline__ float bn_square(const float2 (&v)[4]) {
+    float2 s = mul2(v[0], v[0]);
+    #pragma unroll
+    for (int i = 1; i < 4; ++i) s = fma2(v[i], v[i], s);
+    return s.x + s.y;
+}
+template <typename T> __device__ __forceinline__ float bn_square(const Bn8<T>& r) { float2 v[4]; bn_unpack(r, v); return bn_square(v); }
+template <typename T> __device__ __forceinline__ void bn_clear(Bn8<T>& r) {
+    #pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) * 2; ++i) r.w[i] = 0u;
+}
+
+// What there is in a call, as far as it shapes the loop over the rows.
+enum BnKind { kBnPlain = 0 /* no gate, or one that is part of y's factor */, kBnToken = 1, kBnElement = 2, kBnStream = 3 /* no y */ };
+
+// 64 registers a thread, so two CTAs of 512 threads an SM. 16384 x 4096, 32-bit stream, both norms, channel gate: 130 us (6.2 TB/s); of 8192 x 3072 in bf16 40 us.
+// (One CTA of twice the registers per SM 168 us; sixteen channels a thread 134; rows copied ahead into shared memory by cp.async 160.)
+template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec>
+__global__ void __launch_bounds__(kBnMaxThreads, 2) block_norm_kernel(const BnParams q) {
+    __shared__ __align__(16) float part[2][8][kBnSumWarps];
+    const float inv_h = 1.f / static_cast<float>(q.hidden);
+    const int step = gridDim.x, tokens = static_cast<int>(q.tokens);
+    const bool on = !Vec || static_cast<int>(threadIdx.x) * 8 < q.hidden;
+    Bn8<R> rr;
+    Bn8<X> ry;
+    Bn8<float> rg;
+    float2 a[4], w[4];
+    uint32_t gate_bits = 0u;
+    bn_clear(rr);
+    bn_clear(ry);
+    bn_clear(rg);
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = w[i] = both(0.f);
+    auto fetch = [&](long long row) {
+        if (on) {
+            if (Kind != kBnStream) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry);
+            bn_fetch<R, Vec>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, rr);
+            if (Kind == kBnElement) bn_fetch_gate<X, Vec>(q, row, rg);
+        }
+        if (Kind == kBnToken) gate_bits = bn_gate_bits<X>(q, row);
+    };
+    int row = blockIdx.x;
+    fetch(row);
+    if (on) {
+        if (Kind != kBnStream) bn_y_factor<X, Vec>(q, a);
+        if (Pre) bn_pre_factor<X, Vec>(q, w);
+    }
+    bn_sum_init(part);
+    int turn = 0;
+    float i1 = 1.f;
+    if (Post) {
+        float sum[1] = {bn_square(ry)};
+        bn_sum<1>(sum, part, turn);
+        i1 = rsqrtf(sum[0] * inv_h + q.eps);
+    }
+    while (true) {
+        const bool more = row + step < tokens;
+        float2 r[4], v[4], g[4];
+        bn_unpack(rr, r);
+        if (Kind != kBnStream) bn_unpack(ry, v);
+        if (Kind == kBnElement) bn_unpack_gate<X>(q, rg, g);
+        const float f = Kind == kBnToken ? i1 * bn_gate_value<X>(q, gate_bits) : i1;
+        if (more) fetch(row + step);
+        if (Kind != kBnStream) {
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (Post || Kind == kBnToken) v[i] = mul2(v[i], both(f));
+                if (Kind == kBnElement) v[i] = mul2(v[i], g[i]);
+                r[i] = fma2(v[i], a[i], r[i]);
+            }
+            if (on) bn_put<R, Vec>(static_cast<R*>(q.residual_out) + row * q.residual_out_ld, q.hidden, r);
+        }
+        if (Pre) {
+            // the sum of the next row's squares goes with this row's
+            float sum[2] = {bn_square(r), 0.f};
+            if (Post) {
+                sum[1] = bn_square(ry);
+                bn_sum<2>(sum, part, turn);
+                i1 = rsqrtf(sum[1] * inv_h + q.eps);
+            } else {
+                float only[1] = {sum[0]};
+                bn_sum<1>(only, part, turn);
+                sum[0] = only[0];
+            }
+            const float2 i2 = both(rsqrtf(sum[0] * inv_h + q.eps));
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = mul2(mul2(r[i], i2), w[i]);
+            if (on) bn_put<X, Vec>(static_cast<X*>(q.normed) + row * q.normed_ld, q.hidden, r);
+        } else if (Post) {
+            float sum[1] = {bn_square(ry)};
+            bn_sum<1>(sum, part, turn);
+            i1 = rsqrtf(sum[0] * inv_h + q.eps);
+        }
+        if (!more) return;
+        row += step;
+    }
+}
+
+// Rows are dealt to the CTAs in turn; a thread sums what the gradients of its channels' weights are made of over the CTA's rows and leaves it in `partial`, which
+// `block_norm_sums_kernel` adds up: always in the same order. Registers bound how much of a row's traffic is in flight: 128 a thread, a row being worked on and a row on its
+// way, y two rows ahead (its sum of squares goes with the exchange of the row before). 8192 x 4096, 32-bit stream, both norms: 97 us (6.2 TB/s), 8192 x 3072
+// in bf16 66 us (4.6). (y one row ahead 131 and 101 us; weights or the sums in shared memory, or more threads with fewer registers, no better.)
+template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec>
+__global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_backward_kernel(const BnParams q) {
+    __shared__ __align__(16) float part[2][8][kBnSumWarps];
+    constexpr bool kY = Kind != kBnStream, kSumV = Post || Kind == kBnToken;
+    const float inv_h = 1.f / static_cast<float>(q.hidden);
+    const int step = gridDim.x, tokens = static_cast<int>(q.tokens);
+    const bool on = !Vec || static_cast<int>(threadIdx.x) * 8 < q.hidden, sum_y = Post || q.gate_mode == kBnGateChannel, has_d = q.d_residual_out != nullptr;
+    Bn8<R> rd, rr;
+    Bn8<X> ry, rh, ry_next;
+    Bn8<float> rg;
+    float2 a[4], w[4], acc_pre[4], acc_y[4];
+    uint32_t gate_bits = 0u;
+    bn_clear(rd);
+    bn_clear(rr);
+    bn_clear(ry);
+    bn_clear(rh);
+    bn_clear(ry_next);
+    bn_clear(rg);
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = w[i] = acc_pre[i] = acc_y[i] = both(0.f);
+    auto fetch_y = [&](long long row, Bn8<X>& to) {
+        if (kY && on) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, to);
+    };
+    auto fetch = [&](long long row) {
+        if (on) {
+            if (Post) { if (row + step < tokens) fetch_y(row + step, ry_next); }
+            else fetch_y(row, ry);
+            if (Pre) {
+                bn_fetch<R, Vec>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, rr);
+                bn_fetch<X, Vec>(static_cast<const X*>(q.d_normed) + row * q.d_normed_ld, q.hidden, rh);
+            }
+            if (has_d) bn_fetch<R, Vec>(static_cast<const R*>(q.d_residual_out) + row * q.d_residual_out_ld, q.hidden, rd);
+            if (Kind == kBnElement) bn_fetch_gate<X, Vec>(q, row, rg);
+        }
+        if (Kind == kBnToken) gate_bits = bn_gate_bits<X>(q, row);
+    };
+    int row = blockIdx.x;
+    if (Post) fetch_y(row, ry);
+    fetch(row);
+    if (on) {
+        if (kY) bn_y_factor<X, Vec>(q, a);
+        if (Pre) bn_pre_factor<X, Vec>(q, w);
+    }
+    bn_sum_init(part);
+    int turn = 0;
+    float i1 = 1.f;
+    if (Post) {
+        float sum[1] = {bn_square(ry)};
+        bn_sum<1>(sum, part, turn);
+        i1 = rsqrtf(sum[0] * inv_h + q.eps);
+    }
+    while (true) {
+        const bool more = row + step < tokens;
+        const Bn8<R> cd = rd;
+        const Bn8<X> cy = ry, ch = rh;
+        const Bn8<float> cg = rg;
+        float2 r[4];
+        if (Pre) bn_unpack(rr, r);
+        if (Post) ry = ry_next;
+        const float gate = Kind == kBnToken ? bn_gate_value<X>(q, gate_bits) : 1.f;
+        if (more) fetch(row + step);
+        float sum[8] = {};                                   // r' r', dh w2 r', v d, v dh w2, v r' (v without a token's gate), next y's squares
+        {
+            float2 v[4], dh[4], d[4], g[4], t[5];
+            #pragma unroll
+            for (int k = 0; k < 5; ++k) t[k] = both(0.f);
+            if (kY) bn_unpack(cy, v);
+            if (Kind == kBnElement) bn_unpack_gate<X>(q, cg, g);
+            if (Pre) bn_unpack(ch, dh);
+            if (kSumV) bn_unpack(cd, d);
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (kY) {
+                    v[i] = mul2(Post ? mul2(v[i], both(i1)) : v[i], a[i]);
+                    if (Kind == kBnElement) v[i] = mul2(v[i], g[i]);
+                }
+                if (Pre) {
+                    if (kY) r[i] = fma2(v[i], both(gate), r[i]);
+                    dh[i] = mul2(dh[i], w[i]);
+                    t[0] = fma2(r[i], r[i], t[0]);
+                    t[1] = fma2(dh[i], r[i], t[1]);
+                }
+                if (kSumV) {
+                    t[2] = fma2(v[i], d[i], t[2]);
+                    if (Pre) { t[3] = fma2(v[i], dh[i], t[3]); t[4] = fma2(v[i], r[i], t[4]); }
+                }
+            }
+            #pragma unroll
+            for (int k = 0; k < 5; ++k) sum[k] = t[k].x + t[k].y;
+        }
+        if (Post) sum[5] = bn_square(ry);
+        if (kSumV) {
+            bn_sum<8>(sum, part, turn);
+        } else if (Pre) {
+            float two[2] = {sum[0], sum[1]};
+            bn_sum<2>(two, part, turn);
+            sum[0] = two[0];
+            sum[1] = two[1];
+        }
+        const float i2 = Pre ? rsqrtf(sum[0] * inv_h + q.eps) : 0.f, k = i2 * i2 * i2 * inv_h * sum[1];
+        const float vd = sum[2] + i2 * sum[3] - k * sum[4];
+        if (Kind == kBnToken && threadIdx.x == 0) {
+            if (sizeof(X) == 4 || q.gate32) static_cast<float*>(q.d_gate)[row * q.d_gate_ld] = vd;
+            else static_cast<X*>(q.d_gate)[row * q.d_gate_ld] = bn_round<X>(vd);
+        }
+        float2 d[4];
+        bn_unpack(cd, d);
+        if (Pre) {
+            float2 dh[4];
+            bn_unpack(ch, dh);
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 h2 = mul2(dh[i], both(i2));
+                acc_pre[i] = fma2(h2, r[i], acc_pre[i]);
+                d[i] = fma2(h2, w[i], fma2(r[i], both(-k), d[i]));
+            }
+        }
+        if (on) bn_put<R, Vec>(static_cast<R*>(q.d_residual) + static_cast<long long>(row) * q.d_residual_ld, q.hidden, d);
+        if (kY) {
+            const float2 y_up = both(i1 * gate), y_back = both(-i1 * i1 * gate * inv_h * vd);
+            float2 y[4];
+            bn_unpack(cy, y);
+            if (Kind == kBnElement) {
+                float2 g[4], dg[4];
+                bn_unpack_gate<X>(q, cg, g);
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    dg[i] = mul2(mul2(Post ? mul2(y[i], both(i1)) : y[i], a[i]), d[i]);
+                    d[i] = mul2(d[i], g[i]);
+                }
+                if (on) {
+                    const long long at = static_cast<long long>(row) * q.d_gate_ld;
+                    if (sizeof(X) == 4 || q.gate32) bn_put<float, Vec>(static_cast<float*>(q.d_gate) + at, q.hidden, dg);
+                    else bn_put<X, Vec>(static_cast<X*>(q.d_gate) + at, q.hidden, dg);
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 dy = Post || Kind == kBnToken ? mul2(d[i], y_up) : d[i];
+                acc_y[i] = fma2(dy, y[i], acc_y[i]);
+                d[i] = Post ? fma2(y[i], y_back, mul2(dy, a[i])) : mul2(dy, a[i]);
+            }
+            if (on) bn_put<X, Vec>(static_cast<X*>(q.d_y) + static_cast<long long>(row) * q.d_y_ld, q.hidden, d);
+        }
+        if (Post) i1 = rsqrtf(sum[5] * inv_h + q.eps);
+        if (!more) break;
+        row += step;
+    }
+    if (!on) return;
+    float* p = q.partial + static_cast<long long>(blockIdx.x) * q.hidden;
+    if (Pre) bn_put<float, Vec>(p, q.hidden, acc_pre);
+    if (sum_y) bn_put<float, Vec>(Pre ? p + static_cast<long long>(gridDim.x) * q.hidden : p, q.hidden, acc_y);
+}
+
+// Column sums of the CTAs' partial sums: a block takes 32 channels of one of the two, a thread every 32nd row of four channels; the threads' sums are added up in
+// shared memory in order. 296 rows of 3072 channels are 3.6 MB that lie in the L2.
 template <typename X>
 __global__ void __launch_bounds__(256) block_norm_sums_kernel(const BnSumsParams q) {
-    __shared__ float part[8][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.x * 32 + lane, which = blockIdx.y;
-    float v = 0.f;
-    if (h < q.hidden) {
-        const float* p = q.partial + static_cast<long long>(which) * q.rows * q.hidden + h;
-        for (int r = warp; r < q.rows; r += 8) v += p[static_cast<long long>(r) * q.hidden];
+    __shared__ float part[32][33];
+    const int col = (threadIdx.x & 7) * 4, group = threadIdx.x >> 3, h0 = blockIdx.x * 32;
+    const bool of_pre = q.d_pre_w != nullptr && blockIdx.y == 0;
+    float v[4] = {};
+    const float* p = q.partial + static_cast<long long>(blockIdx.y) * q.rows * q.hidden + h0 + col;
+    if ((q.hidden & 3) == 0) {
+        if (h0 + col < q.hidden) {
+            #pragma unroll 8
+            for (int r = group; r < q.rows; r += 32) {
+                const float4 f = *reinterpret_cast<const float4*>(p + static_cast<long long>(r) * q.hidden);
+                v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+            }
+        }
+    } else {
+        #pragma unroll 2
+        for (int r = group; r < q.rows; r += 32) {
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) if (h0 + col + i < q.hidden) v[i] += p[static_cast<long long>(r) * q.hidden + i];
+        }
     }
-    part[warp][lane] = v;
-    __syncthreads();
-    if (warp != 0 || h >= q.hidden) return;
     #pragma unroll
-    for (int w = 1; w < 8; ++w) v += part[w][lane];
-    if (q.is32[which]) static_cast<float*>(q.out[which])[h] = v;
-    else static_cast<X*>(q.out[which])[h] = bn_round<X>(v);
+    for (int i = 0; i < 4; ++i) part[group][col + i] = v[i];
+    __syncthreads();
+    const int h = h0 + static_cast<int>(threadIdx.x);
+    if (threadIdx.x >= 32 || h >= q.hidden) return;
+    float sum = 0.f;
+    #pragma unroll
+    for (int g = 0; g < 32; ++g) sum += part[g][threadIdx.x];
+    auto put = [&](void* to, int is32, float x) {
+        if (is32) static_cast<float*>(to)[h] = x; else static_cast<X*>(to)[h] = bn_round<X>(x);
+    };
+    auto get = [&](const void* from, int is32) { return is32 ? static_cast<const float*>(from)[h] : bn_float<X>(static_cast<const X*>(from)[h]); };
+    if (of_pre) { put(q.d_pre_w, q.weight32, sum); return; }
+    if (q.d_post_w != nullptr) put(q.d_post_w, q.weight32, q.scale * (q.gate != nullptr ? get(q.gate, q.gate32) : 1.f) * sum);
+    if (q.d_gate != nullptr) put(q.d_gate, q.gate32, q.scale * (q.post_w != nullptr ? get(q.post_w, q.weight32) + q.offset : 1.f) * sum);
+}
+
+// ----------------------------------------------------------------------------- launches
+template <auto Kernel>
+int bn_start(const BnParams& q, int grid, cudaStream_t stream) {
+    Kernel<<<grid, bn_threads(q.hidden), 0, stream>>>(q);
+    MM_CUDA(cudaGetLastError());
+    return MM_OK;
+}
+
+// CTAs of a kernel that an SM holds; asked for once per CTA size and kernel (the answer is the binary's and the GPU's, of which there is one kind).
+template <auto Kernel>
+int bn_per_sm(int threads, int* per) {
+    static std::atomic<int> known[kBnMaxThreads / 32 + 1] = {};
+    const int k = known[threads / 32].load(std::memory_order_relaxed);
+    if (k > 0) { *per = k; return MM_OK; }
+    int n = 0;
+    MM_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, threads, 0));
+    *per = n > 0 ? n : 1;
+    known[threads / 32].store(*per, std::memory_order_relaxed);
+    return MM_OK;
+}
+
+template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec>
+int bn_launch_kind(const BnParams& q, const BnLaunch& how, cudaStream_t stream) {
+    if (how.backward) return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Vec>>(q, how.ctas, stream);
+    int per = 0;
+    const int st = bn_per_sm<block_norm_kernel<X, R, Post, Pre, Kind, Vec>>(bn_threads(q.hidden), &per);
+    if (st != MM_OK) return st;
+    const long long most = static_cast<long long>(per) * how.sms;
+    return bn_start<block_norm_kernel<X, R, Post, Pre, Kind, Vec>>(q, static_cast<int>(q.tokens < most ? q.tokens : most), stream);
+}
+
+template <typename X, typename R, bool Vec>
+int bn_launch_rows(const BnParams& q, const BnLaunch& how, cudaStream_t stream) {
+    const bool post = q.post_w != nullptr, pre = q.pre_w != nullptr;
+    if (q.y == nullptr) return bn_launch_kind<X, R, false, true, kBnStream, Vec>(q, how, stream);
+    auto by_kind = [&](auto p, auto n) {
+        constexpr bool kPost = decltype(p)::value, kPre = decltype(n)::value;
+        if (q.gate_mode == kBnGateToken) return bn_launch_kind<X, R, kPost, kPre, kBnToken, Vec>(q, how, stream);
+        if (q.gate_mode == kBnGateElement) return bn_launch_kind<X, R, kPost, kPre, kBnElement, Vec>(q, how, stream);
+        return bn_launch_kind<X, R, kPost, kPre, kBnPlain, Vec>(q, how, stream);
+    };
+    using std::false_type;
+    using std::true_type;
+    return post ? (pre ? by_kind(true_type{}, true_type{}) : by_kind(true_type{}, false_type{}))
+                : (pre ? by_kind(false_type{}, true_type{}) : by_kind(false_type{}, false_type{}));
+}
+
+template <typename X, typename R>
+int bn_launch(const BnParams& q, const BnLaunch& how, cudaStream_t stream) {
+    if (q.hidden <= kBnHeldHidden) return how.aligned ? bn_launch_rows<X, R, true>(q, how, stream) : bn_launch_rows<X, R, false>(q, how, stream);
+    if (how.backward) return bn_start<block_norm_backward_wide_kernel<X, R>>(q, how.ctas, stream);
+    const long long most = 2ll * how.sms;
+    return bn_start<block_norm_wide_kernel<X, R>>(q, static_cast<int>(q.tokens < most ? q.tokens : most), stream);
+}
+
+template <typename X>
+int bn_launch_sums(const BnSumsParams& q, cudaStream_t stream) {
+    block_norm_sums_kernel<X><<<dim3((q.hidden + 31) / 32, q.sums), 256, 0, stream>>>(q);
+    MM_CUDA(cudaGetLastError());
+    return MM_OK;
 }
 
 }  // namespace mm

@@ -282,7 +282,7 @@ typedef struct mm_block_norm_grads {
     void* d_pre_weight;              /* weight_dtype [hidden] */
     void* d_post_weight;
     int64_t d_residual_out_stride, d_normed_stride, d_residual_stride, d_y_stride, d_gate_stride;
-    void* workspace;                 /* mm_block_norm_workspace_bytes(), 16-byte aligned; needed for weights' and a channel gate's gradients */
+    void* workspace;                 /* mm_block_norm_workspace_bytes(), 32-byte aligned; needed for weights' and a channel gate's gradients */
     int64_t workspace_bytes;
 } mm_block_norm_grads_t;
 

@@ -110,7 +110,7 @@ def test_norm_calls_that_pass_the_checks(change):
 
 @pytest.mark.parametrize('norm, grads', [
     ({}, dict(d_normed=0)), ({}, dict(d_residual=0)), ({}, dict(d_y=0)), ({}, dict(d_pre_weight=0)), ({}, dict(d_post_weight=0)), ({}, dict(workspace=0)),
-    ({}, dict(workspace_bytes=4 * 64 * 3 * 4 - 1)), ({}, dict(workspace=13 * A + 4)), ({}, dict(d_residual=7 * A)), ({}, dict(d_y=9 * A)), ({}, dict(d_y=A)),
+    ({}, dict(workspace_bytes=4 * 64 * 2 * 4 - 1)), ({}, dict(workspace=13 * A + 4)), ({}, dict(d_residual=7 * A)), ({}, dict(d_y=9 * A)), ({}, dict(d_y=A)),
     ({}, dict(d_residual=2 * A)), ({}, dict(d_y=3 * A)), ({}, dict(d_y_stride=63)), (dict(pre_weight=0), {}), (dict(y=0, post_weight=0), {}),
     (dict(gate=14 * A, gate_mode=1), {}), (dict(gate=14 * A, gate_mode=2, gate_stride=1), {}), (dict(gate=14 * A, gate_mode=3, gate_stride=64), dict(d_gate=14 * A)),
     (dict(gate=14 * A, gate_mode=3, gate_stride=64), dict(d_gate=9 * A)), (dict(eps=-1.0), {}), (dict(residual=0), {}),
