@@ -5,7 +5,7 @@
 
 #include "../../include/megamoe_b200.h"
 #include "mm_block_norm.h"
-#include "mm_router.cuh"
+#include "mm_router.h"
 #include "mm_error.h"
 
 namespace {
@@ -130,35 +130,17 @@ int balance_check(const mm_balance_args_t* b) {
     return MM_OK;
 }
 
-#define MM_ROUTER_EXPERTS(L, KERNEL)                                                              \
-    do {                                                                                          \
-        const int v = (q.E + 31) / 32;                                                            \
-        if (v <= 1) KERNEL<L, 1><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);                      \
-        else if (v <= 2) KERNEL<L, 2><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);                 \
-        else if (v <= 4) KERNEL<L, 4><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);                 \
-        else if (v <= 8) KERNEL<L, 8><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);                 \
-        else if (v <= 12) KERNEL<L, 12><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);               \
-        else if (v <= 16) KERNEL<L, 16><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);               \
-        else KERNEL<L, 32><<<grid, mm::kRtWarps * 32, 0, stream>>>(q);                            \
-    } while (0)
-#define MM_ROUTER_LAUNCH(KERNEL)                                                                  \
-    do {                                                                                          \
-        if (a->dtype == MM_DTYPE_FP32) MM_ROUTER_EXPERTS(float, KERNEL);                          \
-        else if (a->dtype == MM_DTYPE_BF16) MM_ROUTER_EXPERTS(__nv_bfloat16, KERNEL);             \
-        else MM_ROUTER_EXPERTS(__half, KERNEL);                                                   \
-    } while (0)
-
-int router_grid(int tokens, int sms) {
-    const int blocks = (tokens + mm::kRtWarps - 1) / mm::kRtWarps, most = sms * 8;
-    return blocks < most ? (blocks > 0 ? blocks : 1) : most;
+int launch_router(int dtype, mm::RtOp op, const mm::RtParams& q, void* stream) {
+    int sms = 0;
+    const int st = sm_count(&sms);
+    if (st != MM_OK) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == MM_DTYPE_BF16 ? mm::launch_router_bf16(op, q, sms, s)
+                                  : (dtype == MM_DTYPE_FP16 ? mm::launch_router_fp16(op, q, sms, s) : mm::launch_router_fp32(op, q, sms, s));
 }
 
-constexpr int kBalanceGrid = 1184;           // CTAs of the balance kernel at most (eight per SM of 148): the workspace does not depend on the device
-
-int balance_grid(int tokens) {
-    const int blocks = (tokens + mm::kRtWarps - 1) / mm::kRtWarps;
-    return blocks < kBalanceGrid ? (blocks > 0 ? blocks : 1) : kBalanceGrid;
-}
+// Workspace of the balance loss: the sums (zeroed by the call), then a number per CTA.
+int64_t balance_zeroed_bytes(int64_t experts, int64_t sequences) { return (sequences * experts * 12 + sequences * 4 + 4 + 7) / 8 * 8; }
 
 }  // namespace
 
@@ -258,19 +240,12 @@ int mm_route_tokens(const mm_router_args_t* a, const float* expert_bias, const u
     if (a->topk_weights == nullptr) return MM_ERR_INVALID_ARGUMENT;
     mm::RtParams q = router_params(a);
     q.bias = expert_bias; q.valid = valid;
-    int sms = 0;
-    st = sm_count(&sms);
-    if (st != MM_OK) return st;
-    const int grid = router_grid(a->tokens, sms);
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-    MM_ROUTER_LAUNCH(mm::route_kernel);
-    MM_CUDA(cudaGetLastError());
-    return MM_OK;
+    return launch_router(a->dtype, mm::kRtRoute, q, stream_ptr);
 }
 
 int64_t mm_balance_workspace_bytes(int32_t num_experts, int32_t num_sequences) {
     if (num_experts < 1 || num_experts > mm::kRtMaxExperts || num_sequences < 1) return -1;
-    return static_cast<int64_t>(num_sequences) * num_experts * 8 + static_cast<int64_t>(kBalanceGrid) * mm::kRtWarps * 8;
+    return balance_zeroed_bytes(num_experts, num_sequences) + static_cast<int64_t>(mm::kRtBalanceCtas) * 8;
 }
 
 int mm_balance_loss(const mm_router_args_t* a, const mm_balance_args_t* b, void* workspace, int64_t workspace_bytes, void* stream_ptr) {
@@ -281,20 +256,14 @@ int mm_balance_loss(const mm_router_args_t* a, const mm_balance_args_t* b, void*
         workspace_bytes < mm_balance_workspace_bytes(a->num_experts, b->num_sequences)) return MM_ERR_INVALID_ARGUMENT;
     mm::RtParams q = router_params(a);
     balance_params(b, q);
-    const int grid = balance_grid(a->tokens);
-    const int64_t cells = static_cast<int64_t>(q.S) * q.E;
+    const int64_t cells = static_cast<int64_t>(q.S) * q.E, zeroed = balance_zeroed_bytes(q.E, q.S);
     q.sums = static_cast<unsigned long long*>(workspace);
-    q.z_part = reinterpret_cast<double*>(q.sums + cells);
-    q.z_parts = grid * mm::kRtWarps;
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-    MM_CUDA(cudaMemsetAsync(q.sums, 0, cells * 8, stream));
-    MM_CUDA(cudaMemsetAsync(q.counts, 0, cells * 4, stream));
-    MM_CUDA(cudaMemsetAsync(q.tokens, 0, static_cast<size_t>(q.S) * 4, stream));
-    MM_ROUTER_LAUNCH(mm::balance_kernel);
-    MM_CUDA(cudaGetLastError());
-    mm::balance_end_kernel<<<1, 1024, 0, stream>>>(q);
-    MM_CUDA(cudaGetLastError());
-    return MM_OK;
+    q.sum_counts = reinterpret_cast<int*>(q.sums + cells);
+    q.sum_tokens = q.sum_counts + cells;
+    q.ticket = reinterpret_cast<unsigned*>(q.sum_tokens + q.S);
+    q.z_part = reinterpret_cast<double*>(static_cast<char*>(workspace) + zeroed);
+    MM_CUDA(cudaMemsetAsync(workspace, 0, zeroed, static_cast<cudaStream_t>(stream_ptr)));
+    return launch_router(a->dtype, mm::kRtBalance, q, stream_ptr);
 }
 
 int mm_router_backward(const mm_router_args_t* a, const float* d_topk_weights, const mm_balance_args_t* b, float d_loss, const float* d_loss_ptr,
@@ -314,14 +283,7 @@ int mm_router_backward(const mm_router_args_t* a, const float* d_topk_weights, c
     q.balance = b != nullptr;
     q.d_weights = d_topk_weights; q.d_loss = d_loss; q.d_loss_ptr = d_loss_ptr;
     q.d_logits = d_logits; q.d_logits_ld = d_logits_stride;
-    int sms = 0;
-    st = sm_count(&sms);
-    if (st != MM_OK) return st;
-    const int grid = router_grid(a->tokens, sms);
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-    MM_ROUTER_LAUNCH(mm::router_backward_kernel);
-    MM_CUDA(cudaGetLastError());
-    return MM_OK;
+    return launch_router(a->dtype, mm::kRtBackward, q, stream_ptr);
 }
 
 }  // extern "C"
