@@ -245,7 +245,7 @@ int mm_route_tokens(const mm_router_args_t* a, const float* expert_bias, const u
 
 int64_t mm_balance_workspace_bytes(int32_t num_experts, int32_t num_sequences) {
     if (num_experts < 1 || num_experts > mm::kRtMaxExperts || num_sequences < 1) return -1;
-    return balance_zeroed_bytes(num_experts, num_sequences) + static_cast<int64_t>(mm::kRtBalanceCtas) * 8;
+    return balance_zeroed_bytes(num_experts, num_sequences) + static_cast<int64_t>(mm::kRtBalanceCtas) * 16;
 }
 
 int mm_balance_loss(const mm_router_args_t* a, const mm_balance_args_t* b, void* workspace, int64_t workspace_bytes, void* stream_ptr) {
@@ -262,6 +262,7 @@ int mm_balance_loss(const mm_router_args_t* a, const mm_balance_args_t* b, void*
     q.sum_tokens = q.sum_counts + cells;
     q.ticket = reinterpret_cast<unsigned*>(q.sum_tokens + q.S);
     q.z_part = reinterpret_cast<double*>(static_cast<char*>(workspace) + zeroed);
+    q.end_part = q.z_part + mm::kRtBalanceCtas;
     MM_CUDA(cudaMemsetAsync(workspace, 0, zeroed, static_cast<cudaStream_t>(stream_ptr)));
     return launch_router(a->dtype, mm::kRtBalance, q, stream_ptr);
 }

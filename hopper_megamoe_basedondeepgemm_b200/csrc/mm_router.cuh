@@ -59,105 +59,122 @@ __device__ __forceinline__ float rt_sum(float v) {
     return v;
 }
 
+// The special function unit's exponential and reciprocal, results below 2^-126 as 0: good to 2^-22 and 2^-23, and an exponent of x log2(e) is off by up to
+// 1.5 |x| 2^-24 of its result.
+__device__ __forceinline__ float rt_exp2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float rt_rcp(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+constexpr float kRtLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float rt_exp(float v) { return rt_exp2(v * kRtLog2e); }
 // sigmoid(v), and 1 - sigmoid(v) without the difference of near numbers
-__device__ __forceinline__ float rt_sigmoid(float v) { return __fdividef(1.f, 1.f + expf(-v)); }       // (exp(-v) above 2^126 gives 0)
-__device__ __forceinline__ float rt_sigmoid_rest(float v) { return __fdividef(1.f, 1.f + expf(v)); }
+__device__ __forceinline__ float rt_sigmoid(float v) { return rt_rcp(1.f + rt_exp(-v)); }
+__device__ __forceinline__ float rt_sigmoid_rest(float v) { return rt_rcp(1.f + rt_exp(v)); }
 
 template <typename L, int V>
-__device__ __forceinline__ void rt_load(const RtParams& q, int row, int lane, float (&l)[V]) {
+__device__ __forceinline__ void rt_fetch(const RtParams& q, int row, int lane, float (&l)[V]) {
     const L* p = static_cast<const L*>(q.logits) + static_cast<long long>(row) * q.logits_ld + lane;
     #pragma unroll
     for (int j = 0; j < V; ++j) l[j] = j * 32 + lane < q.E ? rt_float<L>(p[j * 32]) : rt_off();
+}
+template <int V>
+__device__ __forceinline__ void rt_clean(float (&l)[V]) {
     #pragma unroll
     for (int j = 0; j < V; ++j) l[j] = rt_logit(l[j]);
 }
 
-// The sequence of a token that lies at or behind cu[0]: S if it is behind the last one. Reads cu alone, whatever it holds, and where the result is below S,
-// cu[result + 1] is above the token.
+// The sequence of a token that lies at or behind cu[0], by a whole warp: S if it is behind the last one. Each step looks at 32 ends at once. Reads cu alone, whatever
+// it holds, and where the result is below S, cu[result + 1] is above the token.
 __device__ __forceinline__ int rt_sequence(const int* cu, int S, int row) {
-    int lo = 0, hi = S;                      // the number of ends that are <= row
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = S;                      // the number of ends that are <= row lies between
     while (lo < hi) {
-        const int m = (lo + hi) >> 1;
-        if (cu[m + 1] <= row) lo = m + 1; else hi = m;
+        const int step = (hi - lo + 31) >> 5, m = lo + lane * step;
+        const uint32_t above = __ballot_sync(0xffffffffu, m < hi && cu[min(m, hi - 1) + 1] > row);
+        if (above == 0u) {                   // (none of those looked at: behind the last of them)
+            lo = lo + (hi - lo - 1) / step * step + 1;
+        } else {
+            const int f = __ffs(above) - 1;
+            hi = lo + f * step;
+            lo = f > 0 ? lo + (f - 1) * step + 1 : hi;
+        }
     }
-    return lo;
+    return hi;
 }
 
 // ----------------------------------------------------------------------------- route
-// A row whose candidates do not fit a warp (many equal keys): the largest key, one after the other, over all experts.
+// A row whose candidates do not fit a warp (many equal keys, or more routes than lanes have experts on top): the largest key, one after the other, over all experts.
+// The lane's expert, -1 for none. (A call of its own, by values: a reference to the launch's parameters would have every thread copy them.)
 template <typename L, int Mode>
-__device__ __noinline__ void rt_route_any(const RtParams& q, int row, int* at_out, float* logit_out) {
+__device__ __noinline__ int rt_route_any(const L* p, const float* bias, int experts, int topk) {
     const int lane = threadIdx.x & 31;
-    const L* p = static_cast<const L*>(q.logits) + static_cast<long long>(row) * q.logits_ld;
     double last = 0.0;
     int last_at = -1, mine = -1;
-    float mine_logit = 0.f;
-    for (int k = 0; k < q.K; ++k) {
+    for (int k = 0; k < topk; ++k) {
         double best = static_cast<double>(rt_off());
-        int at = q.E;
-        for (int e = lane; e < q.E; e += 32) {
+        int at = experts;
+        for (int e = lane; e < experts; e += 32) {
             const float v = rt_logit(rt_float<L>(p[e]));
-            if (v == rt_off()) continue;
             double key = static_cast<double>(v);
-            if (Mode == 1) key = 1.0 / (1.0 + exp(-key)) + (q.bias != nullptr ? static_cast<double>(q.bias[e]) : 0.0);
-            if (k > 0 && !(key < last || (key == last && e > last_at))) continue;                // taken already
-            if (key > best) { best = key; at = e; }
+            if (Mode == 1) key = 1.0 / (1.0 + exp(-key)) + (bias != nullptr ? static_cast<double>(bias[e]) : 0.0);
+            const bool open = v != rt_off() && key > static_cast<double>(rt_off()) && (k == 0 || key < last || (key == last && e > last_at));           // on, and not taken already
+            if (open && (at == experts || key > best)) { best = key; at = e; }
         }
         #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const double other = __shfl_xor_sync(0xffffffffu, best, o);
             const int other_at = __shfl_xor_sync(0xffffffffu, at, o);
-            if (other_at < q.E && (at >= q.E || other > best || (other == best && other_at < at))) { best = other; at = other_at; }
+            if (other_at < experts && (at >= experts || other > best || (other == best && other_at < at))) { best = other; at = other_at; }
         }
-        if (at >= q.E) break;
+        if (at >= experts) break;
         last = best;
         last_at = at;
-        if (lane == k) { mine = at; mine_logit = rt_logit(rt_float<L>(p[at])); }
+        if (lane == k) mine = at;
     }
-    *at_out = mine;
-    *logit_out = mine_logit;
+    return mine;
 }
 
 // Twice what a 32-bit key of mode 1 can be off by: 2^-20 for the exponential, the sum and the quotient of a sigmoid, 2^-22 of the key for its last addition.
 __device__ __forceinline__ float rt_key_margin(float key) { return 0x1p-19f + fabsf(key) * 0x1p-21f; }
 
 // The K-th largest of the lanes' own maxima is a bound: no key below it is among the K largest. What is not below it, K experts and a few, moves to one per
-// lane, and the largest of those are taken by turns. In mode 1 keys are first computed in 32 bits; where two that matter come closer than their
-// error, they are computed in 64.
+// lane, in the experts' order, and a candidate's place is the number of those before it. In mode 1 keys are first computed in 32 bits; where two
+// candidates come closer than their error, all of them are computed in 64.
 template <typename L, int V, int Mode>
 __global__ void __launch_bounds__(kRtWarps * 32) route_kernel(const RtParams q) {
     __shared__ float cand_logit[kRtWarps][32];
+    __shared__ __align__(16) float cand_key[kRtWarps][32];
     __shared__ int cand_at[kRtWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t below = (1u << lane) - 1u;
     for (int row = blockIdx.x * kRtWarps + warp; row < q.T; row += gridDim.x * kRtWarps) {
-        int rank = -1, at = -1;                                          // of the expert that this lane has taken
-        float logit = 0.f, top = 0.f;
-        int taken = 0;
+        int rank = q.K, at = -1, taken = 0;                              // this lane's expert and its place
+        float logit = rt_off();
         if (q.valid == nullptr || q.valid[row] != 0) {
-            float l[V];
-            uint32_t key[V], best = 0u;
-            rt_load<L, V>(q, row, lane, l);
+            float l[V], key[V];
+            rt_fetch<L, V>(q, row, lane, l);
+            if (Mode == 1) {
+                #pragma unroll
+                for (int j = 0; j < V; ++j) key[j] = q.bias != nullptr && j * 32 + lane < q.E ? __ldg(q.bias + j * 32 + lane) : 0.f;
+            }
+            rt_clean<V>(l);
+            float best = rt_off();
             #pragma unroll
             for (int j = 0; j < V; ++j) {
-                float k = l[j];
-                if (Mode == 1) {
-                    const float b = q.bias != nullptr && j * 32 + lane < q.E ? __ldg(q.bias + j * 32 + lane) : 0.f;
-                    k = k == rt_off() ? k : __fdividef(1.f, 1.f + __expf(-k)) + b;
-                }
-                key[j] = k > rt_off() ? rt_order(k) : 0u;
-                best = max(best, key[j]);
+                key[j] = Mode == 1 ? (l[j] == rt_off() ? rt_off() : fmaxf(rt_sigmoid(l[j]) + key[j], rt_off())) : l[j];
+                best = fmaxf(best, key[j]);
             }
-            uint32_t bound = 0u, mine = best;
+            uint32_t mine = best == rt_off() ? 0u : rt_order(best), high = 0u;
             for (int n = 0; n < q.K;) {
-                bound = __reduce_max_sync(0xffffffffu, mine);
-                if (bound == 0u) break;
-                const bool is = mine == bound;
+                high = __reduce_max_sync(0xffffffffu, mine);
+                if (high == 0u) break;
+                const bool is = mine == high;
                 n += __popc(__ballot_sync(0xffffffffu, is));
                 if (is) mine = 0u;
             }
-            if (Mode == 1 && bound != 0u) bound = rt_order(rt_unorder(bound) - rt_key_margin(rt_unorder(bound)));
-            if (bound == 0u) bound = 1u;
+            float bound = -FLT_MAX;                                      // (what is on; in mode 1 with an infinite bias, too)
+            if (high != 0u) {
+                bound = rt_unorder(high);
+                if (Mode == 1) bound = fmaxf(bound - rt_key_margin(bound), -FLT_MAX);
+            }
             int n = 0;
             #pragma unroll
             for (int j = 0; j < V; ++j) {
@@ -165,74 +182,62 @@ __global__ void __launch_bounds__(kRtWarps * 32) route_kernel(const RtParams q) 
                 const uint32_t who = __ballot_sync(0xffffffffu, is);
                 if (who != 0u) {
                     const int to = n + __popc(who & below);
-                    if (is && to < 32) { cand_logit[warp][to] = l[j]; cand_at[warp][to] = j * 32 + lane; }
+                    if (is && to < 32) { cand_key[warp][to] = key[j]; cand_at[warp][to] = j * 32 + lane; if (Mode == 1) cand_logit[warp][to] = l[j]; }
                     n += __popc(who);
                 }
             }
             __syncwarp();
             if (n > 32) {
-                rt_route_any<L, Mode>(q, row, &at, &logit);
-                rank = at >= 0 ? lane : -1;
-                top = rt_max(rank >= 0 ? logit : rt_off());
-                taken = __popc(__ballot_sync(0xffffffffu, rank >= 0));
+                at = rt_route_any<L, Mode>(static_cast<const L*>(q.logits) + static_cast<long long>(row) * q.logits_ld, q.bias, q.E, q.K);
+                if (at >= 0) {
+                    rank = lane;
+                    logit = rt_logit(rt_float<L>(static_cast<const L*>(q.logits)[static_cast<long long>(row) * q.logits_ld + at]));
+                }
+                taken = __popc(__ballot_sync(0xffffffffu, at >= 0));
             } else {
-                uint32_t hi = 0u, lo = 0u;                               // this lane's candidate, as a key of 32 bits or 64
-                float k32 = 0.f;
-                if (lane < n) {
-                    logit = cand_logit[warp][lane];
-                    at = cand_at[warp][lane];
-                    k32 = logit;
-                    if (Mode == 1) k32 = __fdividef(1.f, 1.f + __expf(-logit)) + (q.bias != nullptr ? __ldg(q.bias + at) : 0.f);
-                    hi = rt_order(k32);
+                float mine_key = rt_off();
+                if (lane < n) { mine_key = cand_key[warp][lane]; at = cand_at[warp][lane]; logit = Mode == 1 ? cand_logit[warp][lane] : mine_key; }
+                int before = 0;
+                bool close = false;
+                const float margin = Mode == 1 ? rt_key_margin(mine_key) : 0.f;
+                for (int c = 0; c < n; c += 4) {
+                    const float4 k4 = *reinterpret_cast<const float4*>(&cand_key[warp][c]);
+                    const float ks[4] = {k4.x, k4.y, k4.z, k4.w};
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool there = c + i < n;
+                        before += there && (ks[i] > mine_key || (ks[i] == mine_key && c + i < lane));
+                        if (Mode == 1) close = close || (there && c + i != lane && !(fabsf(ks[i] - mine_key) > margin));
+                    }
+                }
+                if (Mode == 1) {
+                    if (__ballot_sync(0xffffffffu, close && lane < n) != 0u) {
+                        const double key64 = lane < n ? 1.0 / (1.0 + exp(-static_cast<double>(logit))) + (q.bias != nullptr ? static_cast<double>(__ldg(q.bias + at)) : 0.0) : 0.0;
+                        before = 0;
+                        for (int c = 0; c < n; ++c) {
+                            const double other = __shfl_sync(0xffffffffu, key64, c);
+                            before += other > key64 || (other == key64 && c < lane);
+                        }
+                    }
                 }
                 __syncwarp();
-                bool close = false;
-                if (Mode == 1) {
-                    // two of them nearer than the error, or equal?
-                    uint32_t left = hi;
-                    float last = 0.f;
-                    for (int k = 0; k <= q.K && k < n; ++k) {
-                        const uint32_t m = __reduce_max_sync(0xffffffffu, left);
-                        const float f = rt_unorder(m);
-                        const uint32_t who = __ballot_sync(0xffffffffu, left == m);
-                        close = close || (k > 0 && last - f <= rt_key_margin(last)) || (who & (who - 1u)) != 0u;
-                        last = f;
-                        if (left == m) left = 0u;
-                    }
-                    if (close) {
-                        unsigned long long b = 0ull;
-                        if (lane < n) {
-                            const double key64 = 1.0 / (1.0 + exp(-static_cast<double>(logit))) + (q.bias != nullptr ? static_cast<double>(__ldg(q.bias + at)) : 0.0);
-                            b = static_cast<unsigned long long>(__double_as_longlong(key64 == 0.0 ? 0.0 : key64));
-                            b ^= static_cast<unsigned long long>(static_cast<long long>(b) >> 63) | 0x8000000000000000ull;
-                        }
-                        hi = static_cast<uint32_t>(b >> 32);
-                        lo = static_cast<uint32_t>(b);
-                    }
-                }
-                const int want = min(q.K, n);
-                for (int k = 0; k < want; ++k) {
-                    const uint32_t m = __reduce_max_sync(0xffffffffu, hi);
-                    bool is = hi == m && m != 0u;
-                    if (Mode == 1 && close) {
-                        const uint32_t m_lo = __reduce_max_sync(0xffffffffu, is ? lo : 0u);
-                        is = is && lo == m_lo;
-                    }
-                    // (candidates lie in the experts' order: of equal ones the first lane's is the lowest)
-                    const uint32_t who = __ballot_sync(0xffffffffu, is);
-                    if (is && (who & below) == 0u) { rank = k; hi = lo = 0u; }
-                }
-                taken = want;
-                if (Mode == 0) top = rt_max(rank >= 0 ? logit : rt_off());
+                taken = min(q.K, n);
+                if (lane < n && before < taken) rank = before; else logit = rt_off();
             }
         }
+        const bool chosen = rank < q.K;
         float s = 0.f;
-        if (rank >= 0) s = Mode == 1 ? rt_sigmoid(logit) : expf(logit - top);
+        if (Mode == 1) {
+            if (chosen) s = rt_sigmoid(logit);
+        } else {
+            const float top = rt_max(logit);
+            if (chosen) s = rt_exp(logit - top);
+        }
         const float total = rt_sum(s);
         const long long to = static_cast<long long>(row) * q.K;
-        if (rank >= 0) {
+        if (chosen) {
             q.idx[to + rank] = at;
-            q.weights[to + rank] = total > 0.f ? s / total * q.route_scale : 0.f;
+            q.weights[to + rank] = total > 0.f ? s * rt_rcp(total) * q.route_scale : 0.f;
         }
         if (lane >= taken && lane < q.K) {
             q.idx[to + lane] = -1;
@@ -241,148 +246,210 @@ __global__ void __launch_bounds__(kRtWarps * 32) route_kernel(const RtParams q) 
     }
 }
 
+// CTAs of the kernels below that an SM is to hold, and the launches fill: registers for a token's logits, those of the next one and what is made of them. A grid of that size
+// has each warp take several tokens, whose sums go out once.
+template <int V>
+constexpr int rt_ctas() { return V <= 4 ? 5 : (V <= 8 ? 4 : (V <= 12 ? 3 : (V <= 16 ? 2 : 1))); }
+
 // ----------------------------------------------------------------------------- balance
-// A token's probabilities p; its softmax and the logarithm of its sum of exponentials; mode 1: its sigmoids' complements.
-template <int V, int Mode, bool Rest>
-__device__ __forceinline__ float rt_probabilities(const float (&l)[V], float (&p)[V], float (&soft)[V], float (&rest)[V]) {
+// What a token's logits give, up to factors of the whole token: exp[j] * exp_scale is its softmax; in mode 1 sig[j] * sig_scale are its sigmoids over their sum, and
+// 1 - sigmoid is rest[j] (where asked for).
+template <int V>
+struct RtScores {
+    float exp[V], sig[V], rest[V], exp_scale, sig_scale, lse;
+};
+
+// `Careful` takes any logits; without it, it says (false) when they hold a NaN, or numbers so large that the result means nothing.
+template <int V, int Mode, bool Rest, bool Careful>
+__device__ __forceinline__ bool rt_scores_try(const float (&l)[V], RtScores<V>& s) {
     float top = l[0];
     #pragma unroll
-    for (int j = 1; j < V; ++j) top = fmaxf(top, l[j]);
+    for (int j = 1; j < V; ++j) top = fmaxf(top, l[j]);                  // (NaN is no maximum)
     top = rt_max(top);
-    if (top == rt_off()) {
+    s.exp_scale = s.sig_scale = s.lse = 0.f;
+    if (Careful && top == rt_off()) {
         #pragma unroll
-        for (int j = 0; j < V; ++j) p[j] = soft[j] = rest[j] = 0.f;
-        return 0.f;
+        for (int j = 0; j < V; ++j) s.exp[j] = s.sig[j] = s.rest[j] = 0.f;
+        return true;
     }
-    float sum = 0.f, sig_sum = 0.f, lse = top;
-    if (Mode == 1 && top <= 60.f) {
-        // exp(l) by itself does not overflow (nor does the sum): it gives the softmax and the sigmoid
-        #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            soft[j] = expf(l[j]);
-            rest[j] = __fdividef(1.f, 1.f + soft[j]);
-            p[j] = soft[j] * rest[j];
-            sum += soft[j];
-            sig_sum += p[j];
-        }
-        if (top >= -40.f) {                                              // (nor do the largest of them get lost)
-            lse = 0.f;
-        } else {
-            sum = 0.f;
-            #pragma unroll
-            for (int j = 0; j < V; ++j) { soft[j] = expf(l[j] - top); sum += soft[j]; }
-        }
-    } else {
-        #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            soft[j] = expf(l[j] - top);
-            sum += soft[j];
-            if (Mode == 1) {
-                p[j] = rt_sigmoid(l[j]);
-                if (Rest) rest[j] = rt_sigmoid_rest(l[j]);
-                sig_sum += p[j];
-            }
-        }
-    }
-    sum = rt_sum(sum);
-    const float inv = 1.f / sum;
-    float sig_inv = 0.f;
-    if (Mode == 1) {
-        sig_sum = rt_sum(sig_sum);
-        sig_inv = sig_sum > 0.f ? 1.f / sig_sum : 0.f;
-    }
+    float sum = 0.f, sig_sum = 0.f;
+    // mode 1: exp(l) by itself, where it neither overflows nor loses the largest of them, gives both the softmax and the sigmoid
+    const bool plain = Mode == 1 && fabsf(top) <= 40.f;
+    const float base = plain ? 0.f : top, shift = base * kRtLog2e;
     #pragma unroll
     for (int j = 0; j < V; ++j) {
-        soft[j] *= inv;
-        p[j] = Mode == 1 ? p[j] * sig_inv : soft[j];
+        s.exp[j] = Careful ? rt_exp(l[j] - base) : rt_exp2(fmaf(l[j], kRtLog2e, -shift));
+        sum += s.exp[j];
     }
-    return lse + logf(sum);
+    sum = rt_sum(sum);
+    if (!Careful && !(sum > 0.f && sum <= FLT_MAX)) return false;
+    if (Mode == 1) {
+        #pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (plain) {
+                s.rest[j] = rt_rcp(1.f + s.exp[j]);
+                s.sig[j] = s.exp[j] * s.rest[j];
+            } else {
+                s.sig[j] = rt_sigmoid(l[j]);
+                if (Rest) s.rest[j] = rt_sigmoid_rest(l[j]);
+            }
+            sig_sum += s.sig[j];
+        }
+        sig_sum = rt_sum(sig_sum);
+        s.sig_scale = sig_sum > 0.f ? rt_rcp(sig_sum) : 0.f;
+    }
+    s.exp_scale = rt_rcp(sum);
+    s.lse = base + __logf(sum);
+    return true;
+}
+template <int V, int Mode, bool Rest>
+__device__ __forceinline__ void rt_scores(float (&l)[V], RtScores<V>& s) {
+    if (rt_scores_try<V, Mode, Rest, false>(l, s)) return;
+    rt_clean<V>(l);
+    rt_scores_try<V, Mode, Rest, true>(l, s);
 }
 
-// Over the CTA, in a fixed order; the result is every thread's.
-__device__ __forceinline__ double rt_block_sum(double v, double* part) {
+// Sums over the CTA, in a fixed order; the results are every thread's.
+template <int N>
+__device__ __forceinline__ void rt_block_sum(double (&v)[N], double (*part)[N]) {
     #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int n = 0; n < N; ++n) {
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        #pragma unroll
+        for (int n = 0; n < N; ++n) part[threadIdx.x >> 5][n] = v[n];
+    }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) v += part[w];
-    return v;
+    #pragma unroll
+    for (int n = 0; n < N; ++n) {
+        v[n] = 0.0;
+        #pragma unroll
+        for (int w = 0; w < kRtWarps; ++w) v[n] += part[w][n];
+    }
 }
 
-// Counts, mean probabilities and losses from the sums, by one CTA.
-__device__ __forceinline__ void rt_balance_end(const RtParams& q, int z_parts, double* part) {
-    double live = 0.0, all = 0.0, z = 0.0, balance = 0.0;
+// Counts and mean probabilities of the cells `first`, `first + stride`, ... (of all threads that take part); what they add to the balance loss.
+__device__ __forceinline__ double rt_balance_cells(const RtParams& q, long long first, long long stride) {
+    constexpr int kBatch = 4;                // cells in flight
+    const long long cells = static_cast<long long>(q.S) * q.E;
+    double balance = 0.0;
+    for (long long i0 = first; i0 < cells; i0 += kBatch * stride) {
+        unsigned long long sum[kBatch];
+        int count[kBatch], n[kBatch];
+        #pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const long long i = i0 + b * stride;
+            const bool there = i < cells;
+            sum[b] = there ? __ldcg(q.sums + i) : 0ull;
+            count[b] = there ? __ldcg(q.sum_counts + i) : 0;
+            n[b] = there ? __ldcg(q.sum_tokens + (q.S == 1 ? 0 : static_cast<int>(static_cast<uint32_t>(i) / static_cast<uint32_t>(q.E)))) : 0;
+        }
+        #pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const long long i = i0 + b * stride;
+            if (i >= cells) break;
+            const double inv = n[b] > 0 ? 1.0 / n[b] : 0.0, mean = static_cast<double>(sum[b]) * (1.0 / static_cast<double>(kRtFixed)) * inv;
+            q.mean[i] = static_cast<float>(mean);
+            q.counts[i] = count[b];
+            balance += static_cast<double>(count[b]) * mean * inv;
+        }
+    }
+    return balance;
+}
+
+// The losses, from what the cells of all CTAs add to the balance loss; by one CTA.
+__device__ __forceinline__ void rt_balance_losses(const RtParams& q, double balance) {
+    __shared__ double part[kRtWarps][4];
+    double v[4] = {0.0, 0.0, 0.0, balance};                  // sequences with tokens, tokens, squares, balance
     for (int s = threadIdx.x; s < q.S; s += blockDim.x) {
         const int n = __ldcg(q.sum_tokens + s);
         q.tokens[s] = n;
-        live += n > 0;
-        all += n;
+        v[0] += n > 0;
+        v[1] += n;
     }
-    for (int i = threadIdx.x; i < z_parts; i += blockDim.x) z += __ldcg(q.z_part + i);
-    for (int s = 0, e = threadIdx.x; ; e += blockDim.x) {
-        while (e >= q.E) { e -= q.E; ++s; }
-        if (s >= q.S) break;
-        const long long i = static_cast<long long>(s) * q.E + e;
-        const int n = __ldcg(q.sum_tokens + s), c = __ldcg(q.sum_counts + i);
-        const double mean = n > 0 ? static_cast<double>(__ldcg(q.sums + i)) / static_cast<double>(kRtFixed) / n : 0.0;
-        q.mean[i] = static_cast<float>(mean);
-        q.counts[i] = c;
-        if (n > 0) balance += static_cast<double>(c) * q.E / (static_cast<double>(q.K) * n) * mean;
-    }
-    live = rt_block_sum(live, part);
-    all = rt_block_sum(all, part);
-    z = rt_block_sum(z, part);
-    balance = rt_block_sum(balance, part);
+    for (int i = threadIdx.x; i < q.z_parts; i += blockDim.x) v[2] += __ldcg(q.z_part + i);
+    rt_block_sum<4>(v, part);
     if (threadIdx.x == 0) {
-        balance = live > 0.0 ? balance / live : 0.0;
-        z = all > 0.0 ? z / all : 0.0;
-        q.losses[0] = static_cast<float>(q.balance_coef * balance + q.z_coef * z);
-        q.losses[1] = static_cast<float>(balance);
+        const double b = v[0] > 0.0 ? v[3] * q.E / q.K / v[0] : 0.0, z = v[1] > 0.0 ? v[2] / v[1] : 0.0;
+        q.losses[0] = static_cast<float>(q.balance_coef * b + q.z_coef * z);
+        q.losses[1] = static_cast<float>(b);
         q.losses[2] = static_cast<float>(z);
     }
 }
 
+// Whether this CTA is the last of the grid to come here; what the others wrote before is visible to it then.
+__device__ __forceinline__ bool rt_last_cta(unsigned* ticket) {
+    __shared__ bool last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();                     // (of what the CTA's threads wrote: the barrier has brought it before this)
+        last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+        __threadfence();
+    }
+    __syncthreads();
+    return last;
+}
+
 // A CTA takes consecutive tokens, piece by piece of one sequence each: its warps add the probabilities up in registers, the CTA adds the warps' sums and puts them to the
-// sequence's. The last CTA to end turns the sums into the results where they are few.
+// sequence's. The last CTA to end turns the sums into the results where they are few. A token's logits are asked for while the one before is worked on.
 template <typename L, int V, int Mode>
-__global__ void __launch_bounds__(kRtWarps * 32) balance_kernel(const RtParams q) {
+__global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(const RtParams q) {
     __shared__ float warp_sum[kRtWarps][V * 32];
     __shared__ int hist[V * 32], warp_tokens[kRtWarps];
-    __shared__ double part[kRtWarps];
-    __shared__ bool last;
+    __shared__ double part[kRtWarps][1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lo = static_cast<int>(static_cast<long long>(q.T) * blockIdx.x / gridDim.x), hi = static_cast<int>(static_cast<long long>(q.T) * (blockIdx.x + 1) / gridDim.x);
     for (int e = threadIdx.x; e < V * 32; e += blockDim.x) hist[e] = 0;
     __syncthreads();
+    float l[V];
+    long long route = -1;
+    // (a warp's tokens are every eighth of the CTA's, whatever the pieces)
+    auto fetch = [&](int r) {
+        if (r < hi) {
+            rt_fetch<L, V>(q, r, lane, l);
+            route = lane < q.K ? q.idx[static_cast<long long>(r) * q.K + lane] : -1;
+        }
+    };
+    int mine = lo + warp;                                                // this warp's next token
+    fetch(mine);
     double z = 0.0;
     int row = lo;
     while (row < hi) {
         int s = 0, end = hi;
         if (q.cu != nullptr) {
             const int first = q.cu[0];
-            if (row < first) { row = min(first, hi); continue; }
-            s = rt_sequence(q.cu, q.S, row);
-            if (s >= q.S) break;
-            end = min(hi, q.cu[s + 1]);
+            if (row < first) {
+                s = -1;
+                end = min(hi, first);
+            } else {
+                s = rt_sequence(q.cu, q.S, row);
+                if (s >= q.S) break;
+                end = min(hi, max(q.cu[s + 1], row + 1));
+            }
         }
         end = min(end, row + kRtFlushRows * kRtWarps);
         float acc[V] = {};
         int n = 0;
-        for (int r = row + warp; r < end; r += kRtWarps) {
-            const long long e = lane < q.K ? q.idx[static_cast<long long>(r) * q.K + lane] : -1;
-            const bool slot = e >= 0 && e < q.E;
-            float l[V], p[V], soft[V], rest[V];
-            rt_load<L, V>(q, r, lane, l);
+        for (; mine < end; mine += kRtWarps) {
+            float x[V];
+            RtScores<V> scores;
+            #pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = l[j];
+            const long long e = route;
+            fetch(mine + kRtWarps);
+            const bool slot = s >= 0 && e >= 0 && e < q.E;
             if (__ballot_sync(0xffffffffu, slot) == 0u) continue;
             if (slot) atomicAdd(hist + e, 1);
-            const float lse = rt_probabilities<V, Mode, false>(l, p, soft, rest);
+            rt_scores<V, Mode, false>(x, scores);
             #pragma unroll
-            for (int j = 0; j < V; ++j) acc[j] += p[j];
-            z += static_cast<double>(lse) * static_cast<double>(lse);
+            for (int j = 0; j < V; ++j) acc[j] = Mode == 1 ? fmaf(scores.sig[j], scores.sig_scale, acc[j]) : fmaf(scores.exp[j], scores.exp_scale, acc[j]);
+            z += static_cast<double>(scores.lse) * static_cast<double>(scores.lse);
             ++n;
         }
+        row = end;
+        if (s < 0) continue;
         #pragma unroll
         for (int j = 0; j < V; ++j) warp_sum[warp][j * 32 + lane] = acc[j];
         if (lane == 0) warp_tokens[warp] = n;
@@ -402,34 +469,32 @@ __global__ void __launch_bounds__(kRtWarps * 32) balance_kernel(const RtParams q
             if (all > 0) atomicAdd(q.sum_tokens + s, all);
         }
         __syncthreads();
-        row = end;
     }
-    z = rt_block_sum(lane == 0 ? z : 0.0, part);
-    if (threadIdx.x == 0) {
-        q.z_part[blockIdx.x] = z;
-        last = false;
-    }
-    if (static_cast<long long>(q.S) * q.E > kRtEndCells) return;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(q.ticket, 1u) == gridDim.x - 1;
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    rt_balance_end(q, gridDim.x, part);
+    double sum[1] = {lane == 0 ? z : 0.0};
+    rt_block_sum<1>(sum, part);
+    if (threadIdx.x == 0) q.z_part[blockIdx.x] = sum[0];
+    if (static_cast<long long>(q.S) * q.E > kRtEndCells || !rt_last_cta(q.ticket)) return;
+    rt_balance_losses(q, rt_balance_cells(q, threadIdx.x, blockDim.x));
 }
 
+// The same for many sums: by as many CTAs as there are thousands of them; the last one adds up what the others found.
 template <typename L>
-__global__ void __launch_bounds__(1024) balance_end_kernel(const RtParams q, int z_parts) {
-    __shared__ double part[32];
-    rt_balance_end(q, z_parts, part);
+__global__ void __launch_bounds__(kRtWarps * 32) balance_end_kernel(const RtParams q) {
+    __shared__ double part[kRtWarps][1];
+    double balance[1] = {rt_balance_cells(q, static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x, static_cast<long long>(gridDim.x) * blockDim.x)};
+    rt_block_sum<1>(balance, part);
+    if (threadIdx.x == 0) q.end_part[blockIdx.x] = balance[0];
+    if (!rt_last_cta(q.ticket)) return;
+    double all = 0.0;
+    for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += blockDim.x) all += __ldcg(q.end_part + i);
+    rt_balance_losses(q, all);
 }
 
 // ----------------------------------------------------------------------------- gradient
 // Consecutive tokens to a warp: the factors of a sequence's experts stay in registers. The routes' gradients, one per lane, get to their experts' lanes through a row in
 // shared memory that is zero between the tokens.
 template <typename L, int V, int Mode>
-__global__ void __launch_bounds__(kRtWarps * 32) router_backward_kernel(const RtParams q) {
+__global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) router_backward_kernel(const RtParams q) {
     __shared__ float rows[kRtWarps][V * 32];
     __shared__ int part_live[kRtWarps];
     __shared__ long long part_all[kRtWarps];
@@ -463,12 +528,23 @@ __global__ void __launch_bounds__(kRtWarps * 32) router_backward_kernel(const Rt
     const int lo = static_cast<int>(static_cast<long long>(q.T) * warp / warps), hi = static_cast<int>(static_cast<long long>(q.T) * (warp + 1) / warps);
     const float zc = 2.f * q.z_coef * g / all;
     int seq = -1, seq_end = -1;
-    float c[V];
+    float c[V], ahead[V], dw_ahead = 0.f;
+    long long e_ahead = -1;
+    auto fetch = [&](int row) {
+        if (row < hi) {
+            rt_fetch<L, V>(q, row, lane, ahead);
+            e_ahead = lane < q.K ? q.idx[static_cast<long long>(row) * q.K + lane] : -1;
+            dw_ahead = q.d_weights != nullptr && lane < q.K ? q.d_weights[static_cast<long long>(row) * q.K + lane] : 0.f;
+        }
+    };
+    fetch(lo);
     for (int row = lo; row < hi; ++row) {
         float l[V], d[V];
-        const long long e64 = lane < q.K ? q.idx[static_cast<long long>(row) * q.K + lane] : -1;
-        const float dw_in = q.d_weights != nullptr && lane < q.K ? q.d_weights[static_cast<long long>(row) * q.K + lane] : 0.f;
-        rt_load<L, V>(q, row, lane, l);
+        #pragma unroll
+        for (int j = 0; j < V; ++j) l[j] = ahead[j];
+        const long long e64 = e_ahead;
+        const float dw_in = dw_ahead;
+        fetch(row + 1);
         const int e = e64 >= 0 && e64 < q.E ? static_cast<int>(e64) : -1;
         const bool routed = __ballot_sync(0xffffffffu, e >= 0) != 0u;
         #pragma unroll
@@ -489,18 +565,17 @@ __global__ void __launch_bounds__(kRtWarps * 32) router_backward_kernel(const Rt
                     c[j] = s < q.S && j * 32 + lane < q.E ? f * static_cast<float>(q.counts[static_cast<long long>(s) * q.E + j * 32 + lane]) : 0.f;
             }
             if (seq < q.S) {
-                float p[V], soft[V], rest[V];
-                const float lse = rt_probabilities<V, Mode, true>(l, p, soft, rest);
+                RtScores<V> x;
+                rt_scores<V, Mode, true>(l, x);
                 float inner = 0.f;
                 #pragma unroll
-                for (int j = 0; j < V; ++j) inner += c[j] * p[j];
-                inner = rt_sum(inner);
-                const float zl = zc * lse;
+                for (int j = 0; j < V; ++j) inner = fmaf(c[j], Mode == 1 ? x.sig[j] : x.exp[j], inner);
+                inner = rt_sum(inner) * (Mode == 1 ? x.sig_scale : x.exp_scale);
+                const float zl = zc * x.lse;
                 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    d[j] = p[j] * (c[j] - inner);
-                    if (Mode == 1) d[j] *= rest[j];
-                    d[j] += zl * soft[j];
+                    if (Mode == 1) d[j] = fmaf(x.sig[j] * x.rest[j], x.sig_scale * (c[j] - inner), x.exp[j] * (x.exp_scale * zl));
+                    else d[j] = x.exp[j] * (x.exp_scale * (c[j] - inner + zl));
                 }
             }
         }
@@ -512,10 +587,10 @@ __global__ void __launch_bounds__(kRtWarps * 32) router_backward_kernel(const Rt
                 if (mine > rt_off()) { w = rt_sigmoid(mine); rest = rt_sigmoid_rest(mine); }
             } else {
                 const float top = rt_max(mine);
-                if (mine > rt_off()) w = expf(mine - top);
+                if (mine > rt_off()) w = rt_exp(mine - top);
             }
             const float total = rt_sum(w);
-            w = total > 0.f ? w / total : 0.f;
+            w = total > 0.f ? w * rt_rcp(total) : 0.f;
             const float inner = rt_sum(w * dw);
             const float dk = w * (dw - inner) * rest;
             // an expert that the token names twice shows by the lane that another one's number has taken the place of
@@ -550,17 +625,22 @@ __global__ void __launch_bounds__(kRtWarps * 32) router_backward_kernel(const Rt
 // ----------------------------------------------------------------------------- launches
 template <typename L, int V, int Mode>
 int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
-    const int blocks = (q.T + kRtWarps - 1) / kRtWarps;
+    const int blocks = (q.T + kRtWarps - 1) / kRtWarps, resident = rt_ctas<V>() * sms;
     if (op == kRtBalance) {
-        // (tokens to spare for each warp's sums: four of them)
-        const int want = (blocks + 3) / 4, grid = want < 1 ? 1 : (want < kRtBalanceCtas ? want : kRtBalanceCtas);
-        balance_kernel<L, V, Mode><<<grid, kRtWarps * 32, 0, stream>>>(q);
-        MM_CUDA(cudaGetLastError());
-        if (static_cast<long long>(q.S) * q.E > kRtEndCells) balance_end_kernel<L><<<1, 1024, 0, stream>>>(q, grid);
+        RtParams b = q;
+        const int most = resident < kRtBalanceCtas ? resident : kRtBalanceCtas;
+        b.z_parts = blocks < 1 ? 1 : (blocks < most ? blocks : most);
+        balance_kernel<L, V, Mode><<<b.z_parts, kRtWarps * 32, 0, stream>>>(b);
+        const long long cells = static_cast<long long>(q.S) * q.E;
+        if (cells > kRtEndCells) {
+            MM_CUDA(cudaGetLastError());
+            const long long want = cells / 2048;
+            balance_end_kernel<L><<<static_cast<int>(want < kRtBalanceCtas ? want : kRtBalanceCtas), kRtWarps * 32, 0, stream>>>(b);
+        }
+    } else if (op == kRtRoute) {
+        route_kernel<L, V, Mode><<<blocks < sms * 8 ? blocks : sms * 8, kRtWarps * 32, 0, stream>>>(q);
     } else {
-        const int grid = blocks < sms * 8 ? blocks : sms * 8;
-        if (op == kRtRoute) route_kernel<L, V, Mode><<<grid, kRtWarps * 32, 0, stream>>>(q);
-        else router_backward_kernel<L, V, Mode><<<grid, kRtWarps * 32, 0, stream>>>(q);
+        router_backward_kernel<L, V, Mode><<<blocks < resident ? blocks : resident, kRtWarps * 32, 0, stream>>>(q);
     }
     MM_CUDA(cudaGetLastError());
     return MM_OK;

@@ -8,7 +8,7 @@ namespace mm {
 
 constexpr int kRtMaxExperts = 1024, kRtMaxTopk = 32, kRtWarps = 8;
 constexpr int kRtBalanceCtas = 1184;         // of the balance kernel at most (eight per SM of 148): the workspace does not depend on the device
-constexpr int kRtEndCells = 16384;           // counts that the balance kernel's last CTA turns into the results itself; more of them get a launch of their own
+constexpr int kRtEndCells = 8192;            // counts that the balance kernel's last CTA turns into the results itself; more of them get a launch of their own
 
 struct RtParams {
     const void* logits;
@@ -31,8 +31,8 @@ struct RtParams {
     int* sum_counts;                         // [S][E]
     int* sum_tokens;                         // [S]
     unsigned* ticket;
-    double* z_part;                          // one per CTA (not zeroed)
-    int balance;
+    double *z_part, *end_part;               // one per CTA (not zeroed)
+    int z_parts, balance;
     void* d_logits;
     long long d_logits_ld;
 };
