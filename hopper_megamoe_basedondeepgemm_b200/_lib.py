@@ -82,7 +82,6 @@ class MMBalanceArgs(ctypes.Structure):
                [(n, ctypes.c_void_p) for n in ('counts', 'seq_tokens', 'mean_probs', 'losses')]
 
 
-GATE = {'none': 0, 'channel': 1, 'token': 2, 'element': 3}
 STATIC_SCRATCH_BYTES = 24 * 1024 * 1024 + 128 * 1024
 TUNE = {'knobs': 0, 'stages': 1, 'prefetch_w1_experts': 2, 'prefetch_w2_experts': 3, 'row_cache': 4}
 KNOB_PREFETCH, KNOB_OWN_ROWS, KNOB_EARLY_COMBINE = 1, 2, 4
@@ -138,7 +137,7 @@ def load(check: bool = False) -> ctypes.CDLL:
     lib.mm_window_alloc.argtypes = [ctypes.c_int64, P(ctypes.c_void_p), ctypes.c_char_p]
     lib.mm_window_open.argtypes = [ctypes.c_char_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, P(ctypes.c_void_p)]
     lib.mm_window_close.argtypes = [P(ctypes.c_void_p), ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
-    # (the Python side hands these structures over as packed bytes)
+    # (the package's own calls of these go through the compiled binding)
     lib.mm_block_norm.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
     lib.mm_block_norm_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32]
     lib.mm_block_norm_workspace_bytes.restype = ctypes.c_int64

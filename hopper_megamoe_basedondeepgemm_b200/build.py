@@ -1,6 +1,7 @@
 """Ahead-of-time build of the CUDA library for sm_100a (in-tree shared object, no JIT cache)."""
 import os
 import subprocess
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, 'csrc')
@@ -8,6 +9,9 @@ LIB_NAME = 'libmegamoe_b200.so'
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 # test build: the same library plus the CUDA-core cross-check engine (`engine='check'`), loaded by the tests only
 CHECK_LIB_PATH = os.path.join(PKG_DIR, 'libmegamoe_b200_check.so')
+# Python binding of the operators around the layer: plain C++ on the C ABI and torch's tensors
+BINDING_PATH = os.path.join(PKG_DIR, 'mm_block_binding.so')
+BINDING_SOURCE = 'mm_block_binding.cpp'
 # each source with the headers it is made from
 _ABI = os.path.join('..', '..', 'include', 'megamoe_b200.h')
 SOURCES = {
@@ -34,7 +38,7 @@ def _run(cmds):
     out = [p.communicate()[0] for p in running]
     for p, text in zip(running, out):
         if p.returncode != 0:
-            raise RuntimeError(f'nvcc failed:\n{text}')
+            raise RuntimeError(f'{p.args[0]} failed:\n{text}')
     return ''.join(out)
 
 
@@ -44,6 +48,8 @@ def build(force: bool = False, verbose: bool = False, check: bool = False) -> st
     path = CHECK_LIB_PATH if check else LIB_PATH
     inputs = [os.path.join(CSRC, f) for s in SOURCES for f in [s] + SOURCES[s]]
     if not force and not _stale(path, inputs):
+        if not check:
+            _build_binding(False)
         return path
     nvcc = os.environ.get('NVCC', '/usr/local/cuda/bin/nvcc')
     os.makedirs(OBJ_DIR, exist_ok=True)
@@ -58,9 +64,27 @@ def build(force: bool = False, verbose: bool = False, check: bool = False) -> st
                         (['-DMM_WITH_CHECK_ENGINE'] if own else []) + [os.path.join(CSRC, source)])
     text = _run(cmds)
     _run([[nvcc, '-gencode', 'arch=compute_100a,code=sm_100a', '-shared', '-Xcompiler', '-fPIC', '-o', path] + objects])
+    if not check:
+        text += _build_binding(force)
     if verbose:
         print(text)
     return path
+
+
+def _build_binding(force: bool) -> str:
+    """Compile the Python binding against the installed torch and the library next to it; returns what the compiler printed."""
+    inputs = [os.path.join(CSRC, BINDING_SOURCE), os.path.join(CSRC, _ABI)]
+    if not force and not _stale(BINDING_PATH, inputs):
+        return ''
+    import importlib.util
+    torch_dir = os.path.dirname(importlib.util.find_spec('torch').origin)
+    include = [os.path.join(torch_dir, 'include'), os.path.join(torch_dir, 'include', 'torch', 'csrc', 'api', 'include'), '/usr/local/cuda/include',
+               sysconfig.get_paths()['include']]
+    # (the system's compiler, whatever CXX names: a binding with a C++ library of its own in it would not share torch's)
+    cxx = '/usr/bin/g++' if os.path.exists('/usr/bin/g++') else 'g++'
+    return _run([[cxx, '-O2', '-std=c++17', '-shared', '-fPIC', '-fvisibility=hidden', '-o', BINDING_PATH] + [f'-I{i}' for i in include] +
+                 [inputs[0], f'-L{PKG_DIR}', f'-l:{LIB_NAME}', f'-L{os.path.join(torch_dir, "lib")}', '-lc10', '-lc10_cuda', '-ltorch_cpu', '-ltorch_cuda',
+                  '-ltorch_python', '-Wl,-rpath,$ORIGIN']])
 
 
 if __name__ == '__main__':

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import hopper_megamoe_basedondeepgemm_b200 as mm
-from hopper_megamoe_basedondeepgemm_b200 import _lib, block, router
+from hopper_megamoe_basedondeepgemm_b200 import _lib
 
 INVALID, UNSUPPORTED = 1, 2
 A = 1 << 20                                   # stand-in addresses, a MiB apart: nothing is read or written before the checks are through
@@ -50,19 +50,13 @@ def _balance(**kw):
     return b
 
 
-def test_packed_arguments_are_the_headers_structures():
-    """The Python side hands the structures over as packed bytes: the same sizes and offsets as the ctypes mirror, and that mirror as the header."""
+def test_ctypes_mirror_matches_the_header():
+    """Sizes and offsets of the structures in the ctypes mirror, as a C compiler sees them in the header."""
     import os
     import re
     import shutil
     import subprocess
     import tempfile
-    for packed, mirror in ((block._NORM_ARGS, _lib.MMBlockNormArgs), (block._GRAD_ARGS, _lib.MMBlockNormGrads),
-                           (router._ROUTER_ARGS, _lib.MMRouterArgs), (router._BALANCE_ARGS, _lib.MMBalanceArgs)):
-        assert packed.size == ctypes.sizeof(mirror)
-        values = list(range(1, len(mirror._fields_) + 1))
-        got = mirror.from_buffer_copy(packed.pack(*values))
-        assert [getattr(got, f[0]) for f in mirror._fields_] == values
     if shutil.which('gcc') is None:
         pytest.skip('no C compiler')
     include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'include')
@@ -77,7 +71,7 @@ def test_packed_arguments_are_the_headers_structures():
     want = [v for m in names.values() for v in [ctypes.sizeof(m)] + [getattr(m, f[0]).offset for f in m._fields_]]
     assert out == want
     enums = re.findall(r'MM_(?:DTYPE|GATE)_\w+ = \d', open(os.path.join(include, 'megamoe_b200.h')).read())
-    assert len(enums) == 7 and block._DTYPE == {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+    assert len(enums) == 7
 
 
 @pytest.mark.parametrize('change, status', [
