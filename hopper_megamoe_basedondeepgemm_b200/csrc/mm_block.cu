@@ -263,7 +263,7 @@ int mm_balance_loss(const mm_router_args_t* a, const mm_balance_args_t* b, void*
     q.ticket = reinterpret_cast<unsigned*>(q.sum_tokens + q.S);
     q.z_part = reinterpret_cast<double*>(static_cast<char*>(workspace) + zeroed);
     q.end_part = q.z_part + mm::kRtBalanceCtas;
-    MM_CUDA(cudaMemsetAsync(workspace, 0, zeroed, static_cast<cudaStream_t>(stream_ptr)));
+    q.zero_words = zeroed / 8;
     return launch_router(a->dtype, mm::kRtBalance, q, stream_ptr);
 }
 

@@ -31,6 +31,8 @@
 #include "../../include/megamoe_b200.h"
 #include "mm_block_norm.h"
 #include "mm_error.h"
+#include "mm_launch.h"
+#include "mm_ptx.cuh"
 
 namespace mm {
 
@@ -631,6 +633,7 @@ __global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_backward_kernel(c
     int row = blockIdx.x;
     if (Post) fetch_y(row, ry);
     fetch(row);
+    grid_launch_dependents();                                // (the sums' kernel waits for this one's end by itself)
     if (on) {
         if (kY) bn_y_factor<X, Vec>(q, a);
         if (Pre) bn_pre_factor<X, Vec>(q, w);
@@ -751,10 +754,11 @@ __global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_backward_kernel(c
 template <typename X>
 __global__ void __launch_bounds__(256) block_norm_sums_kernel(const BnSumsParams q) {
     __shared__ float part[32][33];
-    const int col = (threadIdx.x & 7) * 4, group = threadIdx.x >> 3, h0 = blockIdx.x * 32;
-    const bool of_pre = q.d_pre_w != nullptr && blockIdx.y == 0;
+    const int col = (threadIdx.x & 7) * 4, group = threadIdx.x >> 3, blocks = (q.hidden + 31) / 32, which = blockIdx.x / blocks, h0 = (blockIdx.x - which * blocks) * 32;
+    const bool of_pre = q.d_pre_w != nullptr && which == 0;
     float v[4] = {};
-    const float* p = q.partial + static_cast<long long>(blockIdx.y) * q.rows * q.hidden + h0 + col;
+    const float* p = q.partial + static_cast<long long>(which) * q.rows * q.hidden + h0 + col;
+    grid_dependency_wait();
     if ((q.hidden & 3) == 0) {
         if (h0 + col < q.hidden) {
             #pragma unroll 8
@@ -844,8 +848,7 @@ int bn_launch(const BnParams& q, const BnLaunch& how, cudaStream_t stream) {
 
 template <typename X>
 int bn_launch_sums(const BnSumsParams& q, cudaStream_t stream) {
-    block_norm_sums_kernel<X><<<dim3((q.hidden + 31) / 32, q.sums), 256, 0, stream>>>(q);
-    MM_CUDA(cudaGetLastError());
+    MM_CUDA(launch_behind(block_norm_sums_kernel<X>, (q.hidden + 31) / 32 * q.sums, 256, stream, q));
     return MM_OK;
 }
 

@@ -1,0 +1,19 @@
+// A launch that may begin before the kernel ahead of it in its stream has ended: its launch and the part of it before `grid_dependency_wait` overlap with that kernel's
+// end. What that kernel (and, by its own order, those ahead of it) wrote is there after the wait.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace mm {
+
+template <typename P>
+cudaError_t launch_behind(void (*kernel)(P), unsigned grid, unsigned threads, cudaStream_t stream, const P& params) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(threads); cfg.stream = stream;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, params);
+}
+
+}  // namespace mm

@@ -23,6 +23,8 @@
 
 #include "../../include/megamoe_b200.h"
 #include "mm_error.h"
+#include "mm_launch.h"
+#include "mm_ptx.cuh"
 #include "mm_router.h"
 
 namespace mm {
@@ -155,20 +157,22 @@ __global__ void __launch_bounds__(kRtWarps * 32) route_kernel(const RtParams q) 
                 #pragma unroll
                 for (int j = 0; j < V; ++j) key[j] = q.bias != nullptr && j * 32 + lane < q.E ? __ldg(q.bias + j * 32 + lane) : 0.f;
             }
-            rt_clean<V>(l);
-            float best = rt_off();
+            float best = rt_off();                                       // (NaN is no maximum, and not below: not a candidate)
             #pragma unroll
             for (int j = 0; j < V; ++j) {
-                key[j] = Mode == 1 ? (l[j] == rt_off() ? rt_off() : fmaxf(rt_sigmoid(l[j]) + key[j], rt_off())) : l[j];
+                key[j] = Mode == 1 ? (l[j] > rt_off() ? rt_sigmoid(l[j]) + key[j] : rt_off()) : l[j];
                 best = fmaxf(best, key[j]);
             }
+            if (Mode == 0 && rt_max(best) > FLT_MAX) {                   // infinities count as the largest number
+                best = fminf(best, FLT_MAX);
+                #pragma unroll
+                for (int j = 0; j < V; ++j) key[j] = l[j] = rt_logit(l[j]);
+            }
+            // lanes of one maximum are taken at once: the bound is then lower than it has to be
             uint32_t mine = best == rt_off() ? 0u : rt_order(best), high = 0u;
-            for (int n = 0; n < q.K;) {
+            for (int k = 0; k < q.K; ++k) {
                 high = __reduce_max_sync(0xffffffffu, mine);
-                if (high == 0u) break;
-                const bool is = mine == high;
-                n += __popc(__ballot_sync(0xffffffffu, is));
-                if (is) mine = 0u;
+                mine = mine == high ? 0u : mine;
             }
             float bound = -FLT_MAX;                                      // (what is on; in mode 1 with an infinite bias, too)
             if (high != 0u) {
@@ -186,6 +190,7 @@ __global__ void __launch_bounds__(kRtWarps * 32) route_kernel(const RtParams q) 
                     n += __popc(who);
                 }
             }
+            if (lane >= n && lane < ((n + 3) & ~3)) cand_key[warp][lane] = rt_off();       // (goes before none)
             __syncwarp();
             if (n > 32) {
                 at = rt_route_any<L, Mode>(static_cast<const L*>(q.logits) + static_cast<long long>(row) * q.logits_ld, q.bias, q.E, q.K);
@@ -197,19 +202,18 @@ __global__ void __launch_bounds__(kRtWarps * 32) route_kernel(const RtParams q) 
             } else {
                 float mine_key = rt_off();
                 if (lane < n) { mine_key = cand_key[warp][lane]; at = cand_at[warp][lane]; logit = Mode == 1 ? cand_logit[warp][lane] : mine_key; }
-                int before = 0;
-                bool close = false;
+                int before = 0, near = 0;                                // candidates that go before this one; in mode 1 those that may or may not, itself among them
                 const float margin = Mode == 1 ? rt_key_margin(mine_key) : 0.f;
                 for (int c = 0; c < n; c += 4) {
                     const float4 k4 = *reinterpret_cast<const float4*>(&cand_key[warp][c]);
                     const float ks[4] = {k4.x, k4.y, k4.z, k4.w};
                     #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const bool there = c + i < n;
-                        before += there && (ks[i] > mine_key || (ks[i] == mine_key && c + i < lane));
-                        if (Mode == 1) close = close || (there && c + i != lane && !(fabsf(ks[i] - mine_key) > margin));
+                        before += c + i < lane ? ks[i] >= mine_key : ks[i] > mine_key;
+                        if (Mode == 1) near += !(fabsf(ks[i] - mine_key) > margin);
                     }
                 }
+                const bool close = near != 1;
                 if (Mode == 1) {
                     if (__ballot_sync(0xffffffffu, close && lane < n) != 0u) {
                         const double key64 = lane < n ? 1.0 / (1.0 + exp(-static_cast<double>(logit))) + (q.bias != nullptr ? static_cast<double>(__ldg(q.bias + at)) : 0.0) : 0.0;
@@ -332,25 +336,25 @@ __device__ __forceinline__ void rt_block_sum(double (&v)[N], double (*part)[N]) 
 
 // Counts and mean probabilities of the cells `first`, `first + stride`, ... (of all threads that take part); what they add to the balance loss.
 __device__ __forceinline__ double rt_balance_cells(const RtParams& q, long long first, long long stride) {
-    constexpr int kBatch = 4;                // cells in flight
+    constexpr int kBatch = 6;                // cells in flight
     const long long cells = static_cast<long long>(q.S) * q.E;
+    const float inv_fixed = 1.f / kRtFixed;
     double balance = 0.0;
     for (long long i0 = first; i0 < cells; i0 += kBatch * stride) {
         unsigned long long sum[kBatch];
         int count[kBatch], n[kBatch];
         #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            const long long i = i0 + b * stride;
-            const bool there = i < cells;
-            sum[b] = there ? __ldcg(q.sums + i) : 0ull;
-            count[b] = there ? __ldcg(q.sum_counts + i) : 0;
-            n[b] = there ? __ldcg(q.sum_tokens + (q.S == 1 ? 0 : static_cast<int>(static_cast<uint32_t>(i) / static_cast<uint32_t>(q.E)))) : 0;
+            const long long i = min(i0 + b * stride, cells - 1);
+            sum[b] = __ldcg(q.sums + i);
+            count[b] = __ldcg(q.sum_counts + i);
+            n[b] = __ldcg(q.sum_tokens + (q.S == 1 ? 0 : static_cast<int>(static_cast<uint32_t>(i) / static_cast<uint32_t>(q.E))));
         }
         #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const long long i = i0 + b * stride;
             if (i >= cells) break;
-            const double inv = n[b] > 0 ? 1.0 / n[b] : 0.0, mean = static_cast<double>(sum[b]) * (1.0 / static_cast<double>(kRtFixed)) * inv;
+            const double inv = n[b] > 0 ? 1.0 / n[b] : 0.0, mean = static_cast<double>(sum[b]) * inv_fixed * inv;
             q.mean[i] = static_cast<float>(mean);
             q.counts[i] = count[b];
             balance += static_cast<double>(count[b]) * mean * inv;
@@ -392,6 +396,13 @@ __device__ __forceinline__ bool rt_last_cta(unsigned* ticket) {
     return last;
 }
 
+template <typename L>
+__global__ void __launch_bounds__(256) balance_zero_kernel(const RtParams q) {
+    grid_launch_dependents();
+    unsigned long long* p = q.sums;
+    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < q.zero_words; i += static_cast<long long>(gridDim.x) * blockDim.x) p[i] = 0ull;
+}
+
 // A CTA takes consecutive tokens, piece by piece of one sequence each: its warps add the probabilities up in registers, the CTA adds the warps' sums and puts them to the
 // sequence's. The last CTA to end turns the sums into the results where they are few. A token's logits are asked for while the one before is worked on.
 template <typename L, int V, int Mode>
@@ -416,6 +427,7 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
     fetch(mine);
     double z = 0.0;
     int row = lo;
+    bool zeroed = false;
     while (row < hi) {
         int s = 0, end = hi;
         if (q.cu != nullptr) {
@@ -450,6 +462,7 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
         }
         row = end;
         if (s < 0) continue;
+        if (!zeroed) { grid_dependency_wait(); zeroed = true; }              // (the sums are zero now)
         #pragma unroll
         for (int j = 0; j < V; ++j) warp_sum[warp][j * 32 + lane] = acc[j];
         if (lane == 0) warp_tokens[warp] = n;
@@ -470,6 +483,7 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
         }
         __syncthreads();
     }
+    if (!zeroed) grid_dependency_wait();
     double sum[1] = {lane == 0 ? z : 0.0};
     rt_block_sum<1>(sum, part);
     if (threadIdx.x == 0) q.z_part[blockIdx.x] = sum[0];
@@ -626,11 +640,16 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) router_backward_k
 template <typename L, int V, int Mode>
 int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
     const int blocks = (q.T + kRtWarps - 1) / kRtWarps, resident = rt_ctas<V>() * sms;
+    // a token for a warp up to a CTA an SM, then up to four, then as many CTAs as there is room for: what a CTA does once is that of a few tokens
+    int grid = blocks <= sms ? (blocks > 0 ? blocks : 1) : (blocks / 4 > sms ? blocks / 4 : sms);
+    if (grid > resident) grid = resident;
     if (op == kRtBalance) {
         RtParams b = q;
-        const int most = resident < kRtBalanceCtas ? resident : kRtBalanceCtas;
-        b.z_parts = blocks < 1 ? 1 : (blocks < most ? blocks : most);
-        balance_kernel<L, V, Mode><<<b.z_parts, kRtWarps * 32, 0, stream>>>(b);
+        b.z_parts = grid < kRtBalanceCtas ? grid : kRtBalanceCtas;
+        const long long zero = (b.zero_words + 1023) / 1024;
+        balance_zero_kernel<L><<<static_cast<int>(zero < sms ? zero : sms), 256, 0, stream>>>(b);
+        MM_CUDA(cudaGetLastError());
+        MM_CUDA(launch_behind(balance_kernel<L, V, Mode>, b.z_parts, kRtWarps * 32, stream, b));
         const long long cells = static_cast<long long>(q.S) * q.E;
         if (cells > kRtEndCells) {
             MM_CUDA(cudaGetLastError());
@@ -640,7 +659,7 @@ int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
     } else if (op == kRtRoute) {
         route_kernel<L, V, Mode><<<blocks < sms * 8 ? blocks : sms * 8, kRtWarps * 32, 0, stream>>>(q);
     } else {
-        router_backward_kernel<L, V, Mode><<<blocks < resident ? blocks : resident, kRtWarps * 32, 0, stream>>>(q);
+        router_backward_kernel<L, V, Mode><<<grid, kRtWarps * 32, 0, stream>>>(q);
     }
     MM_CUDA(cudaGetLastError());
     return MM_OK;

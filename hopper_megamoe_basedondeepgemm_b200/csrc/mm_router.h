@@ -26,6 +26,7 @@ struct RtParams {
     int* tokens;                             // [S]
     float* mean;                             // [S][E]
     float* losses;                           // loss, balance, z
+    long long zero_words;                    // of 8 bytes, from `sums` on
     // workspace: zero at first
     unsigned long long* sums;                // [S][E]
     int* sum_counts;                         // [S][E]
