@@ -373,10 +373,20 @@ __device__ __forceinline__ Bn8<__half> bn_pack(const float2 (&v)[4], __half) {
     return r;
 }
 
+// Eight elements on their way: as they will lie in memory, or one to a register, because putting two of them together waits for both.
+template <typename T, bool Vec> struct BnAhead { uint32_t w[Vec || sizeof(T) == 4 ? sizeof(T) * 2 : 8]; };
+template <typename T, bool Vec>
+__device__ __forceinline__ Bn8<T> bn_take(const BnAhead<T, Vec>& a) {
+    Bn8<T> r;
+    #pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) * 2; ++i) r.w[i] = Vec || sizeof(T) == 4 ? a.w[i] : (a.w[(2 * i) & 7] | a.w[(2 * i + 1) & 7] << 16);
+    return r;
+}
+
 // The eight channels of this thread in a row. `Vec`: eight neighbours, in one access (of 32 bytes for 32-bit elements: two of 16 would each move half of
 // every 32-byte sector). Otherwise channels a CTA's width apart, one by one: neighbouring threads still read neighbours.
 template <typename T, bool Vec>
-__device__ __forceinline__ void bn_fetch(const T* row, int hidden, Bn8<T>& r) {
+__device__ __forceinline__ void bn_fetch(const T* row, int hidden, BnAhead<T, Vec>& r) {
     if constexpr (Vec) {
         const T* p = row + static_cast<int>(threadIdx.x) * 8;
         if constexpr (sizeof(T) == 4)
@@ -385,17 +395,13 @@ __device__ __forceinline__ void bn_fetch(const T* row, int hidden, Bn8<T>& r) {
         else
             asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "l"(p) : "memory");
     } else {
-        const int at = static_cast<int>(threadIdx.x), width = static_cast<int>(blockDim.x);
+        int at = static_cast<int>(threadIdx.x);
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int a = at + 2 * i * width, b = a + width;
-            if constexpr (sizeof(T) == 4) {
-                r.w[2 * i] = a < hidden ? reinterpret_cast<const uint32_t*>(row)[a] : 0u;
-                r.w[2 * i + 1] = b < hidden ? reinterpret_cast<const uint32_t*>(row)[b] : 0u;
-            } else {
-                const uint32_t lo = a < hidden ? reinterpret_cast<const uint16_t*>(row)[a] : 0u, hi = b < hidden ? reinterpret_cast<const uint16_t*>(row)[b] : 0u;
-                r.w[i] = lo | hi << 16;
-            }
+        for (int i = 0; i < 8; ++i, at += static_cast<int>(blockDim.x)) {
+            if constexpr (sizeof(T) == 4)
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %2, %3;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "=&r"(r.w[i]) : "l"(row + at), "r"(at), "r"(hidden) : "memory");
+            else
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %2, %3;\n\tmov.b32 %0, 0;\n\t@p ld.global.u16 %0, [%1];\n\t}" : "=&r"(r.w[i]) : "l"(row + at), "r"(at), "r"(hidden) : "memory");
         }
     }
 }
@@ -428,8 +434,8 @@ __device__ __forceinline__ void bn_put(T* row, int hidden, const float2 (&v)[4])
 // weights and gates of the channels
 template <typename X, bool Vec>
 __device__ __forceinline__ void bn_weight(const void* w, int is32, int hidden, float2 (&v)[4]) {
-    if (is32) { Bn8<float> r; bn_fetch<float, Vec>(static_cast<const float*>(w), hidden, r); bn_unpack(r, v); }
-    else { Bn8<X> r; bn_fetch<X, Vec>(static_cast<const X*>(w), hidden, r); bn_unpack(r, v); }
+    if (is32) { BnAhead<float, Vec> r; bn_fetch<float, Vec>(static_cast<const float*>(w), hidden, r); bn_unpack(bn_take(r), v); }
+    else { BnAhead<X, Vec> r; bn_fetch<X, Vec>(static_cast<const X*>(w), hidden, r); bn_unpack(bn_take(r), v); }
 }
 // scale * (channel's gate) * (offset + w_post): the factor of y
 template <typename X, bool Vec>
@@ -470,25 +476,29 @@ __device__ __forceinline__ float bn_gate_value(const BnParams& q, uint32_t bits)
 }
 // an element's gate: of the activations' type or 32 bits, held in room for the latter
 template <typename X, bool Vec>
-__device__ __forceinline__ void bn_fetch_gate(const BnParams& q, long long row, Bn8<float>& r) {
+__device__ __forceinline__ void bn_fetch_gate(const BnParams& q, long long row, uint32_t (&r)[8]) {
     if (sizeof(X) == 4 || q.gate32) {
-        bn_fetch<float, Vec>(static_cast<const float*>(q.gate) + row * q.gate_ld, q.hidden, r);
+        BnAhead<float, Vec> f;
+        bn_fetch<float, Vec>(static_cast<const float*>(q.gate) + row * q.gate_ld, q.hidden, f);
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = f.w[i];
     } else {
-        Bn8<X> h;
+        BnAhead<X, Vec> h;
         bn_fetch<X, Vec>(static_cast<const X*>(q.gate) + row * q.gate_ld, q.hidden, h);
         #pragma unroll
-        for (int i = 0; i < 4; ++i) r.w[i] = h.w[i];
+        for (int i = 0; i < static_cast<int>(sizeof(h.w) / 4); ++i) r[i] = h.w[i];
     }
 }
-template <typename X>
-__device__ __forceinline__ void bn_unpack_gate(const BnParams& q, const Bn8<float>& r, float2 (&g)[4]) {
+template <typename X, bool Vec>
+__device__ __forceinline__ void bn_unpack_gate(const BnParams& q, const uint32_t (&r)[8], float2 (&g)[4]) {
     if (sizeof(X) == 4 || q.gate32) {
-        bn_unpack(r, g);
-    } else {
-        Bn8<X> h;
         #pragma unroll
-        for (int i = 0; i < 4; ++i) h.w[i] = r.w[i];
-        bn_unpack(h, g);
+        for (int i = 0; i < 4; ++i) g[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+    } else {
+        BnAhead<X, Vec> h;
+        #pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(h.w) / 4); ++i) h.w[i] = r[i];
+        bn_unpack(bn_take(h), g);
     }
 }
 
@@ -499,9 +509,10 @@ __device__ __forceinline__ float bn_square(const float2 (&v)[4]) {
     return s.x + s.y;
 }
 template <typename T> __device__ __forceinline__ float bn_square(const Bn8<T>& r) { float2 v[4]; bn_unpack(r, v); return bn_square(v); }
-template <typename T> __device__ __forceinline__ void bn_clear(Bn8<T>& r) {
+template <int N>
+__device__ __forceinline__ void bn_clear(uint32_t (&w)[N]) {
     #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) * 2; ++i) r.w[i] = 0u;
+    for (int i = 0; i < N; ++i) w[i] = 0u;
 }
 
 // What there is in a call, as far as it shapes the loop over the rows.
@@ -510,18 +521,18 @@ enum BnKind { kBnPlain = 0 /* no gate, or one that is part of y's factor */, kBn
 // 64 registers a thread, so two CTAs of 512 threads an SM. 16384 x 4096, 32-bit stream, both norms, channel gate: 130 us (6.2 TB/s); of 8192 x 3072 in bf16 40 us.
 // (One CTA of twice the registers per SM 168 us; sixteen channels a thread 134; rows copied ahead into shared memory by cp.async 160.)
 template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec>
-__global__ void __launch_bounds__(kBnMaxThreads, 2) block_norm_kernel(const BnParams q) {
+__global__ void __maxnreg__((sizeof(R) == 2 && Vec ? 56 : 64)) block_norm_kernel(const BnParams q) {
     __shared__ __align__(16) float part[2][8][kBnSumWarps];
     const float inv_h = 1.f / static_cast<float>(q.hidden);
     const int step = gridDim.x, tokens = static_cast<int>(q.tokens);
     const bool on = !Vec || static_cast<int>(threadIdx.x) * 8 < q.hidden;
-    Bn8<R> rr;
-    Bn8<X> ry;
-    Bn8<float> rg;
+    BnAhead<R, Vec> rr;
+    BnAhead<X, Vec> ry;
+    uint32_t rg[8];
     float2 a[4], w[4];
     uint32_t gate_bits = 0u;
-    bn_clear(rr);
-    bn_clear(ry);
+    bn_clear(rr.w);
+    bn_clear(ry.w);
     bn_clear(rg);
     #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = w[i] = both(0.f);
@@ -543,16 +554,16 @@ __global__ void __launch_bounds__(kBnMaxThreads, 2) block_norm_kernel(const BnPa
     int turn = 0;
     float i1 = 1.f;
     if (Post) {
-        float sum[1] = {bn_square(ry)};
+        float sum[1] = {bn_square(bn_take(ry))};
         bn_sum<1>(sum, part, turn);
         i1 = rsqrtf(sum[0] * inv_h + q.eps);
     }
     while (true) {
         const bool more = row + step < tokens;
         float2 r[4], v[4], g[4];
-        bn_unpack(rr, r);
-        if (Kind != kBnStream) bn_unpack(ry, v);
-        if (Kind == kBnElement) bn_unpack_gate<X>(q, rg, g);
+        bn_unpack(bn_take(rr), r);
+        if (Kind != kBnStream) bn_unpack(bn_take(ry), v);
+        if (Kind == kBnElement) bn_unpack_gate<X, Vec>(q, rg, g);
         const float f = Kind == kBnToken ? i1 * bn_gate_value<X>(q, gate_bits) : i1;
         if (more) fetch(row + step);
         if (Kind != kBnStream) {
@@ -568,7 +579,7 @@ __global__ void __launch_bounds__(kBnMaxThreads, 2) block_norm_kernel(const BnPa
             // the sum of the next row's squares goes with this row's
             float sum[2] = {bn_square(r), 0.f};
             if (Post) {
-                sum[1] = bn_square(ry);
+                sum[1] = bn_square(bn_take(ry));
                 bn_sum<2>(sum, part, turn);
                 i1 = rsqrtf(sum[1] * inv_h + q.eps);
             } else {
@@ -581,7 +592,7 @@ __global__ void __launch_bounds__(kBnMaxThreads, 2) block_norm_kernel(const BnPa
             for (int i = 0; i < 4; ++i) r[i] = mul2(mul2(r[i], i2), w[i]);
             if (on) bn_put<X, Vec>(static_cast<X*>(q.normed) + row * q.normed_ld, q.hidden, r);
         } else if (Post) {
-            float sum[1] = {bn_square(ry)};
+            float sum[1] = {bn_square(bn_take(ry))};
             bn_sum<1>(sum, part, turn);
             i1 = rsqrtf(sum[0] * inv_h + q.eps);
         }
@@ -601,26 +612,27 @@ __global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_backward_kernel(c
     const float inv_h = 1.f / static_cast<float>(q.hidden);
     const int step = gridDim.x, tokens = static_cast<int>(q.tokens);
     const bool on = !Vec || static_cast<int>(threadIdx.x) * 8 < q.hidden, sum_y = Post || q.gate_mode == kBnGateChannel, has_d = q.d_residual_out != nullptr;
-    Bn8<R> rd, rr;
-    Bn8<X> ry, rh, ry_next;
-    Bn8<float> rg;
+    BnAhead<R, Vec> rd, rr;                                  // on their way
+    BnAhead<X, Vec> ry_ahead, rh;
+    Bn8<X> ry;                                               // norm of y: the next row's
+    uint32_t rg[8];
     float2 a[4], w[4], acc_pre[4], acc_y[4];
     uint32_t gate_bits = 0u;
-    bn_clear(rd);
-    bn_clear(rr);
-    bn_clear(ry);
-    bn_clear(rh);
-    bn_clear(ry_next);
+    bn_clear(rd.w);
+    bn_clear(rr.w);
+    bn_clear(ry.w);
+    bn_clear(rh.w);
+    bn_clear(ry_ahead.w);
     bn_clear(rg);
     #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = w[i] = acc_pre[i] = acc_y[i] = both(0.f);
-    auto fetch_y = [&](long long row, Bn8<X>& to) {
-        if (kY && on) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, to);
+    auto fetch_y = [&](long long row) {
+        if (kY && on) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry_ahead);
     };
     auto fetch = [&](long long row) {
         if (on) {
-            if (Post) { if (row + step < tokens) fetch_y(row + step, ry_next); }
-            else fetch_y(row, ry);
+            if (!Post) fetch_y(row);
+            else if (row + step < tokens) fetch_y(row + step);
             if (Pre) {
                 bn_fetch<R, Vec>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, rr);
                 bn_fetch<X, Vec>(static_cast<const X*>(q.d_normed) + row * q.d_normed_ld, q.hidden, rh);
@@ -631,7 +643,7 @@ __global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_backward_kernel(c
         if (Kind == kBnToken) gate_bits = bn_gate_bits<X>(q, row);
     };
     int row = blockIdx.x;
-    if (Post) fetch_y(row, ry);
+    if (Post) { fetch_y(row); ry = bn_take(ry_ahead); }
     fetch(row);
     grid_launch_dependents();                                // (the sums' kernel waits for this one's end by itself)
     if (on) {
@@ -648,12 +660,14 @@ __global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_backward_kernel(c
     }
     while (true) {
         const bool more = row + step < tokens;
-        const Bn8<R> cd = rd;
-        const Bn8<X> cy = ry, ch = rh;
-        const Bn8<float> cg = rg;
+        const Bn8<R> cd = bn_take(rd);
+        const Bn8<X> cy = Post ? ry : bn_take(ry_ahead), ch = bn_take(rh);
+        uint32_t cg[8];
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) cg[i] = rg[i];
         float2 r[4];
-        if (Pre) bn_unpack(rr, r);
-        if (Post) ry = ry_next;
+        if (Pre) bn_unpack(bn_take(rr), r);
+        if (Post) ry = bn_take(ry_ahead);
         const float gate = Kind == kBnToken ? bn_gate_value<X>(q, gate_bits) : 1.f;
         if (more) fetch(row + step);
         float sum[8] = {};                                   // r' r', dh w2 r', v d, v dh w2, v r' (v without a token's gate), next y's squares
@@ -662,7 +676,7 @@ __global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_backward_kernel(c
             #pragma unroll
             for (int k = 0; k < 5; ++k) t[k] = both(0.f);
             if (kY) bn_unpack(cy, v);
-            if (Kind == kBnElement) bn_unpack_gate<X>(q, cg, g);
+            if (Kind == kBnElement) bn_unpack_gate<X, Vec>(q, cg, g);
             if (Pre) bn_unpack(ch, dh);
             if (kSumV) bn_unpack(cd, d);
             #pragma unroll
@@ -719,7 +733,7 @@ __global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_backward_kernel(c
             bn_unpack(cy, y);
             if (Kind == kBnElement) {
                 float2 g[4], dg[4];
-                bn_unpack_gate<X>(q, cg, g);
+                bn_unpack_gate<X, Vec>(q, cg, g);
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     dg[i] = mul2(mul2(Post ? mul2(y[i], both(i1)) : y[i], a[i]), d[i]);
@@ -749,11 +763,12 @@ __global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_backward_kernel(c
     if (sum_y) bn_put<float, Vec>(Pre ? p + static_cast<long long>(gridDim.x) * q.hidden : p, q.hidden, acc_y);
 }
 
-// Column sums of the CTAs' partial sums: a block takes 32 channels of one of the two, a thread every 32nd row of four channels; the threads' sums are added up in
-// shared memory in order. 296 rows of 3072 channels are 3.6 MB that lie in the L2.
+// Column sums of the CTAs' partial sums: a block takes 32 channels of one of the two, a thread every 128th row of four channels, a few loads that are all on their way at
+// once; added up over a warp's four rows by shuffles, then over the warps in order. 148 to 1184 rows that lie in the L2.
+constexpr int kBnSumThreads = 1024;
 template <typename X>
-__global__ void __launch_bounds__(256) block_norm_sums_kernel(const BnSumsParams q) {
-    __shared__ float part[32][33];
+__global__ void __launch_bounds__(kBnSumThreads) block_norm_sums_kernel(const BnSumsParams q) {
+    __shared__ float part[kBnSumThreads / 32][33];
     const int col = (threadIdx.x & 7) * 4, group = threadIdx.x >> 3, blocks = (q.hidden + 31) / 32, which = blockIdx.x / blocks, h0 = (blockIdx.x - which * blocks) * 32;
     const bool of_pre = q.d_pre_w != nullptr && which == 0;
     float v[4] = {};
@@ -761,27 +776,31 @@ __global__ void __launch_bounds__(256) block_norm_sums_kernel(const BnSumsParams
     grid_dependency_wait();
     if ((q.hidden & 3) == 0) {
         if (h0 + col < q.hidden) {
-            #pragma unroll 8
-            for (int r = group; r < q.rows; r += 32) {
+            #pragma unroll 5
+            for (int r = group; r < q.rows; r += kBnSumThreads / 8) {
                 const float4 f = *reinterpret_cast<const float4*>(p + static_cast<long long>(r) * q.hidden);
                 v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
             }
         }
     } else {
-        #pragma unroll 2
-        for (int r = group; r < q.rows; r += 32) {
+        #pragma unroll 5
+        for (int r = group; r < q.rows; r += kBnSumThreads / 8) {
             #pragma unroll
-            for (int i = 0; i < 4; ++i) if (h0 + col + i < q.hidden) v[i] += p[static_cast<long long>(r) * q.hidden + i];
+            for (int i = 0; i < 4; ++i) v[i] += h0 + col + i < q.hidden ? p[static_cast<long long>(r) * q.hidden + i] : 0.f;
         }
     }
     #pragma unroll
-    for (int i = 0; i < 4; ++i) part[group][col + i] = v[i];
+    for (int i = 0; i < 4; ++i) {
+        v[i] += __shfl_xor_sync(0xffffffffu, v[i], 8);
+        v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+        if ((threadIdx.x & 31) < 8) part[threadIdx.x >> 5][col + i] = v[i];
+    }
     __syncthreads();
     const int h = h0 + static_cast<int>(threadIdx.x);
     if (threadIdx.x >= 32 || h >= q.hidden) return;
     float sum = 0.f;
     #pragma unroll
-    for (int g = 0; g < 32; ++g) sum += part[g][threadIdx.x];
+    for (int g = 0; g < kBnSumThreads / 32; ++g) sum += part[g][threadIdx.x];
     auto put = [&](void* to, int is32, float x) {
         if (is32) static_cast<float*>(to)[h] = x; else static_cast<X*>(to)[h] = bn_round<X>(x);
     };
@@ -848,7 +867,7 @@ int bn_launch(const BnParams& q, const BnLaunch& how, cudaStream_t stream) {
 
 template <typename X>
 int bn_launch_sums(const BnSumsParams& q, cudaStream_t stream) {
-    MM_CUDA(launch_behind(block_norm_sums_kernel<X>, (q.hidden + 31) / 32 * q.sums, 256, stream, q));
+    MM_CUDA(launch_behind(block_norm_sums_kernel<X>, (q.hidden + 31) / 32 * q.sums, kBnSumThreads, stream, q));
     return MM_OK;
 }
 
