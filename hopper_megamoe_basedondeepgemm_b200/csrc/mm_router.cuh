@@ -354,26 +354,27 @@ __device__ __forceinline__ double rt_balance_cells(const RtParams& q, long long 
         for (int b = 0; b < kBatch; ++b) {
             const long long i = i0 + b * stride;
             if (i >= cells) break;
-            const double inv = n[b] > 0 ? 1.0 / n[b] : 0.0, mean = static_cast<double>(sum[b]) * inv_fixed * inv;
-            q.mean[i] = static_cast<float>(mean);
+            const float inv = n[b] > 0 ? 1.f / static_cast<float>(n[b]) : 0.f, mean = static_cast<float>(sum[b]) * inv_fixed * inv;
+            q.mean[i] = mean;
             q.counts[i] = count[b];
-            balance += static_cast<double>(count[b]) * mean * inv;
+            balance += static_cast<double>(static_cast<float>(count[b]) * inv) * static_cast<double>(mean);
         }
     }
     return balance;
 }
 
-// The losses, from what the cells of all CTAs add to the balance loss; by one CTA.
-__device__ __forceinline__ void rt_balance_losses(const RtParams& q, double balance) {
+// The results, by one CTA: the losses, and with `cells` all counts and mean probabilities. `balance`: what other CTAs' cells add to the balance loss, in all.
+__device__ __forceinline__ void rt_balance_results(const RtParams& q, bool cells, double balance) {
     __shared__ double part[kRtWarps][4];
     double v[4] = {0.0, 0.0, 0.0, balance};                  // sequences with tokens, tokens, squares, balance
+    for (int i = threadIdx.x; i < q.z_parts; i += blockDim.x) v[2] += __ldcg(q.z_part + i);
     for (int s = threadIdx.x; s < q.S; s += blockDim.x) {
         const int n = __ldcg(q.sum_tokens + s);
         q.tokens[s] = n;
         v[0] += n > 0;
         v[1] += n;
     }
-    for (int i = threadIdx.x; i < q.z_parts; i += blockDim.x) v[2] += __ldcg(q.z_part + i);
+    if (cells) v[3] += rt_balance_cells(q, threadIdx.x, blockDim.x);
     rt_block_sum<4>(v, part);
     if (threadIdx.x == 0) {
         const double b = v[0] > 0.0 ? v[3] * q.E / q.K / v[0] : 0.0, z = v[1] > 0.0 ? v[2] / v[1] : 0.0;
@@ -383,17 +384,11 @@ __device__ __forceinline__ void rt_balance_losses(const RtParams& q, double bala
     }
 }
 
-// Whether this CTA is the last of the grid to come here; what the others wrote before is visible to it then.
-__device__ __forceinline__ bool rt_last_cta(unsigned* ticket) {
-    __shared__ bool last;
+// Thread 0 counts this CTA in, behind a barrier that has brought it what the others wrote: whether it is the last of the grid (then what all CTAs wrote is there).
+__device__ __forceinline__ bool rt_last_cta(unsigned* ticket, bool* last) {
+    if (threadIdx.x == 0) *last = atom_acq_rel_gpu_add(ticket, 1u) == gridDim.x - 1;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();                     // (of what the CTA's threads wrote: the barrier has brought it before this)
-        last = atomicAdd(ticket, 1u) == gridDim.x - 1;
-        __threadfence();
-    }
-    __syncthreads();
-    return last;
+    return *last;
 }
 
 template <typename L>
@@ -409,7 +404,8 @@ template <typename L, int V, int Mode>
 __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(const RtParams q) {
     __shared__ float warp_sum[kRtWarps][V * 32];
     __shared__ int hist[V * 32], warp_tokens[kRtWarps];
-    __shared__ double part[kRtWarps][1];
+    __shared__ double warp_z[kRtWarps];
+    __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lo = static_cast<int>(static_cast<long long>(q.T) * blockIdx.x / gridDim.x), hi = static_cast<int>(static_cast<long long>(q.T) * (blockIdx.x + 1) / gridDim.x);
     for (int e = threadIdx.x; e < V * 32; e += blockDim.x) hist[e] = 0;
@@ -484,24 +480,29 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
         __syncthreads();
     }
     if (!zeroed) grid_dependency_wait();
-    double sum[1] = {lane == 0 ? z : 0.0};
-    rt_block_sum<1>(sum, part);
-    if (threadIdx.x == 0) q.z_part[blockIdx.x] = sum[0];
-    if (static_cast<long long>(q.S) * q.E > kRtEndCells || !rt_last_cta(q.ticket)) return;
-    rt_balance_losses(q, rt_balance_cells(q, threadIdx.x, blockDim.x));
+    if (lane == 0) warp_z[warp] = z;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double sum = 0.0;
+        #pragma unroll
+        for (int w = 0; w < kRtWarps; ++w) sum += warp_z[w];
+        q.z_part[blockIdx.x] = sum;
+    }
+    if (static_cast<long long>(q.S) * q.E <= kRtEndCells && rt_last_cta(q.ticket, &last)) rt_balance_results(q, true, 0.0);
 }
 
 // The same for many sums: by as many CTAs as there are thousands of them; the last one adds up what the others found.
 template <typename L>
 __global__ void __launch_bounds__(kRtWarps * 32) balance_end_kernel(const RtParams q) {
     __shared__ double part[kRtWarps][1];
+    __shared__ bool last;
     double balance[1] = {rt_balance_cells(q, static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x, static_cast<long long>(gridDim.x) * blockDim.x)};
     rt_block_sum<1>(balance, part);
     if (threadIdx.x == 0) q.end_part[blockIdx.x] = balance[0];
-    if (!rt_last_cta(q.ticket)) return;
+    if (!rt_last_cta(q.ticket, &last)) return;
     double all = 0.0;
     for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += blockDim.x) all += __ldcg(q.end_part + i);
-    rt_balance_losses(q, all);
+    rt_balance_results(q, false, all);
 }
 
 // ----------------------------------------------------------------------------- gradient
@@ -510,38 +511,10 @@ __global__ void __launch_bounds__(kRtWarps * 32) balance_end_kernel(const RtPara
 template <typename L, int V, int Mode>
 __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) router_backward_kernel(const RtParams q) {
     __shared__ float rows[kRtWarps][V * 32];
-    __shared__ int part_live[kRtWarps];
-    __shared__ long long part_all[kRtWarps];
     const int lane = threadIdx.x & 31, warp_in = threadIdx.x >> 5;
-    float* buf = rows[warp_in];
-    float live = 1.f, all = 1.f;
-    #pragma unroll
-    for (int j = 0; j < V; ++j) buf[j * 32 + lane] = 0.f;
-    __syncwarp();
-    if (q.balance) {
-        // sequences that have tokens, and their tokens: whole numbers
-        int a = 0;
-        long long b = 0;
-        if (q.S == 1) {
-            b = q.tokens[0];
-            a = b > 0;
-        } else {
-            for (int s = threadIdx.x; s < q.S; s += blockDim.x) { a += q.tokens[s] > 0; b += q.tokens[s]; }
-            #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
-            if (lane == 0) { part_live[warp_in] = a; part_all[warp_in] = b; }
-            __syncthreads();
-            a = 0; b = 0;
-            for (int w = 0; w < kRtWarps; ++w) { a += part_live[w]; b += part_all[w]; }
-        }
-        live = static_cast<float>(a > 0 ? a : 1);
-        all = static_cast<float>(b > 0 ? b : 1);
-    }
-    const float g = q.d_loss_ptr != nullptr ? *q.d_loss_ptr : q.d_loss;
     const int warp = blockIdx.x * kRtWarps + warp_in, warps = gridDim.x * kRtWarps;
     const int lo = static_cast<int>(static_cast<long long>(q.T) * warp / warps), hi = static_cast<int>(static_cast<long long>(q.T) * (warp + 1) / warps);
-    const float zc = 2.f * q.z_coef * g / all;
-    int seq = -1, seq_end = -1;
+    float* buf = rows[warp_in];
     float c[V], ahead[V], dw_ahead = 0.f;
     long long e_ahead = -1;
     auto fetch = [&](int row) {
@@ -552,6 +525,28 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) router_backward_k
         }
     };
     fetch(lo);
+    const float g = q.d_loss_ptr != nullptr ? *q.d_loss_ptr : q.d_loss;
+    float live = 1.f, all = 1.f;
+    #pragma unroll
+    for (int j = 0; j < V; ++j) buf[j * 32 + lane] = 0.f;
+    __syncwarp();
+    if (q.balance) {
+        // sequences that have tokens, and their tokens: whole numbers, by every warp for itself
+        int a = 0;
+        long long b = 0;
+        for (int s = lane; s < q.S; s += 32) {
+            const int n = q.tokens[s];
+            a += n > 0;
+            b += n;
+        }
+        a = __reduce_add_sync(0xffffffffu, a);
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) b += __shfl_xor_sync(0xffffffffu, b, o);
+        live = static_cast<float>(a > 0 ? a : 1);
+        all = static_cast<float>(b > 0 ? b : 1);
+    }
+    const float zc = 2.f * q.z_coef * g / all;
+    int seq = -1, seq_end = -1;
     for (int row = lo; row < hi; ++row) {
         float l[V], d[V];
         #pragma unroll
@@ -640,9 +635,7 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) router_backward_k
 template <typename L, int V, int Mode>
 int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
     const int blocks = (q.T + kRtWarps - 1) / kRtWarps, resident = rt_ctas<V>() * sms;
-    // a token for a warp up to a CTA an SM, then up to four, then as many CTAs as there is room for: what a CTA does once is that of a few tokens
-    int grid = blocks <= sms ? (blocks > 0 ? blocks : 1) : (blocks / 4 > sms ? blocks / 4 : sms);
-    if (grid > resident) grid = resident;
+    const int grid = blocks < 1 ? 1 : (blocks < resident ? blocks : resident);
     if (op == kRtBalance) {
         RtParams b = q;
         b.z_parts = grid < kRtBalanceCtas ? grid : kRtBalanceCtas;
