@@ -638,7 +638,11 @@ int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
     const int grid = blocks < 1 ? 1 : (blocks < resident ? blocks : resident);
     if (op == kRtBalance) {
         RtParams b = q;
-        b.z_parts = grid < kRtBalanceCtas ? grid : kRtBalanceCtas;
+        // one sequence: two CTAs an SM at most, because what each CTA adds to the same sums and counts costs more than its share of the tokens (16384 tokens of 48 experts
+        // 10.0 us, with five an SM 11.8); several sequences: all that fit, because a CTA takes its pieces of sequences one after the other (12000 tokens of 128
+        // experts in 37 sequences 16.2 us, with two an SM 18.0)
+        const int most = q.cu == nullptr && 2 * sms < kRtBalanceCtas ? 2 * sms : kRtBalanceCtas;
+        b.z_parts = grid < most ? grid : most;
         const long long zero = (b.zero_words + 1023) / 1024;
         balance_zero_kernel<L><<<static_cast<int>(zero < sms ? zero : sms), 256, 0, stream>>>(b);
         MM_CUDA(cudaGetLastError());
