@@ -47,7 +47,7 @@ bool writes_safely(const Rows& out, const Rows* others, int n, bool in_place) {
 }
 
 int norm_check(const mm_block_norm_args_t* a) {
-    if (a == nullptr || a->tokens < 0 || a->tokens > 0x7fffffffll || a->hidden < 1) return MM_ERR_INVALID_ARGUMENT;
+    if (a == nullptr || a->tokens < 0 || a->tokens > (1ll << 30) || a->hidden < 1) return MM_ERR_INVALID_ARGUMENT;
     if (!known_dtype(a->dtype) || !known_dtype(a->stream_dtype) || !known_dtype(a->weight_dtype) || !known_dtype(a->gate_dtype)) return MM_ERR_INVALID_ARGUMENT;
     if (a->hidden > mm::kBnMaxHidden) return MM_ERR_UNSUPPORTED;
     if (a->stream_dtype != a->dtype && a->stream_dtype != MM_DTYPE_FP32) return MM_ERR_UNSUPPORTED;
@@ -123,8 +123,11 @@ void balance_params(const mm_balance_args_t* b, mm::RtParams& q) {
     q.counts = b->counts; q.tokens = b->seq_tokens; q.mean = b->mean_probs; q.losses = b->losses;
 }
 
+constexpr int kMaxSequences = 1 << 21;       // times 1024 experts: sums are numbered in 32 bits
+
 int balance_check(const mm_balance_args_t* b) {
     if (b == nullptr || b->num_sequences < 1 || (b->cu_seqlens == nullptr && b->num_sequences != 1)) return MM_ERR_INVALID_ARGUMENT;
+    if (b->num_sequences > kMaxSequences) return MM_ERR_UNSUPPORTED;
     if (b->counts == nullptr || b->seq_tokens == nullptr) return MM_ERR_INVALID_ARGUMENT;
     if (!std::isfinite(b->balance_coef) || !std::isfinite(b->z_coef)) return MM_ERR_INVALID_ARGUMENT;
     return MM_OK;
@@ -159,11 +162,11 @@ int mm_block_norm(const mm_block_norm_args_t* a, void* stream_ptr) {
                             : rows_of(a->gate, a->gate_mode == MM_GATE_TOKEN ? a->gate_stride : 0, a->gate_mode == MM_GATE_TOKEN ? t : 1,
                                       a->gate_mode == MM_GATE_TOKEN ? 1 : a->hidden, a->gate_dtype),
                     rows_of(a->pre_weight, 0, 1, a->hidden, a->weight_dtype), rows_of(a->post_weight, 0, 1, a->hidden, a->weight_dtype)};
+    if (t == 1) for (Rows& r : rows) r.ld = 0;                              // (how far the next row would be says nothing)
     for (int i = 0; i < 2; ++i)
         if (t > 1 && rows[i].p != nullptr && rows[i].ld < rows[i].width) return MM_ERR_INVALID_ARGUMENT;
     if (!writes_safely(rows[0], rows + 1, 1, false) || !writes_safely(rows[0], rows + 2, 2, true) || !writes_safely(rows[0], rows + 4, 3, false) ||
         !writes_safely(rows[1], rows + 2, 2, true) || !writes_safely(rows[1], rows + 4, 3, false)) return MM_ERR_INVALID_ARGUMENT;
-    if (t == 1) for (Rows& r : rows) r.ld = 0;
     if (a->gate_mode == MM_GATE_TOKEN) rows[4].p = nullptr;                 // (read one by one)
     mm::BnLaunch how = {false, a->stream_dtype == MM_DTYPE_FP32, norm_rows_aligned(a->hidden, rows, 7), 0, 0};
     st = sm_count(&how.sms);
@@ -199,12 +202,12 @@ int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_gr
                          rows_of(a->residual, a->residual_stride, t, a->hidden, a->stream_dtype), rows_of(a->y, a->y_stride, t, a->hidden, a->dtype),
                          element ? rows_of(a->gate, a->gate_stride, t, a->hidden, a->gate_dtype) : (token ? rows_of(a->gate, a->gate_stride, t, 1, a->gate_dtype) : rows_of(a->gate, 0, 1, a->hidden, a->gate_dtype)),
                          rows_of(a->pre_weight, 0, 1, a->hidden, a->weight_dtype), rows_of(a->post_weight, 0, 1, a->hidden, a->weight_dtype)};
+        if (t == 1) for (Rows& r : rows) r.ld = 0;
         for (int i = 0; i < 3; ++i) {
             if (t > 1 && rows[i].p != nullptr && rows[i].ld < rows[i].width) return MM_ERR_INVALID_ARGUMENT;
             for (int k = 0; k < 10; ++k)         // gradients are written apart from everything else
                 if (k != i && share_memory(rows[i], rows[k])) return MM_ERR_INVALID_ARGUMENT;
         }
-        if (t == 1) for (Rows& r : rows) r.ld = 0;
         if (token) rows[2].p = rows[7].p = nullptr;
         mm::BnParams q = norm_params(a);
         q.d_residual_out = g->d_residual_out; q.d_residual_out_ld = g->d_residual_out_stride;
@@ -244,7 +247,7 @@ int mm_route_tokens(const mm_router_args_t* a, const float* expert_bias, const u
 }
 
 int64_t mm_balance_workspace_bytes(int32_t num_experts, int32_t num_sequences) {
-    if (num_experts < 1 || num_experts > mm::kRtMaxExperts || num_sequences < 1) return -1;
+    if (num_experts < 1 || num_experts > mm::kRtMaxExperts || num_sequences < 1 || num_sequences > kMaxSequences) return -1;
     return balance_zeroed_bytes(num_experts, num_sequences) + static_cast<int64_t>(mm::kRtBalanceCtas) * 16;
 }
 
@@ -276,8 +279,9 @@ int mm_router_backward(const mm_router_args_t* a, const float* d_topk_weights, c
     if (a->tokens == 0) return MM_OK;
     if (d_logits == nullptr || (a->tokens > 1 && d_logits_stride < a->num_experts)) return MM_ERR_INVALID_ARGUMENT;
     const int bytes = dtype_bytes(a->dtype);
-    const Rows logits = {a->logits, a->logits_stride * bytes, static_cast<int64_t>(a->num_experts) * bytes, a->tokens};
-    const Rows grads = {d_logits, d_logits_stride * bytes, static_cast<int64_t>(a->num_experts) * bytes, a->tokens};
+    const int64_t apart = a->tokens > 1 ? 1 : 0;                            // (how far a second token would be)
+    const Rows logits = {a->logits, apart * a->logits_stride * bytes, static_cast<int64_t>(a->num_experts) * bytes, a->tokens};
+    const Rows grads = {d_logits, apart * d_logits_stride * bytes, static_cast<int64_t>(a->num_experts) * bytes, a->tokens};
     if (!writes_safely(grads, &logits, 1, true)) return MM_ERR_INVALID_ARGUMENT;
     mm::RtParams q = router_params(a);
     if (b != nullptr) balance_params(b, q);

@@ -40,6 +40,10 @@ int dtype_of(ScalarType t) { return t == at::kBFloat16 ? MM_DTYPE_BF16 : (t == a
 void* address(const Tensor* t) { return t != nullptr ? t->data_ptr() : nullptr; }
 
 Tensor empty(at::IntArrayRef shape, ScalarType type, const Tensor& like) { return at::detail::empty_cuda(shape, type, like.device(), std::nullopt); }
+// a tensor of the caller's that has been written: autograd is to know (inference tensors keep no count)
+void written(const Tensor* t) {
+    if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
 PyObject* wrap_or_none(const Tensor& t) {
     if (t.defined()) return THPVariable_Wrap(t);
@@ -87,6 +91,7 @@ Block block_inputs(PyObject* const* arg, ScalarType type, const Tensor& residual
                 "residual must be a CUDA [tokens, hidden] tensor; types are bf16, fp16 and fp32");
     TORCH_CHECK(stream == type || stream == at::kFloat, "the residual stream must be of the type of the activations or fp32");
     const int64_t tokens = residual.size(0), hidden = residual.size(1);
+    TORCH_CHECK(tokens <= (1ll << 30), "at most 2^30 tokens");
     TORCH_CHECK(hidden >= 1 && hidden <= 8192, "hidden must be 1 to 8192");
     TORCH_CHECK(y != nullptr || (b.gate == nullptr && b.post == nullptr && b.pre != nullptr),
                 "without y there is only the norm of the stream: pre_weight, and neither post_weight nor gate");
@@ -157,6 +162,8 @@ PyObject* block_norm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
         const c10::cuda::CUDAGuard guard(residual.device());
         check(mm_block_norm(&b.a, stream_of(residual)), "block_norm");
     }
+    if (!own_out.defined()) written(y != nullptr ? out : nullptr);
+    if (!own_normed.defined()) written(normed);
     PyObject* first = own_out.defined() ? wrap(own_out) : Py_NewRef(y != nullptr ? arg[8] : arg[0]);
     return tuple_of({first, own_normed.defined() ? wrap(own_normed) : Py_NewRef(arg[9])});
     END_HANDLE_TH_ERRORS
@@ -236,7 +243,7 @@ int64_t topk_of(const Tensor& idx) {
 int32_t* sequences(const Tensor* cu, const Tensor& logits, int64_t* n) {
     *n = 1;
     if (cu == nullptr) return nullptr;
-    TORCH_CHECK(cu->dim() == 1 && cu->size(0) >= 2 && cu->size(0) <= 0x7fffffff, "cu_seqlens must be int32 [sequences + 1]");
+    TORCH_CHECK(cu->dim() == 1 && cu->size(0) >= 2 && cu->size(0) <= (1 << 21) + 1, "cu_seqlens must be int32 [sequences + 1] of at most 2^21 sequences");
     *n = cu->size(0) - 1;
     return static_cast<int32_t*>(plain(*cu, "cu_seqlens", cu->sizes(), at::kInt, logits));
 }
@@ -267,6 +274,8 @@ PyObject* route_tokens(PyObject*, PyObject* const* arg, Py_ssize_t n) {
         const c10::cuda::CUDAGuard guard(logits.device());
         check(mm_route_tokens(&a, bias_ptr, valid_ptr, stream_of(logits)), "route_tokens");
     }
+    if (!own_idx.defined()) written(idx);
+    if (!own_weights.defined()) written(weights);
     return tuple_of({own_idx.defined() ? wrap(own_idx) : Py_NewRef(arg[6]), own_weights.defined() ? wrap(own_weights) : Py_NewRef(arg[7])});
     END_HANDLE_TH_ERRORS
 }
@@ -341,7 +350,9 @@ PyObject* router_backward(PyObject*, PyObject* const* arg, Py_ssize_t n) {
         const c10::cuda::CUDAGuard guard(logits.device());
         check(mm_router_backward(&a, dw_ptr, counts != nullptr ? &b : nullptr, d_loss, d_loss_ptr, d->data_ptr(), d->stride(0), stream_of(logits)), "router_backward");
     }
-    return own.defined() ? wrap(own) : Py_NewRef(arg[11]);
+    if (own.defined()) return wrap(own);
+    written(d);
+    return Py_NewRef(arg[11]);
     END_HANDLE_TH_ERRORS
 }
 

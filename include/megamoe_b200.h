@@ -263,7 +263,7 @@ typedef struct mm_block_norm_args {
     const void* post_weight;         /* weight_dtype [hidden], or NULL: y as it is */
     void* residual_out;              /* stream_dtype [tokens][hidden]; NULL if y is; may be `residual` itself */
     void* normed;                    /* dtype [tokens][hidden]; NULL if pre_weight is; may be `y` or `residual` itself */
-    int64_t tokens;
+    int64_t tokens;                  /* at most 2^30 */
     int64_t residual_stride, y_stride, gate_stride, residual_out_stride, normed_stride;
     int32_t hidden;
     int32_t dtype;                   /* enum mm_dtype, of y and normed */
@@ -306,7 +306,7 @@ typedef struct mm_router_args {
 
 typedef struct mm_balance_args {
     const int32_t* cu_seqlens;       /* [num_sequences + 1] ascending, sequence s is tokens cu[s] .. cu[s+1]-1; NULL: one sequence of all tokens */
-    int32_t num_sequences;
+    int32_t num_sequences;           /* at most 2^21 */
     float balance_coef, z_coef;
     int32_t* counts;                 /* [num_sequences][num_experts] routing slots per expert */
     int32_t* seq_tokens;             /* [num_sequences] tokens with a route */

@@ -75,7 +75,7 @@ def test_ctypes_mirror_matches_the_header():
 
 
 @pytest.mark.parametrize('change, status', [
-    (dict(tokens=-1), INVALID), (dict(hidden=0), INVALID), (dict(hidden=8193), UNSUPPORTED), (dict(dtype=3), INVALID), (dict(stream_dtype=-1), INVALID),
+    (dict(tokens=-1), INVALID), (dict(tokens=(1 << 30) + 1), INVALID), (dict(hidden=0), INVALID), (dict(hidden=8193), UNSUPPORTED), (dict(dtype=3), INVALID), (dict(stream_dtype=-1), INVALID),
     (dict(stream_dtype=1), UNSUPPORTED), (dict(weight_dtype=1), UNSUPPORTED), (dict(gate_dtype=1), UNSUPPORTED), (dict(gate_mode=4), INVALID),
     (dict(gate_mode=1), INVALID), (dict(gate=14 * A), INVALID), (dict(y=0, residual_out=0), INVALID), (dict(y=0, residual_out=0, post_weight=0, pre_weight=0, normed=0), INVALID),
     (dict(eps=0.0), INVALID), (dict(eps=float('nan')), INVALID), (dict(scale=float('inf')), INVALID), (dict(weight_offset=float('nan')), INVALID),
@@ -91,7 +91,7 @@ def test_norm_refusals(change, status):
 
 
 @pytest.mark.parametrize('change', [
-    dict(), dict(tokens=1, residual_out_stride=0), dict(residual_out=A), dict(normed=2 * A), dict(normed=A), dict(residual_out=A, normed=2 * A),
+    dict(), dict(tokens=1, residual_out_stride=0), dict(tokens=1, residual_out=A, residual_out_stride=7, normed=2 * A, normed_stride=1), dict(residual_out=A), dict(normed=2 * A), dict(normed=A), dict(residual_out=A, normed=2 * A),
     dict(residual=A, residual_out=A + 128, residual_stride=128, residual_out_stride=128),              # two halves of one buffer's rows
     dict(y=0, post_weight=0, residual_out=0), dict(pre_weight=0, normed=0),
 ])
@@ -150,6 +150,7 @@ def test_router_refusals_of_its_other_arguments():
     assert lib.mm_balance_loss(ctypes.byref(a), ctypes.byref(b), 9 * A, need - 1, None) == INVALID
     assert lib.mm_balance_loss(ctypes.byref(a), ctypes.byref(b), 9 * A + 4, need, None) == INVALID
     assert lib.mm_balance_loss(ctypes.byref(a), ctypes.byref(b), None, need, None) == INVALID
+    assert lib.mm_balance_workspace_bytes(48, (1 << 21) + 1) == -1 and lib.mm_balance_loss(ctypes.byref(a), ctypes.byref(_balance(num_sequences=(1 << 21) + 1)), 9 * A, 1 << 40, None) == UNSUPPORTED
     assert lib.mm_balance_workspace_bytes(0, 1) == -1 and lib.mm_balance_workspace_bytes(48, 0) == -1 and lib.mm_balance_workspace_bytes(1025, 1) == -1
     assert lib.mm_router_backward(ctypes.byref(a), None, None, 1.0, None, 10 * A, 48, None) == INVALID     # nothing to take the gradient of
     assert lib.mm_router_backward(ctypes.byref(a), 9 * A, None, 1.0, None, None, 48, None) == INVALID

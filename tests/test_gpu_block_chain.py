@@ -103,6 +103,7 @@ def test_training_step_of_a_block():
     logits64 = normed64 @ b[5].t()
     loss64 = B.balance_reference(logits64, idx, 0, None, 0.5, 0.1)[0][0]
     ((stream64 * d_stream.double()).sum() + (B.route_weights(logits64, idx, 0, 1.0) * d_w.double()).sum() + loss64).backward()
+    loss, loss64 = loss.detach(), loss64.detach()
     assert abs(float(loss) - float(loss64)) <= 512 * B.U * float(loss64)
     for x, y in zip(a, b):
         assert float((x.grad.double() - y.grad).norm()) <= 512 * B.U * float(y.grad.norm())

@@ -178,6 +178,19 @@ def test_in_place(tokens, hidden):
     assert torch.equal(got[0], want[0]) and torch.equal(r, want[1])
 
 
+def test_writes_are_known_to_autograd():
+    """A tensor that something has saved for its backward pass and that is then written in place is refused there, as torch's own operators have it."""
+    x, _, _ = _inputs(8, 64, dtype=FP32)
+    w = torch.ones(8, 64, device='cuda', requires_grad=True)
+    product = w * x['residual']                                             # saves the stream
+    mm.block_norm(x['residual'], x['y'], pre_weight=x['pre_weight'], residual_out=x['residual'])
+    with pytest.raises(RuntimeError):
+        product.sum().backward()
+    with torch.inference_mode():
+        r = x['y'].clone()
+        mm.block_norm(r, x['y'], pre_weight=x['pre_weight'], residual_out=r)
+
+
 def test_captured_and_replayed():
     """A graph of both directions, replayed with new inputs, beside another graph of the same calls."""
     x, d_stream, d_normed = _inputs(300, 1024, gate='channel')

@@ -112,6 +112,36 @@ def test_route_of_equal_keys(mode, experts):
         _check_route(logits[:8], 8, mode, bias, None, 1.0, mm.route_tokens(logits[:8], 8, mode, bias))
 
 
+def test_biases_of_any_size():
+    """Biases that dwarf the scores (their keys' 32-bit errors are of another size than the border's), infinite ones, and -inf or NaN, which switch an expert off."""
+    inf = float('inf')
+    logits = _logits(300, 96)
+    bias = _bias(96)
+    for scale in (1e6, 1e30):
+        big = bias.clone()
+        big[::5] *= scale
+        big[1::7] -= 3.0
+        _check_route(logits, 8, 1, big, None, 1.0, mm.route_tokens(logits, 8, 1, big))
+    bias[3:6] = inf
+    _check_route(logits, 8, 1, bias, None, 1.0, mm.route_tokens(logits, 8, 1, bias))
+    bias[10:90] = -inf
+    bias[90:93] = float('nan')
+    idx, w = mm.route_tokens(logits, 16, 1, bias)
+    on = torch.cat([torch.arange(10), torch.arange(93, 96)]).cuda()
+    want, _ = B.route_reference(logits[:, on].contiguous(), 13, 1, bias[on].contiguous(), None, 1.0)
+    assert torch.equal(idx[:, :13], on[want]) and bool((idx[:, 13:] == -1).all()) and not w[:, 13:].any()
+
+
+@pytest.mark.parametrize('mode', [0, 1])
+def test_many_equal_keys(mode):
+    """More candidates than a warp has lanes, and more routes than lanes with an expert on top."""
+    logits = (_logits(64, 1024, seed=6) * 2).round()
+    for topk in (1, 8, 32):
+        _check_route(logits, topk, mode, None, None, 1.0, mm.route_tokens(logits, topk, mode))
+    short = _logits(40, 40, seed=7)
+    _check_route(short, 32, mode, None, None, 1.0, mm.route_tokens(short, 32, mode))
+
+
 @pytest.mark.parametrize('mode', [0, 1])
 def test_experts_that_are_off(mode):
     """-inf and NaN switch an expert off; rows with fewer experts left than routes, and with none; +inf; the type's lowest value is a value."""
@@ -263,6 +293,29 @@ def test_logits_far_apart():
     b = mm.balance_loss(far, out[0])
     _check_balance(logits, out[0], 0, None, 1.0, 0.0, b)
     assert torch.equal(mm.router_backward(far, out[0], balance=b, d_logits=far), mm.router_backward(logits, out[0], balance=b))
+
+
+def test_infinities_and_the_ends_of_the_range():
+    """Rows with NaN, infinities and the largest numbers beside ordinary ones: losses and gradients of the ordinary rows are what they are without them."""
+    inf, top = float('inf'), torch.finfo(FP32).max
+    for mode in (0, 1):
+        plain = _logits(12, 48)
+        idx = mm.route_tokens(plain, 8, mode)[0]
+        odd = plain.clone()
+        odd[0, 3], odd[1, 4], odd[2, 5], odd[3], odd[4] = float('nan'), -inf, inf, top, -top
+        odd[5] = -inf
+        b = mm.balance_loss(odd, idx, mode)
+        assert b.counts.sum() == 96 and b.losses[1].isfinite() and b.mean_probs.isfinite().all()
+        p = torch.full((12, 48), 0.0, dtype=torch.float64, device='cuda')
+        for r in range(12):
+            l = B.clean_logits(odd[r:r + 1])[0]
+            if bool((l > -inf).any()):
+                s = torch.exp(l - l.max()) if mode == 0 else torch.where(l > -inf, torch.sigmoid(l), 0.0)
+                p[r] = s / s.sum().clamp(min=1e-300)
+        B.assert_near(b.mean_probs, p.mean(dim=0, keepdim=True), p.mean(dim=0, keepdim=True) + 2.0 ** -12, CHAIN + ROWS, 'mean_probs')
+        whole = mm.balance_loss(plain, idx, mode)
+        d, want = mm.router_backward(odd, idx, mode, balance=b), mm.router_backward(plain, idx, mode, balance=whole)
+        assert torch.equal(d[6:], want[6:]) and not d[5].any()                # (the counts are the same)
 
 
 def test_sums_over_ranks():
