@@ -82,8 +82,9 @@ __device__ __forceinline__ float bn_token_gate(const BnParams& q, long long row)
 // halves both the values of a lane and the lanes of a value. Each warp's sums go through shared memory (`part`, all zero at first, of which a turn
 // is used at a time: the next sums' values go where no thread can still be reading, so one barrier does), and four lanes add up one value.
 constexpr int kBnSumWarps = kBnMaxThreads / 32;
-template <int N>
-__device__ __forceinline__ void bn_sum(float (&v)[N], float (*part)[8][kBnSumWarps], int& turn) {
+template <int N, int Room>
+__device__ __forceinline__ void bn_sum(float (&v)[N], float (*part)[Room][kBnSumWarps], int& turn) {
+    static_assert(N <= Room && N <= 16);
     const uint32_t lane = threadIdx.x & 31u;
     float s[N];
     #pragma unroll
@@ -106,12 +107,15 @@ __device__ __forceinline__ void bn_sum(float (&v)[N], float (*part)[8][kBnSumWar
         turn ^= 1;
         if (lane % (32 / N) == 0) p[mine][threadIdx.x >> 5] = s[0];
         __syncthreads();
-        const float4 w = *reinterpret_cast<const float4*>(&p[(lane >> 2) % N][(lane & 3u) * 4u]);
-        float t = (w.x + w.y) + (w.z + w.w);
-        t += __shfl_xor_sync(0xffffffffu, t, 1);
-        t += __shfl_xor_sync(0xffffffffu, t, 2);
         #pragma unroll
-        for (int n = 0; n < N; ++n) v[n] = __shfl_sync(0xffffffffu, t, n * 4);
+        for (int first = 0; first < N; first += 8) {         // eight values at a time
+            const float4 w = *reinterpret_cast<const float4*>(&p[first + (lane >> 2) % (N < 8 ? N : 8)][(lane & 3u) * 4u]);
+            float t = (w.x + w.y) + (w.z + w.w);
+            t += __shfl_xor_sync(0xffffffffu, t, 1);
+            t += __shfl_xor_sync(0xffffffffu, t, 2);
+            #pragma unroll
+            for (int n = 0; n < 8 && first + n < N; ++n) v[first + n] = __shfl_sync(0xffffffffu, t, n * 4);
+        }
     } else {
         #pragma unroll
         for (int n = 0; n < N; ++n) v[n] = __shfl_sync(0xffffffffu, s[0], n * (32 / N));
@@ -119,9 +123,10 @@ __device__ __forceinline__ void bn_sum(float (&v)[N], float (*part)[8][kBnSumWar
 }
 static_assert(kBnSumWarps == 16, "four lanes read four warps' sums each");
 
-__device__ __forceinline__ void bn_sum_init(float (*part)[8][kBnSumWarps]) {
+template <int Room>
+__device__ __forceinline__ void bn_sum_init(float (*part)[Room][kBnSumWarps]) {
     if (blockDim.x > 32) {
-        for (int i = threadIdx.x; i < 2 * 8 * kBnSumWarps; i += blockDim.x) (&part[0][0][0])[i] = 0.f;
+        for (int i = threadIdx.x; i < 2 * Room * kBnSumWarps; i += blockDim.x) (&part[0][0][0])[i] = 0.f;
         __syncthreads();
     }
 }
@@ -142,7 +147,7 @@ __device__ __forceinline__ void bn_gate(const BnParams& q, long long row, int c,
 
 template <typename X, typename R>
 __global__ void __launch_bounds__(kBnMaxThreads) block_norm_wide_kernel(const BnParams q) {
-    __shared__ __align__(16) float part[2][8][kBnSumWarps];
+    __shared__ __align__(16) float part[2][2][kBnSumWarps];
     constexpr int C = 2;
     bn_sum_init(part);
     int turn = 0;
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_wide_kernel(const Bn
 // `partial`, which `block_norm_sums_kernel` adds up: always in the same order.
 template <typename X, typename R>
 __global__ void __launch_bounds__(kBnMaxThreads) block_norm_backward_wide_kernel(const BnParams q) {
-    __shared__ __align__(16) float part[2][8][kBnSumWarps];
+    __shared__ __align__(16) float part[2][2][kBnSumWarps];
     constexpr int C = 2;
     bn_sum_init(part);
     int turn = 0;
@@ -462,17 +467,25 @@ __device__ __forceinline__ void bn_pre_factor(const BnParams& q, float2 (&w)[4])
     for (int i = 0; i < 4; ++i) w[i] = make_float2(w[i].x + q.offset, w[i].y + q.offset);
 }
 
-// A token's gate is asked for a row ahead as it lies in memory, and turned into a number when its row comes: a conversion at the load would wait for it.
+// A token's gate is asked for a row ahead as it lies in memory, and turned into a number when its row comes: a conversion at the load would wait for it. No
+// branches: they would part the work of two rows.
 template <typename X>
 __device__ __forceinline__ uint32_t bn_gate_bits(const BnParams& q, long long row) {
-    if (sizeof(X) == 4 || q.gate32) return static_cast<const uint32_t*>(q.gate)[row * q.gate_ld];
-    return static_cast<const uint16_t*>(q.gate)[row * q.gate_ld];
+    uint32_t bits;
+    const long long at = row * q.gate_ld;
+    if constexpr (sizeof(X) == 4)
+        asm volatile("ld.global.b32 %0, [%1];" : "=r"(bits) : "l"(static_cast<const uint32_t*>(q.gate) + at) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\t@p ld.global.b32 %0, [%1];\n\t@!p ld.global.u16 %0, [%1];\n\t}"
+                     : "=r"(bits) : "l"(static_cast<const char*>(q.gate) + (at << (q.gate32 ? 2 : 1))), "r"(q.gate32) : "memory");
+    return bits;
 }
 template <typename X>
 __device__ __forceinline__ float bn_gate_value(const BnParams& q, uint32_t bits) {
-    if (sizeof(X) == 4 || q.gate32) return __uint_as_float(bits);
+    if constexpr (sizeof(X) == 4) return __uint_as_float(bits);
     const uint16_t half = static_cast<uint16_t>(bits);
-    return bn_float<X>(*reinterpret_cast<const X*>(&half));
+    const float narrow = bn_float<X>(*reinterpret_cast<const X*>(&half));
+    return q.gate32 ? __uint_as_float(bits) : narrow;
 }
 // an element's gate: of the activations' type or 32 bits, held in room for the latter
 template <typename X, bool Vec>
@@ -522,7 +535,7 @@ enum BnKind { kBnPlain = 0 /* no gate, or one that is part of y's factor */, kBn
 // (One CTA of twice the registers per SM 168 us; sixteen channels a thread 134; rows copied ahead into shared memory by cp.async 160.)
 template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec>
 __global__ void __maxnreg__((sizeof(R) == 2 && Vec ? 56 : 64)) block_norm_kernel(const BnParams q) {
-    __shared__ __align__(16) float part[2][8][kBnSumWarps];
+    __shared__ __align__(16) float part[2][2][kBnSumWarps];
     const float inv_h = 1.f / static_cast<float>(q.hidden);
     const int step = gridDim.x, tokens = static_cast<int>(q.tokens);
     const bool on = !Vec || static_cast<int>(threadIdx.x) * 8 < q.hidden;
@@ -602,160 +615,208 @@ __global__ void __maxnreg__((sizeof(R) == 2 && Vec ? 56 : 64)) block_norm_kernel
 }
 
 // Rows are dealt to the CTAs in turn; a thread sums what the gradients of its channels' weights are made of over the CTA's rows and leaves it in `partial`, which
-// `block_norm_sums_kernel` adds up: always in the same order. Registers bound how much of a row's traffic is in flight: 128 a thread, a row being worked on and a row on its
-// way, y two rows ahead (its sum of squares goes with the exchange of the row before). 8192 x 4096, 32-bit stream, both norms: 97 us (6.2 TB/s), 8192 x 3072
-// in bf16 66 us (4.6). (y one row ahead 131 and 101 us; weights or the sums in shared memory, or more threads with fewer registers, no better.)
-template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec>
-__global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_backward_kernel(const BnParams q) {
-    __shared__ __align__(16) float part[2][8][kBnSumWarps];
+// `block_norm_sums_kernel` adds up: always in the same order. Some 400 instructions a warp and row, so the issue slots are half full; what is left is the wait for a row's
+// exchange, and registers bound what can go on meanwhile: 128 a thread, a row being worked on and a row on its way, y two rows ahead (its sum of squares goes
+// with the exchange of the row before). 8192 x 4096, 32-bit stream, both norms: 97 us (6.2 TB/s); y one row ahead 131.
+// Where a CTA of 128 registers a thread leaves an SM's registers half used and no second one fits (more than 256 threads, up to 384: hidden 2056 to 3072), it takes two rows
+// at a time through one exchange, with 168: 8192 x 3072 in bf16 59 us instead of 67, only the stream's norm 53 instead of 64, 32-bit stream 74 instead of 81. (With 256 threads
+// two CTAs of one row win, 42 us against 46 for 8192 x 2048; with an element's gate, or 32-bit
+// activations, two rows do not fit the registers.)
+template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec, int Rows>
+__global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1) block_norm_backward_kernel(const BnParams q) {
     constexpr bool kY = Kind != kBnStream, kSumV = Post || Kind == kBnToken;
+    constexpr int kSums = (kSumV ? 8 : 2) * Rows;
+    __shared__ __align__(16) float part[2][kSums][kBnSumWarps];
     const float inv_h = 1.f / static_cast<float>(q.hidden);
-    const int step = gridDim.x, tokens = static_cast<int>(q.tokens);
+    const int step = gridDim.x * Rows, tokens = static_cast<int>(q.tokens);
     const bool on = !Vec || static_cast<int>(threadIdx.x) * 8 < q.hidden, sum_y = Post || q.gate_mode == kBnGateChannel, has_d = q.d_residual_out != nullptr;
-    BnAhead<R, Vec> rd, rr;                                  // on their way
-    BnAhead<X, Vec> ry_ahead, rh;
-    Bn8<X> ry;                                               // norm of y: the next row's
-    uint32_t rg[8];
+    BnAhead<R, Vec> rd[Rows], rr[Rows];                      // on their way
+    BnAhead<X, Vec> ry_ahead[Rows], rh[Rows];
+    Bn8<X> ry[Rows];                                         // norm of y: the next rows'
+    uint32_t rg[Rows][8], gate_bits[Rows];
     float2 a[4], w[4], acc_pre[4], acc_y[4];
-    uint32_t gate_bits = 0u;
-    bn_clear(rd.w);
-    bn_clear(rr.w);
-    bn_clear(ry.w);
-    bn_clear(rh.w);
-    bn_clear(ry_ahead.w);
-    bn_clear(rg);
+    #pragma unroll
+    for (int n = 0; n < Rows; ++n) {
+        bn_clear(rd[n].w);
+        bn_clear(rr[n].w);
+        bn_clear(ry[n].w);
+        bn_clear(rh[n].w);
+        bn_clear(ry_ahead[n].w);
+        bn_clear(rg[n]);
+        gate_bits[n] = 0u;
+    }
     #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = w[i] = acc_pre[i] = acc_y[i] = both(0.f);
-    auto fetch_y = [&](long long row) {
-        if (kY && on) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry_ahead);
-    };
-    auto fetch = [&](long long row) {
-        if (on) {
-            if (!Post) fetch_y(row);
-            else if (row + step < tokens) fetch_y(row + step);
-            if (Pre) {
-                bn_fetch<R, Vec>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, rr);
-                bn_fetch<X, Vec>(static_cast<const X*>(q.d_normed) + row * q.d_normed_ld, q.hidden, rh);
-            }
-            if (has_d) bn_fetch<R, Vec>(static_cast<const R*>(q.d_residual_out) + row * q.d_residual_out_ld, q.hidden, rd);
-            if (Kind == kBnElement) bn_fetch_gate<X, Vec>(q, row, rg);
+    auto fetch_y = [&](int first) {
+        #pragma unroll
+        for (int n = 0; n < Rows; ++n) {
+            const long long row = first + n;
+            if (kY && on && row < tokens) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry_ahead[n]);
+            else bn_clear(ry_ahead[n].w);
         }
-        if (Kind == kBnToken) gate_bits = bn_gate_bits<X>(q, row);
     };
-    int row = blockIdx.x;
-    if (Post) { fetch_y(row); ry = bn_take(ry_ahead); }
-    fetch(row);
+    auto fetch = [&](int first) {
+        fetch_y(Post ? first + step : first);
+        #pragma unroll
+        for (int n = 0; n < Rows; ++n) {
+            const long long row = first + n;
+            if (n > 0 && row >= tokens) {                    // (a pair without its second row works on zeros)
+                bn_clear(rr[n].w);
+                bn_clear(rh[n].w);
+                bn_clear(rd[n].w);
+                continue;
+            }
+            if (on) {
+                if (Pre) {
+                    bn_fetch<R, Vec>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, rr[n]);
+                    bn_fetch<X, Vec>(static_cast<const X*>(q.d_normed) + row * q.d_normed_ld, q.hidden, rh[n]);
+                }
+                if (has_d) bn_fetch<R, Vec>(static_cast<const R*>(q.d_residual_out) + row * q.d_residual_out_ld, q.hidden, rd[n]);
+                if (Kind == kBnElement) bn_fetch_gate<X, Vec>(q, row, rg[n]);
+            }
+            if (Kind == kBnToken) gate_bits[n] = bn_gate_bits<X>(q, row);
+        }
+    };
+    int first = blockIdx.x * Rows;
+    if (Post) {
+        fetch_y(first);
+        #pragma unroll
+        for (int n = 0; n < Rows; ++n) ry[n] = bn_take(ry_ahead[n]);
+    }
+    fetch(first);
     grid_launch_dependents();                                // (the sums' kernel waits for this one's end by itself)
     if (on) {
         if (kY) bn_y_factor<X, Vec>(q, a);
         if (Pre) bn_pre_factor<X, Vec>(q, w);
     }
-    bn_sum_init(part);
+    bn_sum_init<kSums>(part);
     int turn = 0;
-    float i1 = 1.f;
+    float i1[Rows];
+    #pragma unroll
+    for (int n = 0; n < Rows; ++n) i1[n] = 1.f;
     if (Post) {
-        float sum[1] = {bn_square(ry)};
-        bn_sum<1>(sum, part, turn);
-        i1 = rsqrtf(sum[0] * inv_h + q.eps);
+        float sum[Rows];
+        #pragma unroll
+        for (int n = 0; n < Rows; ++n) sum[n] = bn_square(ry[n]);
+        bn_sum<Rows, kSums>(sum, part, turn);
+        #pragma unroll
+        for (int n = 0; n < Rows; ++n) i1[n] = rsqrtf(sum[n] * inv_h + q.eps);
     }
     while (true) {
-        const bool more = row + step < tokens;
-        const Bn8<R> cd = bn_take(rd);
-        const Bn8<X> cy = Post ? ry : bn_take(ry_ahead), ch = bn_take(rh);
-        uint32_t cg[8];
+        const bool more = first + step < tokens;
+        Bn8<R> cd[Rows];
+        Bn8<X> cy[Rows], ch[Rows];
+        uint32_t cg[Rows][8];
+        float2 r[Rows][4];
+        float gate[Rows];
         #pragma unroll
-        for (int i = 0; i < 8; ++i) cg[i] = rg[i];
-        float2 r[4];
-        if (Pre) bn_unpack(bn_take(rr), r);
-        if (Post) ry = bn_take(ry_ahead);
-        const float gate = Kind == kBnToken ? bn_gate_value<X>(q, gate_bits) : 1.f;
-        if (more) fetch(row + step);
-        float sum[8] = {};                                   // r' r', dh w2 r', v d, v dh w2, v r' (v without a token's gate), next y's squares
-        {
+        for (int n = 0; n < Rows; ++n) {
+            cd[n] = bn_take(rd[n]);
+            cy[n] = Post ? ry[n] : bn_take(ry_ahead[n]);
+            ch[n] = bn_take(rh[n]);
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) cg[n][i] = rg[n][i];
+            if (Pre) bn_unpack(bn_take(rr[n]), r[n]);
+            if (Post) ry[n] = bn_take(ry_ahead[n]);
+            gate[n] = Kind == kBnToken ? bn_gate_value<X>(q, gate_bits[n]) : 1.f;
+        }
+        if (more) fetch(first + step);
+        float sum[kSums];                                    // of each row: r' r', dh w2 r'; v d, v dh w2, v r' (v without a token's gate), next y's squares
+        #pragma unroll
+        for (int n = 0; n < Rows; ++n) {
             float2 v[4], dh[4], d[4], g[4], t[5];
             #pragma unroll
             for (int k = 0; k < 5; ++k) t[k] = both(0.f);
-            if (kY) bn_unpack(cy, v);
-            if (Kind == kBnElement) bn_unpack_gate<X, Vec>(q, cg, g);
-            if (Pre) bn_unpack(ch, dh);
-            if (kSumV) bn_unpack(cd, d);
+            if (kY) bn_unpack(cy[n], v);
+            if (Kind == kBnElement) bn_unpack_gate<X, Vec>(q, cg[n], g);
+            if (Pre) bn_unpack(ch[n], dh);
+            if (kSumV) bn_unpack(cd[n], d);
             #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (kY) {
-                    v[i] = mul2(Post ? mul2(v[i], both(i1)) : v[i], a[i]);
+                    v[i] = mul2(Post ? mul2(v[i], both(i1[n])) : v[i], a[i]);
                     if (Kind == kBnElement) v[i] = mul2(v[i], g[i]);
                 }
                 if (Pre) {
-                    if (kY) r[i] = fma2(v[i], both(gate), r[i]);
+                    if (kY) r[n][i] = fma2(v[i], both(gate[n]), r[n][i]);
                     dh[i] = mul2(dh[i], w[i]);
-                    t[0] = fma2(r[i], r[i], t[0]);
-                    t[1] = fma2(dh[i], r[i], t[1]);
+                    t[0] = fma2(r[n][i], r[n][i], t[0]);
+                    t[1] = fma2(dh[i], r[n][i], t[1]);
                 }
                 if (kSumV) {
                     t[2] = fma2(v[i], d[i], t[2]);
-                    if (Pre) { t[3] = fma2(v[i], dh[i], t[3]); t[4] = fma2(v[i], r[i], t[4]); }
+                    if (Pre) { t[3] = fma2(v[i], dh[i], t[3]); t[4] = fma2(v[i], r[n][i], t[4]); }
                 }
             }
-            #pragma unroll
-            for (int k = 0; k < 5; ++k) sum[k] = t[k].x + t[k].y;
-        }
-        if (Post) sum[5] = bn_square(ry);
-        if (kSumV) {
-            bn_sum<8>(sum, part, turn);
-        } else if (Pre) {
-            float two[2] = {sum[0], sum[1]};
-            bn_sum<2>(two, part, turn);
-            sum[0] = two[0];
-            sum[1] = two[1];
-        }
-        const float i2 = Pre ? rsqrtf(sum[0] * inv_h + q.eps) : 0.f, k = i2 * i2 * i2 * inv_h * sum[1];
-        const float vd = sum[2] + i2 * sum[3] - k * sum[4];
-        if (Kind == kBnToken && threadIdx.x == 0) {
-            if (sizeof(X) == 4 || q.gate32) static_cast<float*>(q.d_gate)[row * q.d_gate_ld] = vd;
-            else static_cast<X*>(q.d_gate)[row * q.d_gate_ld] = bn_round<X>(vd);
-        }
-        float2 d[4];
-        bn_unpack(cd, d);
-        if (Pre) {
-            float2 dh[4];
-            bn_unpack(ch, dh);
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 h2 = mul2(dh[i], both(i2));
-                acc_pre[i] = fma2(h2, r[i], acc_pre[i]);
-                d[i] = fma2(h2, w[i], fma2(r[i], both(-k), d[i]));
+            float* to = sum + n * (kSums / Rows);
+            to[0] = t[0].x + t[0].y;
+            to[1] = t[1].x + t[1].y;
+            if (kSumV) {
+                #pragma unroll
+                for (int k = 2; k < 5; ++k) to[k] = t[k].x + t[k].y;
+                to[5] = Post ? bn_square(ry[n]) : 0.f;
+                to[6] = to[7] = 0.f;
             }
         }
-        if (on) bn_put<R, Vec>(static_cast<R*>(q.d_residual) + static_cast<long long>(row) * q.d_residual_ld, q.hidden, d);
-        if (kY) {
-            const float2 y_up = both(i1 * gate), y_back = both(-i1 * i1 * gate * inv_h * vd);
-            float2 y[4];
-            bn_unpack(cy, y);
-            if (Kind == kBnElement) {
-                float2 g[4], dg[4];
-                bn_unpack_gate<X, Vec>(q, cg, g);
+        if (kSumV || Pre) bn_sum<kSums, kSums>(sum, part, turn);
+        float gate_back[Rows];
+        #pragma unroll
+        for (int n = 0; n < Rows; ++n) {
+            const long long row = first + n;
+            const bool there = n == 0 || row < tokens;
+            const float* of = sum + n * (kSums / Rows);
+            const float i2 = Pre ? rsqrtf(of[0] * inv_h + q.eps) : 0.f, k = Pre ? i2 * i2 * i2 * inv_h * of[1] : 0.f;
+            const float vd = kSumV ? (Pre ? of[2] + i2 * of[3] - k * of[4] : of[2]) : 0.f;
+            gate_back[n] = vd;
+            float2 d[4];
+            bn_unpack(cd[n], d);
+            if (Pre) {
+                float2 dh[4];
+                bn_unpack(ch[n], dh);
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    dg[i] = mul2(mul2(Post ? mul2(y[i], both(i1)) : y[i], a[i]), d[i]);
-                    d[i] = mul2(d[i], g[i]);
-                }
-                if (on) {
-                    const long long at = static_cast<long long>(row) * q.d_gate_ld;
-                    if (sizeof(X) == 4 || q.gate32) bn_put<float, Vec>(static_cast<float*>(q.d_gate) + at, q.hidden, dg);
-                    else bn_put<X, Vec>(static_cast<X*>(q.d_gate) + at, q.hidden, dg);
+                    const float2 h2 = mul2(dh[i], both(i2));
+                    acc_pre[i] = fma2(h2, r[n][i], acc_pre[i]);
+                    d[i] = fma2(h2, w[i], fma2(r[n][i], both(-k), d[i]));
                 }
             }
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 dy = Post || Kind == kBnToken ? mul2(d[i], y_up) : d[i];
-                acc_y[i] = fma2(dy, y[i], acc_y[i]);
-                d[i] = Post ? fma2(y[i], y_back, mul2(dy, a[i])) : mul2(dy, a[i]);
+            if (on && there) bn_put<R, Vec>(static_cast<R*>(q.d_residual) + row * q.d_residual_ld, q.hidden, d);
+            if (kY) {
+                const float2 y_up = both(i1[n] * gate[n]), y_back = both(-i1[n] * i1[n] * gate[n] * inv_h * vd);
+                float2 y[4];
+                bn_unpack(cy[n], y);
+                if (Kind == kBnElement) {
+                    float2 g[4], dg[4];
+                    bn_unpack_gate<X, Vec>(q, cg[n], g);
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        dg[i] = mul2(mul2(Post ? mul2(y[i], both(i1[n])) : y[i], a[i]), d[i]);
+                        d[i] = mul2(d[i], g[i]);
+                    }
+                    if (on && there) {
+                        const long long at = row * q.d_gate_ld;
+                        if (sizeof(X) == 4 || q.gate32) bn_put<float, Vec>(static_cast<float*>(q.d_gate) + at, q.hidden, dg);
+                        else bn_put<X, Vec>(static_cast<X*>(q.d_gate) + at, q.hidden, dg);
+                    }
+                }
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 dy = Post || Kind == kBnToken ? mul2(d[i], y_up) : d[i];
+                    acc_y[i] = fma2(dy, y[i], acc_y[i]);
+                    d[i] = Post ? fma2(y[i], y_back, mul2(dy, a[i])) : mul2(dy, a[i]);
+                }
+                if (on && there) bn_put<X, Vec>(static_cast<X*>(q.d_y) + row * q.d_y_ld, q.hidden, d);
             }
-            if (on) bn_put<X, Vec>(static_cast<X*>(q.d_y) + static_cast<long long>(row) * q.d_y_ld, q.hidden, d);
+            if (Post) i1[n] = rsqrtf(of[5] * inv_h + q.eps);
         }
-        if (Post) i1 = rsqrtf(sum[5] * inv_h + q.eps);
+        if (Kind == kBnToken && threadIdx.x < Rows && first + static_cast<int>(threadIdx.x) < tokens) {
+            const long long at = (first + static_cast<int>(threadIdx.x)) * q.d_gate_ld;
+            const float of = Rows == 2 && threadIdx.x == 1 ? gate_back[Rows - 1] : gate_back[0];
+            if (sizeof(X) == 4 || q.gate32) static_cast<float*>(q.d_gate)[at] = of;
+            else static_cast<X*>(q.d_gate)[at] = bn_round<X>(of);
+        }
         if (!more) break;
-        row += step;
+        first += step;
     }
     if (!on) return;
     float* p = q.partial + static_cast<long long>(blockIdx.x) * q.hidden;
@@ -833,7 +894,14 @@ int bn_per_sm(int threads, int* per) {
 
 template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec>
 int bn_launch_kind(const BnParams& q, const BnLaunch& how, cudaStream_t stream) {
-    if (how.backward) return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Vec>>(q, how.ctas, stream);
+    if (how.backward) {
+        if constexpr (Vec && Kind != kBnElement && sizeof(X) == 2) {
+            const int threads = bn_threads(q.hidden);
+            if (threads > kBnMaxThreads / 2 && threads <= kBnPairThreads && q.tokens >= 2ll * how.ctas)
+                return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, true, 2>>(q, how.ctas, stream);
+        }
+        return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Vec, 1>>(q, how.ctas, stream);
+    }
     int per = 0;
     const int st = bn_per_sm<block_norm_kernel<X, R, Post, Pre, Kind, Vec>>(bn_threads(q.hidden), &per);
     if (st != MM_OK) return st;

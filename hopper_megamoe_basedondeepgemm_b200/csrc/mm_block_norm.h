@@ -7,6 +7,7 @@ namespace mm {
 
 constexpr int kBnMaxHidden = 8192;
 constexpr int kBnMaxThreads = 512;
+constexpr int kBnPairThreads = 384;
 constexpr int kBnHeldHidden = 8 * kBnMaxThreads;             // up to here a thread holds eight channels of a row
 enum BnGate { kBnGateNone = 0, kBnGateChannel = 1, kBnGateToken = 2, kBnGateElement = 3 };
 

@@ -86,6 +86,17 @@ def test_many_rows(tokens, hidden):
     assert all(torch.equal(a, b) for a, b in zip(grads, again))            # the same sums in the same order
 
 
+@pytest.mark.parametrize('hidden', [2056, 2560, 3072])
+@pytest.mark.parametrize('tokens', [295, 296, 297, 741])
+def test_rows_in_pairs(tokens, hidden):
+    """Widths and row counts around those at which a CTA takes two rows at a time, the last pair without its second row."""
+    for i, kind in enumerate([dict(), dict(gate='token'), dict(gate='channel', post=False), dict(pre=False), dict(gate='element'), dict(y=False, post=False), dict(gate='token', pre=False)]):
+        types = TYPES[(i + tokens) % len(TYPES)]
+        x, d_stream, d_normed = _inputs(tokens, hidden, **{**types, 'stream': None}, **kind, seed=i)
+        _check_gradients(x, d_stream, d_normed, mm.block_norm_backward(d_stream, d_normed, **x))
+        assert all(a is None or torch.equal(a, b) for a, b in zip(mm.block_norm_backward(d_stream, d_normed, **x), mm.block_norm_backward(d_stream, d_normed, **x)))
+
+
 def test_one_gradient_only():
     x, d_stream, d_normed = _inputs(40, 512, gate='token')
     grads = mm.block_norm_backward(None, d_normed, **x)
