@@ -16,4 +16,16 @@ cudaError_t launch_behind(void (*kernel)(P), unsigned grid, unsigned threads, cu
     return cudaLaunchKernelEx(&cfg, kernel, params);
 }
 
+// One cluster of `ctas` CTAs (at most eight).
+template <typename P>
+cudaError_t launch_cluster(void (*kernel)(P), unsigned ctas, unsigned threads, cudaStream_t stream, const P& params) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(threads); cfg.stream = stream;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, params);
+}
+
 }  // namespace mm

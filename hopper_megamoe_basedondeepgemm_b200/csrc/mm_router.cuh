@@ -314,7 +314,7 @@ __device__ __forceinline__ void rt_scores(float (&l)[V], RtScores<V>& s) {
 }
 
 // Sums over the CTA, in a fixed order; the results are every thread's.
-template <int N>
+template <int N, int Warps = kRtWarps>
 __device__ __forceinline__ void rt_block_sum(double (&v)[N], double (*part)[N]) {
     #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -330,7 +330,7 @@ __device__ __forceinline__ void rt_block_sum(double (&v)[N], double (*part)[N]) 
     for (int n = 0; n < N; ++n) {
         v[n] = 0.0;
         #pragma unroll
-        for (int w = 0; w < kRtWarps; ++w) v[n] += part[w][n];
+        for (int w = 0; w < Warps; ++w) v[n] += part[w][n];
     }
 }
 
@@ -398,21 +398,15 @@ __global__ void __launch_bounds__(256) balance_zero_kernel(const RtParams q) {
     for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < q.zero_words; i += static_cast<long long>(gridDim.x) * blockDim.x) p[i] = 0ull;
 }
 
-// A CTA takes consecutive tokens, piece by piece of one sequence each: its warps add the probabilities up in registers, the CTA adds the warps' sums and puts them to the
-// sequence's. The last CTA to end turns the sums into the results where they are few. A token's logits are asked for while the one before is worked on.
-template <typename L, int V, int Mode>
-__global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(const RtParams q) {
-    __shared__ float warp_sum[kRtWarps][V * 32];
-    __shared__ int hist[V * 32], warp_tokens[kRtWarps];
-    __shared__ double warp_z[kRtWarps];
-    __shared__ bool last;
+// The tokens lo to hi - 1, piece by piece of one sequence each: the CTA's warps take them in turn and add up their probabilities in registers, a token's logits asked for while
+// the one before is worked on. `count(s, e)` is told every slot; `flush(s, acc, n)` at the end of a piece what a warp has summed, and of how many
+// tokens. Returns the warp's sum of squares.
+template <typename L, int V, int Mode, int Warps, typename Count, typename Flush>
+__device__ __forceinline__ double rt_balance_tokens(const RtParams& q, int lo, int hi, Count count, Flush flush) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int lo = static_cast<int>(static_cast<long long>(q.T) * blockIdx.x / gridDim.x), hi = static_cast<int>(static_cast<long long>(q.T) * (blockIdx.x + 1) / gridDim.x);
-    for (int e = threadIdx.x; e < V * 32; e += blockDim.x) hist[e] = 0;
-    __syncthreads();
     float l[V];
     long long route = -1;
-    // (a warp's tokens are every eighth of the CTA's, whatever the pieces)
+    // (a warp's tokens are one in `Warps` of the CTA's, whatever the pieces)
     auto fetch = [&](int r) {
         if (r < hi) {
             rt_fetch<L, V>(q, r, lane, l);
@@ -423,7 +417,6 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
     fetch(mine);
     double z = 0.0;
     int row = lo;
-    bool zeroed = false;
     while (row < hi) {
         int s = 0, end = hi;
         if (q.cu != nullptr) {
@@ -437,19 +430,19 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
                 end = min(hi, max(q.cu[s + 1], row + 1));
             }
         }
-        end = min(end, row + kRtFlushRows * kRtWarps);
+        end = min(end, row + kRtFlushRows * Warps);
         float acc[V] = {};
         int n = 0;
-        for (; mine < end; mine += kRtWarps) {
+        for (; mine < end; mine += Warps) {
             float x[V];
             RtScores<V> scores;
             #pragma unroll
             for (int j = 0; j < V; ++j) x[j] = l[j];
             const long long e = route;
-            fetch(mine + kRtWarps);
+            fetch(mine + Warps);
             const bool slot = s >= 0 && e >= 0 && e < q.E;
             if (__ballot_sync(0xffffffffu, slot) == 0u) continue;
-            if (slot) atomicAdd(hist + e, 1);
+            if (slot) count(s, static_cast<int>(e));
             rt_scores<V, Mode, false>(x, scores);
             #pragma unroll
             for (int j = 0; j < V; ++j) acc[j] = Mode == 1 ? fmaf(scores.sig[j], scores.sig_scale, acc[j]) : fmaf(scores.exp[j], scores.exp_scale, acc[j]);
@@ -457,28 +450,48 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
             ++n;
         }
         row = end;
-        if (s < 0) continue;
-        if (!zeroed) { grid_dependency_wait(); zeroed = true; }              // (the sums are zero now)
-        #pragma unroll
-        for (int j = 0; j < V; ++j) warp_sum[warp][j * 32 + lane] = acc[j];
-        if (lane == 0) warp_tokens[warp] = n;
-        __syncthreads();
-        for (int e = threadIdx.x; e < q.E; e += blockDim.x) {
-            unsigned long long sum = 0ull;
-            #pragma unroll
-            for (int w = 0; w < kRtWarps; ++w) sum += __float2ull_rn(warp_sum[w][e] * kRtFixed);
-            const long long to = static_cast<long long>(s) * q.E + e;
-            if (sum != 0ull) atomicAdd(q.sums + to, sum);
-            if (hist[e] != 0) { atomicAdd(q.sum_counts + to, hist[e]); hist[e] = 0; }
-        }
-        if (threadIdx.x == 0) {
-            int all = 0;
-            #pragma unroll
-            for (int w = 0; w < kRtWarps; ++w) all += warp_tokens[w];
-            if (all > 0) atomicAdd(q.sum_tokens + s, all);
-        }
-        __syncthreads();
+        if (s >= 0) flush(s, acc, n);
     }
+    return z;
+}
+
+// Many tokens: a CTA adds its warps' sums up and puts them to the sequence's in memory, which `balance_zero_kernel` has cleared. The last CTA to end turns the
+// sums into the results where they are few.
+template <typename L, int V, int Mode>
+__global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(const RtParams q) {
+    __shared__ float warp_sum[kRtWarps][V * 32];
+    __shared__ int hist[V * 32], warp_tokens[kRtWarps];
+    __shared__ double warp_z[kRtWarps];
+    __shared__ bool last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lo = static_cast<int>(static_cast<long long>(q.T) * blockIdx.x / gridDim.x), hi = static_cast<int>(static_cast<long long>(q.T) * (blockIdx.x + 1) / gridDim.x);
+    for (int e = threadIdx.x; e < V * 32; e += blockDim.x) hist[e] = 0;
+    __syncthreads();
+    bool zeroed = false;
+    const double z = rt_balance_tokens<L, V, Mode, kRtWarps>(
+        q, lo, hi, [&](int, int e) { atomicAdd(hist + e, 1); },
+        [&](int s, const float (&acc)[V], int n) {
+            if (!zeroed) { grid_dependency_wait(); zeroed = true; }          // (the sums are zero now)
+            #pragma unroll
+            for (int j = 0; j < V; ++j) warp_sum[warp][j * 32 + lane] = acc[j];
+            if (lane == 0) warp_tokens[warp] = n;
+            __syncthreads();
+            for (int e = threadIdx.x; e < q.E; e += blockDim.x) {
+                unsigned long long sum = 0ull;
+                #pragma unroll
+                for (int w = 0; w < kRtWarps; ++w) sum += __float2ull_rn(warp_sum[w][e] * kRtFixed);
+                const long long to = static_cast<long long>(s) * q.E + e;
+                if (sum != 0ull) atomicAdd(q.sums + to, sum);
+                if (hist[e] != 0) { atomicAdd(q.sum_counts + to, hist[e]); hist[e] = 0; }
+            }
+            if (threadIdx.x == 0) {
+                int all = 0;
+                #pragma unroll
+                for (int w = 0; w < kRtWarps; ++w) all += warp_tokens[w];
+                if (all > 0) atomicAdd(q.sum_tokens + s, all);
+            }
+            __syncthreads();
+        });
     if (!zeroed) grid_dependency_wait();
     if (lane == 0) warp_z[warp] = z;
     __syncthreads();
@@ -489,6 +502,106 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
         q.z_part[blockIdx.x] = sum;
     }
     if (static_cast<long long>(q.S) * q.E <= kRtEndCells && rt_last_cta(q.ticket, &last)) rt_balance_results(q, true, 0.0);
+}
+
+// Few tokens: one cluster, whose CTAs keep their sums in shared memory and add up each other's: one launch, nothing in memory but the results. A call from Python takes
+// 2.5 us less of the host than with two launches (with the gradient 12.9 and 15.4 us a pass). On the GPU 16 tokens of 48 experts take 4.7 us (6.4), 64 5.4 (6.4), 256 6.5
+// (6.4), 400 7.2 (6.4): the border is where that costs more than it gives.
+template <typename T>
+__device__ __forceinline__ T rt_of_cta(const T* p, uint32_t rank) {      // the same variable of another CTA of the cluster
+    static_assert(sizeof(T) == 4 || sizeof(T) == 8);
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    if constexpr (sizeof(T) == 4) {
+        uint32_t v;
+        asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+        return *reinterpret_cast<T*>(&v);
+    } else {
+        unsigned long long v;
+        asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+        return *reinterpret_cast<T*>(&v);
+    }
+}
+
+template <typename L, int V, int Mode>
+__global__ void __launch_bounds__(kRtSmallWarps * 32) balance_small_kernel(const RtParams q) {
+    __shared__ float warp_sum[kRtSmallWarps][V * 32], sums[kRtSmallCells];
+    __shared__ int counts[kRtSmallCells], tokens[kRtSmallSequences];
+    __shared__ double warp_z[kRtSmallWarps], cta[2], part[kRtSmallWarps][1];       // cta: sum of squares; what its cells add to the balance loss
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t rank = cluster_rank(), ctas = gridDim.x;
+    const int cells = q.S * q.E;
+    const int lo = static_cast<int>(static_cast<long long>(q.T) * rank / ctas), hi = static_cast<int>(static_cast<long long>(q.T) * (rank + 1) / ctas);
+    for (int i = threadIdx.x; i < cells; i += blockDim.x) { sums[i] = 0.f; counts[i] = 0; }
+    for (int i = threadIdx.x; i < q.S; i += blockDim.x) tokens[i] = 0;
+    __syncthreads();
+    const double z = rt_balance_tokens<L, V, Mode, kRtSmallWarps>(
+        q, lo, hi, [&](int s, int e) { atomicAdd(counts + s * q.E + e, 1); },
+        [&](int s, const float (&acc)[V], int n) {
+            #pragma unroll
+            for (int j = 0; j < V; ++j) warp_sum[warp][j * 32 + lane] = acc[j];
+            if (lane == 0 && n > 0) atomicAdd(tokens + s, n);
+            __syncthreads();
+            for (int e = threadIdx.x; e < q.E; e += blockDim.x) {
+                float sum = sums[s * q.E + e];
+                #pragma unroll
+                for (int w = 0; w < kRtSmallWarps; ++w) sum += warp_sum[w][e];
+                sums[s * q.E + e] = sum;
+            }
+            __syncthreads();
+        });
+    if (lane == 0) warp_z[warp] = z;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double sum = 0.0;
+        #pragma unroll
+        for (int w = 0; w < kRtSmallWarps; ++w) sum += warp_z[w];
+        cta[0] = sum;
+    }
+    cluster_arrive();
+    cluster_wait();
+    double balance[1] = {0.0};
+    for (int i = static_cast<int>(rank * blockDim.x + threadIdx.x); i < cells; i += static_cast<int>(ctas * blockDim.x)) {
+        const int s = q.S == 1 ? 0 : i / q.E;
+        float sum = 0.f;
+        int count = 0, n = 0;
+        for (uint32_t r = 0; r < ctas; ++r) {
+            sum += rt_of_cta(sums + i, r);
+            count += rt_of_cta(counts + i, r);
+            n += rt_of_cta(tokens + s, r);
+        }
+        const float inv = n > 0 ? 1.f / static_cast<float>(n) : 0.f, mean = sum * inv;
+        q.mean[i] = mean;
+        q.counts[i] = count;
+        balance[0] += static_cast<double>(static_cast<float>(count) * inv) * static_cast<double>(mean);
+    }
+    rt_block_sum<1, kRtSmallWarps>(balance, part);
+    if (threadIdx.x == 0) cta[1] = balance[0];
+    cluster_arrive();
+    cluster_wait();
+    if (rank == 0 && warp == 0) {
+        int live = 0, all = 0;
+        for (int s = lane; s < q.S; s += 32) {
+            int n = 0;
+            for (uint32_t r = 0; r < ctas; ++r) n += rt_of_cta(tokens + s, r);
+            q.tokens[s] = n;
+            live += n > 0;
+            all += n;
+        }
+        live = __reduce_add_sync(0xffffffffu, live);
+        all = __reduce_add_sync(0xffffffffu, all);
+        if (lane == 0) {
+            double b = 0.0, squares = 0.0;
+            for (uint32_t r = 0; r < ctas; ++r) { b += rt_of_cta(cta + 1, r); squares += rt_of_cta(cta, r); }
+            b = live > 0 ? b * q.E / q.K / live : 0.0;
+            squares = all > 0 ? squares / all : 0.0;
+            q.losses[0] = static_cast<float>(q.balance_coef * b + q.z_coef * squares);
+            q.losses[1] = static_cast<float>(b);
+            q.losses[2] = static_cast<float>(squares);
+        }
+    }
+    cluster_arrive();                        // (no CTA leaves while its shared memory is read)
+    cluster_wait();
 }
 
 // The same for many sums: by as many CTAs as there are thousands of them; the last one adds up what the others found.
@@ -636,6 +749,14 @@ template <typename L, int V, int Mode>
 int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
     const int blocks = (q.T + kRtWarps - 1) / kRtWarps, resident = rt_ctas<V>() * sms;
     const int grid = blocks < 1 ? 1 : (blocks < resident ? blocks : resident);
+    if constexpr (V <= kRtSmallExperts / 32) {
+        if (op == kRtBalance && q.T <= kRtSmallTokens && static_cast<long long>(q.S) * q.E <= kRtSmallCells && q.S <= kRtSmallSequences) {
+            // (sequences: all the CTAs there can be, because each takes its pieces of them one after the other)
+            const int want = q.S > 1 ? q.T : (q.T + kRtSmallWarps - 1) / kRtSmallWarps, ctas = want < 1 ? 1 : (want < kRtSmallCtas ? want : kRtSmallCtas);
+            MM_CUDA(launch_cluster(balance_small_kernel<L, V, Mode>, ctas, kRtSmallWarps * 32, stream, q));
+            return MM_OK;
+        }
+    }
     if (op == kRtBalance) {
         RtParams b = q;
         // one sequence: two CTAs an SM at most, because what each CTA adds to the same sums and counts costs more than its share of the tokens (16384 tokens of 48 experts

@@ -10,6 +10,9 @@ constexpr int kRtMaxExperts = 1024, kRtMaxTopk = 32, kRtWarps = 8;
 constexpr int kRtBalanceCtas = 1184;         // of the balance kernel at most (eight per SM of 148): the workspace does not depend on the device
 constexpr int kRtEndCells = 8192;            // counts that the balance kernel's last CTA turns into the results itself; more of them get a launch of their own
 
+// A balance loss of so few tokens, sequences and sums is one cluster's work.
+constexpr int kRtSmallTokens = 384, kRtSmallCells = 2048, kRtSmallSequences = 512, kRtSmallExperts = 384, kRtSmallCtas = 8, kRtSmallWarps = 16;
+
 struct RtParams {
     const void* logits;
     long long logits_ld;

@@ -210,7 +210,7 @@ def test_balance_and_gradient(experts, topk, dtype, mode):
         _check_gradient(logits, idx, mode, None, None, None, 1.5, dw, None, mm.router_backward(logits, idx, mode, d_topk_weights=dw, route_scale=1.5))
 
 
-@pytest.mark.parametrize('tokens, experts, sequences', [(20000, 48, 0), (9000, 384, 3), (5000, 64, 600), (40, 16, 2000)])
+@pytest.mark.parametrize('tokens, experts, sequences', [(20000, 48, 0), (383, 64, 32), (384, 64, 32), (385, 64, 32), (384, 64, 33), (384, 384, 5), (384, 385, 3), (384, 4, 511), (384, 4, 513), (9, 256, 8), (9000, 384, 3), (5000, 64, 600), (40, 16, 2000)])
 @pytest.mark.parametrize('mode', [0, 1])
 def test_many_tokens_and_sequences(tokens, experts, sequences, mode):
     logits = _logits(tokens, experts)
@@ -333,10 +333,11 @@ def test_sums_over_ranks():
     assert torch.equal(torch.cat([mm.router_backward(l, i, balance=b) for (l, i), b in zip(halves, parts)]), want)
 
 
-def test_captured_and_replayed():
+@pytest.mark.parametrize('tokens', [300, 2000])
+def test_captured_and_replayed(tokens):
     """A training step's calls as a graph, replayed with new logits, two graphs at once."""
-    logits, dw = _logits(500, 96), _logits(500, 8, seed=5)
-    cu = _sequences(500, 6)
+    logits, dw = _logits(tokens, 96), _logits(tokens, 8, seed=5)
+    cu = _sequences(tokens, 6)
 
     def step(l):
         idx, w = mm.route_tokens(l, 8, 1, route_scale=2.0)
@@ -349,7 +350,7 @@ def test_captured_and_replayed():
         with torch.cuda.graph(g):
             out = step(logits)
         graphs.append((g, out))
-    logits.copy_(_logits(500, 96, seed=8))
+    logits.copy_(_logits(tokens, 96, seed=8))
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
     torch.cuda.synchronize()
     for _ in range(3):
