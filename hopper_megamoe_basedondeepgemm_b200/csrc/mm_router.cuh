@@ -83,6 +83,9 @@ __device__ __forceinline__ void rt_clean(float (&l)[V]) {
     for (int j = 0; j < V; ++j) l[j] = rt_logit(l[j]);
 }
 
+// The first token of a share, of those that the launch deals out.
+__device__ __forceinline__ int rt_share(const RtParams& q, int n) { return n * q.share + min(n, q.shares_more); }
+
 // The sequence of a token that lies at or behind cu[0], by a whole warp: S if it is behind the last one. Each step looks at 32 ends at once. Reads cu alone, whatever
 // it holds, and where the result is below S, cu[result + 1] is above the token.
 __device__ __forceinline__ int rt_sequence(const int* cu, int S, int row) {
@@ -464,7 +467,7 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
     __shared__ double warp_z[kRtWarps];
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int lo = static_cast<int>(static_cast<long long>(q.T) * blockIdx.x / gridDim.x), hi = static_cast<int>(static_cast<long long>(q.T) * (blockIdx.x + 1) / gridDim.x);
+    const int lo = rt_share(q, blockIdx.x), hi = rt_share(q, blockIdx.x + 1);
     for (int e = threadIdx.x; e < V * 32; e += blockDim.x) hist[e] = 0;
     __syncthreads();
     bool zeroed = false;
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(kRtSmallWarps * 32) balance_small_kernel(const
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rank = cluster_rank(), ctas = gridDim.x;
     const int cells = q.S * q.E;
-    const int lo = static_cast<int>(static_cast<long long>(q.T) * rank / ctas), hi = static_cast<int>(static_cast<long long>(q.T) * (rank + 1) / ctas);
+    const int lo = rt_share(q, rank), hi = rt_share(q, rank + 1);
     for (int i = threadIdx.x; i < cells; i += blockDim.x) { sums[i] = 0.f; counts[i] = 0; }
     for (int i = threadIdx.x; i < q.S; i += blockDim.x) tokens[i] = 0;
     __syncthreads();
@@ -625,8 +628,7 @@ template <typename L, int V, int Mode>
 __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) router_backward_kernel(const RtParams q) {
     __shared__ float rows[kRtWarps][V * 32];
     const int lane = threadIdx.x & 31, warp_in = threadIdx.x >> 5;
-    const int warp = blockIdx.x * kRtWarps + warp_in, warps = gridDim.x * kRtWarps;
-    const int lo = static_cast<int>(static_cast<long long>(q.T) * warp / warps), hi = static_cast<int>(static_cast<long long>(q.T) * (warp + 1) / warps);
+    const int lo = rt_share(q, blockIdx.x * kRtWarps + warp_in), hi = rt_share(q, blockIdx.x * kRtWarps + warp_in + 1);
     float* buf = rows[warp_in];
     float c[V], ahead[V], dw_ahead = 0.f;
     long long e_ahead = -1;
@@ -681,7 +683,7 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) router_backward_k
                 }
                 seq = s;
                 const float n = s < q.S ? static_cast<float>(q.tokens[s]) : 0.f;
-                const float f = n > 0.f ? q.balance_coef * g * static_cast<float>(q.E) / (static_cast<float>(q.K) * n * n * live) : 0.f;
+                const float f = n > 0.f ? __fdividef(q.balance_coef * g * static_cast<float>(q.E), static_cast<float>(q.K) * n) * __fdividef(1.f, n * live) : 0.f;
                 #pragma unroll
                 for (int j = 0; j < V; ++j)
                     c[j] = s < q.S && j * 32 + lane < q.E ? f * static_cast<float>(q.counts[static_cast<long long>(s) * q.E + j * 32 + lane]) : 0.f;
@@ -749,21 +751,28 @@ template <typename L, int V, int Mode>
 int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
     const int blocks = (q.T + kRtWarps - 1) / kRtWarps, resident = rt_ctas<V>() * sms;
     const int grid = blocks < 1 ? 1 : (blocks < resident ? blocks : resident);
+    auto shared_out = [&](int shares) {
+        RtParams p = q;
+        p.share = q.T / shares;
+        p.shares_more = q.T % shares;
+        return p;
+    };
     if constexpr (V <= kRtSmallExperts / 32) {
         if (op == kRtBalance && q.T <= kRtSmallTokens && static_cast<long long>(q.S) * q.E <= kRtSmallCells && q.S <= kRtSmallSequences) {
             // (sequences: all the CTAs there can be, because each takes its pieces of them one after the other)
             const int want = q.S > 1 ? q.T : (q.T + kRtSmallWarps - 1) / kRtSmallWarps, ctas = want < 1 ? 1 : (want < kRtSmallCtas ? want : kRtSmallCtas);
-            MM_CUDA(launch_cluster(balance_small_kernel<L, V, Mode>, ctas, kRtSmallWarps * 32, stream, q));
+            MM_CUDA(launch_cluster(balance_small_kernel<L, V, Mode>, ctas, kRtSmallWarps * 32, stream, shared_out(ctas)));
             return MM_OK;
         }
     }
     if (op == kRtBalance) {
-        RtParams b = q;
         // one sequence: two CTAs an SM at most, because what each CTA adds to the same sums and counts costs more than its share of the tokens (16384 tokens of 48 experts
         // 10.0 us, with five an SM 11.8); several sequences: all that fit, because a CTA takes its pieces of sequences one after the other (12000 tokens of 128
         // experts in 37 sequences 16.2 us, with two an SM 18.0)
         const int most = q.cu == nullptr && 2 * sms < kRtBalanceCtas ? 2 * sms : kRtBalanceCtas;
-        b.z_parts = grid < most ? grid : most;
+        const int ctas = grid < most ? grid : most;
+        RtParams b = shared_out(ctas);
+        b.z_parts = ctas;
         const long long zero = (b.zero_words + 1023) / 1024;
         balance_zero_kernel<L><<<static_cast<int>(zero < sms ? zero : sms), 256, 0, stream>>>(b);
         MM_CUDA(cudaGetLastError());
@@ -777,7 +786,7 @@ int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
     } else if (op == kRtRoute) {
         route_kernel<L, V, Mode><<<blocks < sms * 8 ? blocks : sms * 8, kRtWarps * 32, 0, stream>>>(q);
     } else {
-        router_backward_kernel<L, V, Mode><<<grid, kRtWarps * 32, 0, stream>>>(q);
+        router_backward_kernel<L, V, Mode><<<grid, kRtWarps * 32, 0, stream>>>(shared_out(grid * kRtWarps));
     }
     MM_CUDA(cudaGetLastError());
     return MM_OK;

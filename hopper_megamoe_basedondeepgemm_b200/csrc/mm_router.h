@@ -22,6 +22,7 @@ struct RtParams {
     float* weights;                          // [T][K]
     const int* cu;                           // [S + 1], or nullptr: one sequence of all tokens
     int T, E, K, S, mode;
+    int share, shares_more;                  // tokens of a CTA or warp, and how many of the first ones have one more
     float route_scale, balance_coef, z_coef, d_loss;
     const float* d_loss_ptr;                 // device scalar, or nullptr: d_loss
     const float* d_weights;                  // [T][K] or nullptr
