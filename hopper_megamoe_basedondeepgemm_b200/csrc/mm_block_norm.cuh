@@ -531,33 +531,41 @@ __device__ __forceinline__ void bn_clear(uint32_t (&w)[N]) {
 // What there is in a call, as far as it shapes the loop over the rows.
 enum BnKind { kBnPlain = 0 /* no gate, or one that is part of y's factor */, kBnToken = 1, kBnElement = 2, kBnStream = 3 /* no y */ };
 
-// 64 registers a thread, so two CTAs of 512 threads an SM. 16384 x 4096, 32-bit stream, both norms, channel gate: 130 us (6.2 TB/s); of 8192 x 3072 in bf16 40 us.
-// (One CTA of twice the registers per SM 168 us; sixteen channels a thread 134; rows copied ahead into shared memory by cp.async 160.)
+// 64 registers a thread, so two CTAs of 512 threads an SM; 16-bit streams 56, so three of 384. 16384 x 4096, 32-bit stream, both norms, channel gate: 127 us (6.3 TB/s); 8192 x
+// 3072 in bf16 37 us (5.4). (One CTA of twice the registers an SM 168 us; sixteen channels a thread 134; rows copied ahead into shared memory by cp.async
+// 160. y one row ahead, bf16 40 us; two rows ahead with a 32-bit stream, which then has no register left, 137.)
 template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec>
-__global__ void __maxnreg__((sizeof(R) == 2 && Vec ? 56 : 64)) block_norm_kernel(const BnParams q) {
+__global__ void __maxnreg__((sizeof(R) == 2 && Vec && Kind != kBnElement ? 56 : 64)) block_norm_kernel(const BnParams q) {
     __shared__ __align__(16) float part[2][2][kBnSumWarps];
     const float inv_h = 1.f / static_cast<float>(q.hidden);
+    constexpr bool kFar = Post && Vec && sizeof(R) == 2;      // y two rows ahead: its squares are summed a row before its turn
     const int step = gridDim.x, tokens = static_cast<int>(q.tokens);
     const bool on = !Vec || static_cast<int>(threadIdx.x) * 8 < q.hidden;
     BnAhead<R, Vec> rr;
-    BnAhead<X, Vec> ry;
+    BnAhead<X, Vec> ry, ry_far;
     uint32_t rg[8];
     float2 a[4], w[4];
     uint32_t gate_bits = 0u;
     bn_clear(rr.w);
     bn_clear(ry.w);
+    bn_clear(ry_far.w);
     bn_clear(rg);
     #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = w[i] = both(0.f);
     auto fetch = [&](long long row) {
         if (on) {
-            if (Kind != kBnStream) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry);
+            if (kFar) {
+                if (row + step < tokens) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + (row + step) * q.y_ld, q.hidden, ry_far);
+            } else if (Kind != kBnStream) {
+                bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry);
+            }
             bn_fetch<R, Vec>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, rr);
             if (Kind == kBnElement) bn_fetch_gate<X, Vec>(q, row, rg);
         }
         if (Kind == kBnToken) gate_bits = bn_gate_bits<X>(q, row);
     };
     int row = blockIdx.x;
+    if (kFar && on) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry);
     fetch(row);
     if (on) {
         if (Kind != kBnStream) bn_y_factor<X, Vec>(q, a);
@@ -578,6 +586,7 @@ __global__ void __maxnreg__((sizeof(R) == 2 && Vec ? 56 : 64)) block_norm_kernel
         if (Kind != kBnStream) bn_unpack(bn_take(ry), v);
         if (Kind == kBnElement) bn_unpack_gate<X, Vec>(q, rg, g);
         const float f = Kind == kBnToken ? i1 * bn_gate_value<X>(q, gate_bits) : i1;
+        if (kFar) ry = ry_far;
         if (more) fetch(row + step);
         if (Kind != kBnStream) {
             #pragma unroll
