@@ -22,7 +22,7 @@ SOURCES = {
     **{f'mm_router_{t}.cu': ['mm_router.cuh', 'mm_router.h', 'mm_launch.h', 'mm_ptx.cuh', 'mm_error.h', _ABI] for t in ('bf16', 'fp16', 'fp32')},
 }
 CHECK_SOURCES = ('mm_abi.cu',)           # those that the test build compiles anew; it shares the others' objects
-OBJ_DIR = os.path.join(PKG_DIR, 'build')
+OBJ_DIR = os.path.join(PKG_DIR, 'obj')
 
 
 def _stale(path: str, files) -> bool:

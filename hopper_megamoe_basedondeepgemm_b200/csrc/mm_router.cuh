@@ -12,8 +12,8 @@
 //             over the selected slots; of the square 2 lse softmax_e.
 //
 // One warp holds a token's logits in registers, expert j * 32 + lane in slot j of a lane: neighbouring lanes read neighbouring experts wherever a row starts,
-// and the order of slots and lanes is that of the experts. Bound by instructions more than by memory: some 300 to 400 a token against 4 bytes an
-// expert.
+// and the order of slots and lanes is that of the experts. Bound by instructions more than by memory: 680 a token to route one over 384 experts,
+// 250 for its balance loss, 420 for its gradient, against 4 bytes an expert.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

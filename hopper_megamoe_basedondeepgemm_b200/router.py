@@ -19,8 +19,8 @@ def route_tokens(logits: torch.Tensor, topk: int, score_mode: int = 0, expert_bi
 
     score_mode 0: the largest logits; weights are the softmax over the selected ones. 1: the largest `sigmoid(logit) + expert_bias` (fp32
     `[experts]`, optional), compared as in 64 bits; weights are the sigmoids over their sum. Both times `route_scale`. Experts come in descending
-    order, equal ones lower index first. A logit of -inf or NaN switches an expert off for the token. Slots for which no expert is left, and
-    tokens whose `valid` (bool or uint8 `[tokens]`) is 0, get index -1 and weight 0: the layer's masked slots. `topk_idx` / `topk_weights` may
+    order, equal ones lower index first. A logit of -inf or NaN switches an expert off for the token, a bias of -inf or NaN for all. Slots for which no expert is left,
+    and tokens whose `valid` (bool or uint8 `[tokens]`) is 0, get index -1 and weight 0: the layer's masked slots. `topk_idx` / `topk_weights` may
     be given, e.g. `sym_buffer.topk_idx[:tokens]`. At most 1024 experts and 32 routes per token.
     """
     return binding.route_tokens(logits, topk, score_mode, expert_bias, valid, route_scale, topk_idx, topk_weights)
