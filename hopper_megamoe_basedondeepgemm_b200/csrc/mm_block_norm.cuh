@@ -552,6 +552,8 @@ __global__ void __maxnreg__((sizeof(R) == 2 && Vec && Kind != kBnElement ? 56 : 
     bn_clear(rg);
     #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = w[i] = both(0.f);
+    grid_dependency_wait();
+    grid_launch_dependents();
     auto fetch = [&](long long row) {
         if (on) {
             if (kFar) {
@@ -687,13 +689,14 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
         }
     };
     int first = blockIdx.x * Rows;
+    grid_dependency_wait();
+    grid_launch_dependents();                                // (the sums' kernel waits for this one's end by itself)
     if (Post) {
         fetch_y(first);
         #pragma unroll
         for (int n = 0; n < Rows; ++n) ry[n] = bn_take(ry_ahead[n]);
     }
     fetch(first);
-    grid_launch_dependents();                                // (the sums' kernel waits for this one's end by itself)
     if (on) {
         if (kY) bn_y_factor<X, Vec>(q, a);
         if (Pre) bn_pre_factor<X, Vec>(q, w);
@@ -844,6 +847,7 @@ __global__ void __launch_bounds__(kBnSumThreads) block_norm_sums_kernel(const Bn
     float v[4] = {};
     const float* p = q.partial + static_cast<long long>(which) * q.rows * q.hidden + h0 + col;
     grid_dependency_wait();
+    grid_launch_dependents();
     if ((q.hidden & 3) == 0) {
         if (h0 + col < q.hidden) {
             #pragma unroll 5
@@ -887,6 +891,11 @@ int bn_start(const BnParams& q, int grid, cudaStream_t stream) {
     MM_CUDA(cudaGetLastError());
     return MM_OK;
 }
+template <auto Kernel>
+int bn_start_behind(const BnParams& q, int grid, cudaStream_t stream) {
+    MM_CUDA(launch_behind(Kernel, grid, bn_threads(q.hidden), stream, q));
+    return MM_OK;
+}
 
 // CTAs of a kernel that an SM holds; asked for once per CTA size and kernel (the answer is the binary's and the GPU's, of which there is one kind).
 template <auto Kernel>
@@ -907,15 +916,15 @@ int bn_launch_kind(const BnParams& q, const BnLaunch& how, cudaStream_t stream) 
         if constexpr (Vec && Kind != kBnElement && sizeof(X) == 2) {
             const int threads = bn_threads(q.hidden);
             if (threads > kBnMaxThreads / 2 && threads <= kBnPairThreads && q.tokens >= 2ll * how.ctas)
-                return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, true, 2>>(q, how.ctas, stream);
+                return bn_start_behind<block_norm_backward_kernel<X, R, Post, Pre, Kind, true, 2>>(q, how.ctas, stream);
         }
-        return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Vec, 1>>(q, how.ctas, stream);
+        return bn_start_behind<block_norm_backward_kernel<X, R, Post, Pre, Kind, Vec, 1>>(q, how.ctas, stream);
     }
     int per = 0;
     const int st = bn_per_sm<block_norm_kernel<X, R, Post, Pre, Kind, Vec>>(bn_threads(q.hidden), &per);
     if (st != MM_OK) return st;
     const long long most = static_cast<long long>(per) * how.sms;
-    return bn_start<block_norm_kernel<X, R, Post, Pre, Kind, Vec>>(q, static_cast<int>(q.tokens < most ? q.tokens : most), stream);
+    return bn_start_behind<block_norm_kernel<X, R, Post, Pre, Kind, Vec>>(q, static_cast<int>(q.tokens < most ? q.tokens : most), stream);
 }
 
 template <typename X, typename R, bool Vec>

@@ -1,5 +1,6 @@
 // A launch that may begin before the kernel ahead of it in its stream has ended: its launch and the part of it before `grid_dependency_wait` overlap with that kernel's
-// end. What that kernel (and, by its own order, those ahead of it) wrote is there after the wait.
+// end. What that kernel wrote is there after the wait. A kernel launched so lets the next one in (`grid_launch_dependents`) only behind its own wait: then whatever
+// runs early has at most one kernel of its stream ahead of it that has not ended, and waits for that one.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -16,15 +17,17 @@ cudaError_t launch_behind(void (*kernel)(P), unsigned grid, unsigned threads, cu
     return cudaLaunchKernelEx(&cfg, kernel, params);
 }
 
-// One cluster of `ctas` CTAs (at most eight).
+// One cluster of `ctas` CTAs (at most eight), as early.
 template <typename P>
 cudaError_t launch_cluster(void (*kernel)(P), unsigned ctas, unsigned threads, cudaStream_t stream, const P& params) {
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(threads); cfg.stream = stream;
-    cfg.attrs = attr; cfg.numAttrs = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, params);
 }
 

@@ -150,6 +150,8 @@ __global__ void __launch_bounds__(kRtWarps * 32) route_kernel(const RtParams q) 
     __shared__ int cand_at[kRtWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t below = (1u << lane) - 1u;
+    grid_dependency_wait();
+    grid_launch_dependents();
     for (int row = blockIdx.x * kRtWarps + warp; row < q.T; row += gridDim.x * kRtWarps) {
         int rank = q.K, at = -1, taken = 0;                              // this lane's expert and its place
         float logit = rt_off();
@@ -396,6 +398,7 @@ __device__ __forceinline__ bool rt_last_cta(unsigned* ticket, bool* last) {
 
 template <typename L>
 __global__ void __launch_bounds__(256) balance_zero_kernel(const RtParams q) {
+    grid_dependency_wait();
     grid_launch_dependents();
     unsigned long long* p = q.sums;
     for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < q.zero_words; i += static_cast<long long>(gridDim.x) * blockDim.x) p[i] = 0ull;
@@ -468,6 +471,7 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lo = rt_share(q, blockIdx.x), hi = rt_share(q, blockIdx.x + 1);
+    grid_launch_dependents();                // (what was ahead of `balance_zero_kernel` has ended)
     for (int e = threadIdx.x; e < V * 32; e += blockDim.x) hist[e] = 0;
     __syncthreads();
     bool zeroed = false;
@@ -538,6 +542,8 @@ __global__ void __launch_bounds__(kRtSmallWarps * 32) balance_small_kernel(const
     for (int i = threadIdx.x; i < cells; i += blockDim.x) { sums[i] = 0.f; counts[i] = 0; }
     for (int i = threadIdx.x; i < q.S; i += blockDim.x) tokens[i] = 0;
     __syncthreads();
+    grid_dependency_wait();
+    grid_launch_dependents();
     const double z = rt_balance_tokens<L, V, Mode, kRtSmallWarps>(
         q, lo, hi, [&](int s, int e) { atomicAdd(counts + s * q.E + e, 1); },
         [&](int s, const float (&acc)[V], int n) {
@@ -639,6 +645,8 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) router_backward_k
             dw_ahead = q.d_weights != nullptr && lane < q.K ? q.d_weights[static_cast<long long>(row) * q.K + lane] : 0.f;
         }
     };
+    grid_dependency_wait();
+    grid_launch_dependents();
     fetch(lo);
     const float g = q.d_loss_ptr != nullptr ? *q.d_loss_ptr : q.d_loss;
     float live = 1.f, all = 1.f;
@@ -774,8 +782,7 @@ int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
         RtParams b = shared_out(ctas);
         b.z_parts = ctas;
         const long long zero = (b.zero_words + 1023) / 1024;
-        balance_zero_kernel<L><<<static_cast<int>(zero < sms ? zero : sms), 256, 0, stream>>>(b);
-        MM_CUDA(cudaGetLastError());
+        MM_CUDA(launch_behind(balance_zero_kernel<L>, static_cast<int>(zero < sms ? zero : sms), 256, stream, b));
         MM_CUDA(launch_behind(balance_kernel<L, V, Mode>, b.z_parts, kRtWarps * 32, stream, b));
         const long long cells = static_cast<long long>(q.S) * q.E;
         if (cells > kRtEndCells) {
@@ -784,9 +791,9 @@ int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
             balance_end_kernel<L><<<static_cast<int>(want < kRtBalanceCtas ? want : kRtBalanceCtas), kRtWarps * 32, 0, stream>>>(b);
         }
     } else if (op == kRtRoute) {
-        route_kernel<L, V, Mode><<<blocks < sms * 8 ? blocks : sms * 8, kRtWarps * 32, 0, stream>>>(q);
+        MM_CUDA(launch_behind(route_kernel<L, V, Mode>, blocks < sms * 8 ? blocks : sms * 8, kRtWarps * 32, stream, q));
     } else {
-        router_backward_kernel<L, V, Mode><<<grid, kRtWarps * 32, 0, stream>>>(shared_out(grid * kRtWarps));
+        MM_CUDA(launch_behind(router_backward_kernel<L, V, Mode>, grid, kRtWarps * 32, stream, shared_out(grid * kRtWarps)));
     }
     MM_CUDA(cudaGetLastError());
     return MM_OK;

@@ -52,6 +52,64 @@ def test_block_around_the_layer(tokens):
     assert buf.device_status()[0] == 0 and O.rel_rmse(y2.cpu(), layer_out.cpu()) <= 3e-3      # (the layer's parity bound)
 
 
+@pytest.mark.parametrize('tokens', [1, 24])
+def test_chain_without_a_pause(tokens):
+    """Norm, layer, norm and routing of several blocks one behind the other, eager and as a graph: kernels that start before the ones ahead of them have ended find
+    what those write. The same as with a wait after every call."""
+    experts, hidden, inter, fmt, blocks = 48, 1024, 512, 'mxfp4', 4
+    g = torch.Generator(device='cuda').manual_seed(8)
+
+    def randn(*shape):
+        return torch.randn(shape, generator=g, device='cuda')
+    start, attn = randn(tokens, hidden), randn(tokens, hidden).bfloat16()
+    w = (1 + 0.1 * randn(hidden)).bfloat16()
+    router = (randn(experts, hidden) / hidden ** 0.5).bfloat16()
+    l1, l2, _ = W.make_layer_weights(experts, hidden, inter, fmt, seed=3, std=0.05)
+    buf = mm.get_symm_buffer_for_mega_moe(None, experts, 32, 8, hidden, inter, act_format=fmt)
+    ws = torch.zeros(mm.fe_workspace_bytes(buf), dtype=torch.uint8, device='cuda')
+    stream, hid, y, own = start.clone(), torch.empty_like(attn), torch.empty_like(attn), torch.empty((tokens, experts), device='cuda')
+
+    def run(wait):
+        seen = []
+        stream.copy_(start)
+        hid.copy_(attn)
+        for _ in range(blocks):
+            mm.block_norm(stream, hid, pre_weight=w, residual_out=stream, normed=hid)
+            wait()
+            mm.mega_moe_from_hidden(y, hid, router, l1, l2, buf, ws, activation_clamp=10.0, timeout_ms=500.0)
+            wait()
+            mm.block_norm(stream, y, post_weight=w, pre_weight=w, residual_out=stream, normed=hid)
+            wait()
+            torch.matmul(hid.float(), router.float().t(), out=own)
+            wait()
+            idx, weights = mm.route_tokens(own, 8, topk_idx=buf.topk_idx[:tokens], topk_weights=buf.topk_weights[:tokens])
+            wait()
+            b = mm.balance_loss(own, idx, z_coef=0.1)
+            wait()
+            d = mm.router_backward(own, idx, d_topk_weights=weights, balance=b)
+            wait()
+            mm.fp4_fp4_mega_moe(y, l1, l2, buf, activation_clamp=10.0, timeout_ms=500.0)
+            wait()
+            seen += [idx.clone(), b.counts, b.losses, d]
+        return [stream.clone(), y.clone()] + seen
+    want = run(torch.cuda.synchronize)
+    for _ in range(3):
+        got = run(lambda: None)
+        torch.cuda.synchronize()
+        assert buf.device_status()[0] == 0
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run(lambda: None)
+    for _ in range(3):
+        for t in captured:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert buf.device_status()[0] == 0
+        assert all(torch.equal(a, b) for a, b in zip(captured, want))
+
+
 class _Norm(torch.autograd.Function):
     """How a program hooks the pair into autograd."""
 
