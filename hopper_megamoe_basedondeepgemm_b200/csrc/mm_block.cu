@@ -107,6 +107,20 @@ int router_check(const mm_router_args_t* a) {
     return MM_OK;
 }
 
+Rows logit_rows(const mm_router_args_t* a, const void* p, int64_t ld) {
+    const int64_t bytes = dtype_bytes(a->dtype);
+    return Rows{p, a->tokens > 1 ? ld * bytes : 0, a->num_experts * bytes, a->tokens};      // (how far the row behind a single one would be says nothing)
+}
+// A tensor without gaps, as rows: its own only one.
+Rows packed(const void* p, int64_t bytes) { return Rows{p, 0, bytes, 1}; }
+
+// Whether the router's outputs lie apart from each other and from what is read.
+bool lie_apart(const Rows* outputs, int n_out, const Rows* inputs, int n_in) {
+    for (int i = 0; i < n_out; ++i)
+        if (!writes_safely(outputs[i], inputs, n_in, false) || !writes_safely(outputs[i], outputs + i + 1, n_out - i - 1, false)) return false;
+    return true;
+}
+
 mm::RtParams router_params(const mm_router_args_t* a) {
     mm::RtParams q;
     memset(&q, 0, sizeof(q));
@@ -241,6 +255,10 @@ int mm_route_tokens(const mm_router_args_t* a, const float* expert_bias, const u
     if ((expert_bias != nullptr && a->score_mode != 1) || !std::isfinite(a->route_scale)) return MM_ERR_INVALID_ARGUMENT;
     if (a->tokens == 0) return MM_OK;
     if (a->topk_weights == nullptr) return MM_ERR_INVALID_ARGUMENT;
+    const int64_t t = a->tokens;
+    const Rows outputs[2] = {packed(a->topk_idx, t * a->topk * 8), packed(a->topk_weights, t * a->topk * 4)};
+    const Rows inputs[3] = {logit_rows(a, a->logits, a->logits_stride), packed(expert_bias, a->num_experts * 4), packed(valid, t)};
+    if (!lie_apart(outputs, 2, inputs, 3)) return MM_ERR_INVALID_ARGUMENT;
     mm::RtParams q = router_params(a);
     q.bias = expert_bias; q.valid = valid;
     return launch_router(a->dtype, mm::kRtRoute, q, stream_ptr);
@@ -257,6 +275,11 @@ int mm_balance_loss(const mm_router_args_t* a, const mm_balance_args_t* b, void*
     if (st != MM_OK) return st;
     if (b->mean_probs == nullptr || b->losses == nullptr || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 7u) != 0u ||
         workspace_bytes < mm_balance_workspace_bytes(a->num_experts, b->num_sequences)) return MM_ERR_INVALID_ARGUMENT;
+    const int64_t s = b->num_sequences, t = a->tokens;
+    const Rows outputs[5] = {packed(b->counts, s * a->num_experts * 4), packed(b->mean_probs, s * a->num_experts * 4), packed(b->seq_tokens, s * 4), packed(b->losses, 12),
+                             packed(workspace, workspace_bytes)};
+    const Rows inputs[3] = {logit_rows(a, a->logits, a->logits_stride), packed(a->topk_idx, t * a->topk * 8), packed(b->cu_seqlens, s * 4 + 4)};
+    if (!lie_apart(outputs, 5, inputs, 3)) return MM_ERR_INVALID_ARGUMENT;
     mm::RtParams q = router_params(a);
     balance_params(b, q);
     const int64_t cells = static_cast<int64_t>(q.S) * q.E, zeroed = balance_zeroed_bytes(q.E, q.S);
@@ -278,11 +301,11 @@ int mm_router_backward(const mm_router_args_t* a, const float* d_topk_weights, c
     if ((d_topk_weights == nullptr && b == nullptr) || !std::isfinite(a->route_scale)) return MM_ERR_INVALID_ARGUMENT;
     if (a->tokens == 0) return MM_OK;
     if (d_logits == nullptr || (a->tokens > 1 && d_logits_stride < a->num_experts)) return MM_ERR_INVALID_ARGUMENT;
-    const int bytes = dtype_bytes(a->dtype);
-    const int64_t apart = a->tokens > 1 ? 1 : 0;                            // (how far a second token would be)
-    const Rows logits = {a->logits, apart * a->logits_stride * bytes, static_cast<int64_t>(a->num_experts) * bytes, a->tokens};
-    const Rows grads = {d_logits, apart * d_logits_stride * bytes, static_cast<int64_t>(a->num_experts) * bytes, a->tokens};
-    if (!writes_safely(grads, &logits, 1, true)) return MM_ERR_INVALID_ARGUMENT;
+    const int64_t slots = static_cast<int64_t>(a->tokens) * a->topk, s = b != nullptr ? b->num_sequences : 0;
+    const Rows logits = logit_rows(a, a->logits, a->logits_stride), grads = logit_rows(a, d_logits, d_logits_stride);
+    const Rows others[6] = {packed(a->topk_idx, slots * 8), packed(d_topk_weights, slots * 4), packed(d_loss_ptr, 4), packed(b != nullptr ? b->counts : nullptr, s * a->num_experts * 4),
+                            packed(b != nullptr ? b->seq_tokens : nullptr, s * 4), packed(b != nullptr ? b->cu_seqlens : nullptr, s * 4 + 4)};
+    if (!writes_safely(grads, &logits, 1, true) || !writes_safely(grads, others, 6, false)) return MM_ERR_INVALID_ARGUMENT;
     mm::RtParams q = router_params(a);
     if (b != nullptr) balance_params(b, q);
     q.balance = b != nullptr;

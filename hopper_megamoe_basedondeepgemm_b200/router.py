@@ -21,7 +21,7 @@ def route_tokens(logits: torch.Tensor, topk: int, score_mode: int = 0, expert_bi
     `[experts]`, optional), compared as in 64 bits; weights are the sigmoids over their sum. Both times `route_scale`. Experts come in descending
     order, equal ones lower index first. A logit of -inf or NaN switches an expert off for the token, a bias of -inf or NaN for all. Slots for which no expert is left,
     and tokens whose `valid` (bool or uint8 `[tokens]`) is 0, get index -1 and weight 0: the layer's masked slots. `topk_idx` / `topk_weights` may
-    be given, e.g. `sym_buffer.topk_idx[:tokens]`. At most 1024 experts and 32 routes per token.
+    be given, e.g. `sym_buffer.topk_idx[:tokens]`, apart from everything that the call reads. At most 1024 experts and 32 routes per token.
     """
     return binding.route_tokens(logits, topk, score_mode, expert_bias, valid, route_scale, topk_idx, topk_weights)
 
@@ -70,7 +70,7 @@ def router_backward(logits: torch.Tensor, topk_idx: torch.Tensor, score_mode: in
     bias that takes part in it, have no gradient. `balance` is what `balance_loss` returned for the same logits and indices. Either may be left
     out. `d_loss` is a number, or an fp32 tensor with one element on the GPU. Where the tokens of a batch lie on several ranks and it is balanced as a whole,
     `balance.counts` and `balance.tokens` may be summed over the ranks in between: the result is then the gradient of the loss over all of them.
-    `d_logits` (the logits' type and shape) may be given, and may be `logits`.
+    `d_logits` (the logits' type and shape) may be given, and may be `logits`, but nothing else that the call reads.
     """
     if balance is None:
         return binding.router_backward(logits, topk_idx, score_mode, d_topk_weights, route_scale, None, None, None, 0.0, 0.0, d_loss, d_logits)

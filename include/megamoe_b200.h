@@ -316,7 +316,8 @@ typedef struct mm_balance_args {
 
 /* The topk experts with the largest keys (logits; or sigmoid + expert_bias, compared as in 64 bits), ties to the lower expert, and their
  * weights: what mm_fe_forward and mm_frontend_launch work out from hidden states, from logits that the caller has. Tokens whose `valid` is
- * 0, and slots for which no expert is left, get -1 and weight 0. */
+ * 0, and slots for which no expert is left, get -1 and weight 0. Here and below, outputs (and the workspace) that share memory with each
+ * other or with an input are refused. */
 int mm_route_tokens(const mm_router_args_t* args, const float* expert_bias, const uint8_t* valid, void* stream);
 int64_t mm_balance_workspace_bytes(int32_t num_experts, int32_t num_sequences);
 /* balance = mean over the sequences with tokens of sum_e (E c_e / (topk n)) P_e (c counts, n seq_tokens, P mean_probs), z = mean over those

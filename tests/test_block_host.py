@@ -158,6 +158,33 @@ def test_router_refusals_of_its_other_arguments():
     assert lib.mm_router_backward(ctypes.byref(a), 9 * A, None, 1.0, None, A + 64, 48, None) == INVALID    # over part of the logits
 
 
+def test_router_outputs_lie_apart():
+    """An output that shares memory with what the call reads, or with another output, is refused (first and last byte of 4 tokens of 48 experts, 8 routes)."""
+    lib = _lib.load()
+    logits, idx, weights = 4 * 48 * 4, 4 * 8 * 8, 4 * 8 * 4
+
+    def route(bias=None, valid=None, **kw):
+        return lib.mm_route_tokens(ctypes.byref(_router(score_mode=1, **kw)), bias, valid, None)
+    for where in (A - 4, A, A + logits - 4, 2 * A - 4, 2 * A + idx - 4):
+        assert route(topk_weights=where) == INVALID
+    assert route(bias=2 * A + 8) == INVALID and route(bias=3 * A - 4) == INVALID and route(valid=3 * A + weights - 1) == INVALID and route(valid=2 * A - 3) == INVALID
+    assert route(topk_idx=A + logits - 8) == INVALID
+
+    need = lib.mm_balance_workspace_bytes(48, 2)
+
+    def balance(workspace=9 * A, **kw):
+        return lib.mm_balance_loss(ctypes.byref(_router()), ctypes.byref(_balance(**kw)), workspace, need, None)
+    cells = 2 * 48 * 4
+    for kw in (dict(counts=A), dict(mean_probs=2 * A + idx - 4), dict(seq_tokens=4 * A + 8), dict(losses=4 * A - 8), dict(counts=7 * A + cells - 4), dict(losses=6 * A + 4),
+               dict(seq_tokens=5 * A - 4), dict(losses=9 * A + 8), dict(mean_probs=9 * A - 8), dict(workspace=2 * A), dict(workspace=8 * A + 8)):
+        assert balance(**kw) == INVALID, kw
+
+    def backward(d_logits, dw=9 * A, balance=True, d_loss=11 * A):
+        return lib.mm_router_backward(ctypes.byref(_router()), dw, ctypes.byref(_balance()) if balance else None, 1.0, d_loss, d_logits, 48, None)
+    for where in (2 * A, 2 * A + idx - 4, 9 * A, 9 * A + weights - 4, 4 * A + 8, 5 * A + cells - 4, 6 * A + 4, 11 * A - logits + 4, 11 * A):
+        assert backward(where) == INVALID
+
+
 def test_functions_take_gpu_tensors():
     x, w = torch.zeros(4, 64), torch.ones(64)
     with pytest.raises(RuntimeError):
