@@ -18,7 +18,7 @@ SOURCES = {
     'mm_abi.cu': ['mm_kernel.cuh', 'mm_frontend.cuh', 'mm_frontend_route.h', 'mm_device_attribute.h', 'mm_ptx.cuh', 'mm_prep.cuh', 'mm_batch.cuh',
                   'mm_decode.cuh', 'mm_error.h', _ABI],
     'mm_block.cu': ['mm_block_norm.h', 'mm_router.h', 'mm_error.h', _ABI],
-    **{f'mm_block_norm_{t}.cu': ['mm_block_norm.cuh', 'mm_block_norm.h', 'mm_launch.h', 'mm_ptx.cuh', 'mm_error.h', _ABI] for t in ('bf16', 'fp16', 'fp32')},
+    **{f'mm_block_norm_{w}{t}.cu': ['mm_block_norm.cuh', 'mm_block_norm.h', 'mm_launch.h', 'mm_ptx.cuh', 'mm_error.h', _ABI] for w in ('', 'wide_') for t in ('bf16', 'fp16', 'fp32')},
     **{f'mm_router_{t}.cu': ['mm_router.cuh', 'mm_router.h', 'mm_launch.h', 'mm_ptx.cuh', 'mm_error.h', _ABI] for t in ('bf16', 'fp16', 'fp32')},
 }
 CHECK_SOURCES = ('mm_abi.cu',)           # those that the test build compiles anew; it shares the others' objects

@@ -189,7 +189,7 @@ int mm_block_norm(const mm_block_norm_args_t* a, void* stream_ptr) {
 
 int64_t mm_block_norm_workspace_bytes(int64_t tokens, int32_t hidden) {
     if (tokens < 0 || hidden < 1 || hidden > mm::kBnMaxHidden) return -1;
-    return mm::bn_backward_ctas(tokens, hidden) * hidden * 2 * 4;
+    return mm::bn_backward_teams(tokens, hidden) * hidden * 2 * 4;
 }
 
 int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_grads_t* g, void* stream_ptr) {
@@ -207,7 +207,7 @@ int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_gr
         if (sums > 0 && (g->workspace == nullptr || g->workspace_bytes < mm_block_norm_workspace_bytes(t, a->hidden) || (reinterpret_cast<uintptr_t>(g->workspace) & 31u) != 0u)) return MM_ERR_INVALID_ARGUMENT;
     }
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-    const int64_t ctas = mm::bn_backward_ctas(t, a->hidden);
+    const int64_t teams = mm::bn_backward_teams(t, a->hidden);
     if (t > 0) {
         const Rows none = {nullptr, 0, 0, 0};
         Rows rows[10] = {rows_of(g->d_residual, g->d_residual_stride, t, a->hidden, a->stream_dtype), rows_of(g->d_y, g->d_y_stride, t, a->hidden, a->dtype),
@@ -230,14 +230,14 @@ int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_gr
         q.d_y = g->d_y; q.d_y_ld = g->d_y_stride;
         q.d_gate = g->d_gate; q.d_gate_ld = g->d_gate_stride;
         q.partial = static_cast<float*>(g->workspace);
-        st = launch_norm(a->dtype, q, {true, a->stream_dtype == MM_DTYPE_FP32, norm_rows_aligned(a->hidden, rows, 10), 0, static_cast<int>(ctas)}, stream);
+        st = launch_norm(a->dtype, q, {true, a->stream_dtype == MM_DTYPE_FP32, norm_rows_aligned(a->hidden, rows, 10), 0, static_cast<int>(teams)}, stream);
         if (st != MM_OK) return st;
     }
     if (sums > 0) {
         mm::BnSumsParams q;
         memset(&q, 0, sizeof(q));
         q.partial = static_cast<const float*>(g->workspace);
-        q.rows = static_cast<int>(ctas); q.hidden = a->hidden;
+        q.rows = static_cast<int>(teams); q.hidden = a->hidden;
         q.gate = channel ? a->gate : nullptr; q.post_w = a->post_weight;
         q.d_pre_w = g->d_pre_weight; q.d_post_w = g->d_post_weight; q.d_gate = channel ? g->d_gate : nullptr;
         q.weight32 = a->weight_dtype == MM_DTYPE_FP32; q.gate32 = a->gate_dtype == MM_DTYPE_FP32;

@@ -17,7 +17,7 @@
 // those of the norm of r', so that a row needs one exchange between its threads. The gradients of a channel's gate and of w_post are one sum over
 // the rows, of dr n1 (token's or element's gate), times the other's factor.
 //
-// A row belongs to one CTA, eight channels to a thread, up to 4096 channels. Bound by memory: the bytes of the rows, in and out. CTAs stay and walk over the rows; a
+// A row belongs to one CTA, or from 4096 channels on to two (a cluster), eight channels to a thread. Bound by memory: the bytes of the rows, in and out. CTAs stay and walk over the rows; a
 // thread asks for its part of the next row before it works on the one it has, and while a row's sums are exchanged, the sum of squares of the next row's
 // y goes with them: one barrier a row.
 #pragma once
@@ -45,46 +45,29 @@ template <> __device__ __forceinline__ float bn_round<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 bn_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half bn_round<__half>(float v) { return __float2half_rn(v); }
 
-// Eight elements of a row, a CTA's width apart, so that neighbouring threads read neighbouring elements wherever the row starts.
-__device__ __forceinline__ int bn_at(int c, int j) { return (c * 8 + j) * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x); }
+// How a row lies over the threads. kBnWhole: every row starts on 16 bytes (32-bit elements: 32) and is made of groups of eight channels, of which a thread has one, in one
+// access. Otherwise a thread's eight channels lie the threads' number apart, so that neighbouring threads read neighbouring elements wherever the row starts.
+// kBnTwo: the row belongs to a cluster of two CTAs (more than 4096 channels).
+enum BnLayout { kBnWhole = 1, kBnTwo = 2 };
+template <int Lay>
+__device__ __forceinline__ int bn_thread() { return static_cast<int>((Lay & kBnTwo) != 0 ? (blockIdx.x & 1u) * blockDim.x + threadIdx.x : threadIdx.x); }
+template <int Lay>
+__device__ __forceinline__ int bn_width() { return static_cast<int>((Lay & kBnTwo) != 0 ? 2u * blockDim.x : blockDim.x); }
 
-template <typename T>
-__device__ __forceinline__ void bn_load(const T* row, int hidden, int c, float (&v)[8]) {
-    #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int at = bn_at(c, j);
-        v[j] = at < hidden ? bn_float<T>(row[at]) : 0.f;
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void bn_store(T* row, int hidden, int c, const float (&v)[8]) {
-    #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int at = bn_at(c, j);
-        if (at < hidden) row[at] = bn_round<T>(v[j]);
-    }
-}
-
-// a weight or gate row that is 32 bits wide or of the activations' type
-template <typename X>
-__device__ __forceinline__ void bn_load_either(const void* row, int is32, long long at_row, int hidden, int c, float (&v)[8]) {
-    if (is32) bn_load<float>(static_cast<const float*>(row) + at_row, hidden, c, v);
-    else bn_load<X>(static_cast<const X*>(row) + at_row, hidden, c, v);
-}
-
-template <typename X>
-__device__ __forceinline__ float bn_token_gate(const BnParams& q, long long row) {
-    return q.gate32 ? static_cast<const float*>(q.gate)[row * q.gate_ld] : bn_float<X>(static_cast<const X*>(q.gate)[row * q.gate_ld]);
-}
-
-// Sums of N values (a power of two) over the CTA, the same in every thread. In a warp the values are dealt out while they are added: each step
+// Sums of N values (a power of two) over the row's threads, the same in every thread. In a warp the values are dealt out while they are added: each step
 // halves both the values of a lane and the lanes of a value. Each warp's sums go through shared memory (`part`, all zero at first, of which a turn
-// is used at a time: the next sums' values go where no thread can still be reading, so one barrier does), and four lanes add up one value.
+// is used at a time: the next sums' values go where no thread can still be reading, so one barrier does), and four lanes add up one value. Two CTAs leave
+// their warps' sums in the shared memory of both, each in its half, so both add the same numbers in the same order; no CTA writes to the other behind the last barrier.
 constexpr int kBnSumWarps = kBnMaxThreads / 32;
-template <int N, int Room>
-__device__ __forceinline__ void bn_sum(float (&v)[N], float (*part)[Room][kBnSumWarps], int& turn) {
+template <int Room, int Lay> using BnSums = float[2][Room][kBnSumWarps * ((Lay & kBnTwo) != 0 ? 2 : 1)];
+template <int Lay>
+__device__ __forceinline__ void bn_barrier() {
+    if constexpr ((Lay & kBnTwo) != 0) { cluster_arrive(); cluster_wait(); } else { __syncthreads(); }
+}
+template <int N, int Lay, int Room>
+__device__ __forceinline__ void bn_sum(float (&v)[N], BnSums<Room, Lay>& part, int& turn) {
     static_assert(N <= Room && N <= 16);
+    constexpr bool kTwo = (Lay & kBnTwo) != 0;
     const uint32_t lane = threadIdx.x & 31u;
     float s[N];
     #pragma unroll
@@ -102,15 +85,29 @@ __device__ __forceinline__ void bn_sum(float (&v)[N], float (*part)[Room][kBnSum
     #pragma unroll
     for (; o > 0; o /= 2) s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
     const uint32_t mine = lane * N / 32;                     // the value that this lane has the warp's sum of
-    if (blockDim.x > 32) {
-        float (*p)[kBnSumWarps] = part[turn];
+    if (kTwo || blockDim.x > 32) {
+        auto& p = part[turn];
         turn ^= 1;
-        if (lane % (32 / N) == 0) p[mine][threadIdx.x >> 5] = s[0];
-        __syncthreads();
+        if (lane % (32 / N) == 0) {
+            if constexpr (kTwo) {
+                const uint32_t rank = blockIdx.x & 1u;
+                float* at = &p[mine][rank * kBnSumWarps + (threadIdx.x >> 5)];
+                *at = s[0];
+                st_cluster_f32(at, rank ^ 1u, s[0]);
+            } else {
+                p[mine][threadIdx.x >> 5] = s[0];
+            }
+        }
+        bn_barrier<Lay>();
         #pragma unroll
         for (int first = 0; first < N; first += 8) {         // eight values at a time
-            const float4 w = *reinterpret_cast<const float4*>(&p[first + (lane >> 2) % (N < 8 ? N : 8)][(lane & 3u) * 4u]);
+            const float* of = &p[first + (lane >> 2) % (N < 8 ? N : 8)][(lane & 3u) * 4u];
+            const float4 w = *reinterpret_cast<const float4*>(of);
             float t = (w.x + w.y) + (w.z + w.w);
+            if constexpr (kTwo) {
+                const float4 x = *reinterpret_cast<const float4*>(of + kBnSumWarps);
+                t += (x.x + x.y) + (x.z + x.w);
+            }
             t += __shfl_xor_sync(0xffffffffu, t, 1);
             t += __shfl_xor_sync(0xffffffffu, t, 2);
             #pragma unroll
@@ -123,212 +120,15 @@ __device__ __forceinline__ void bn_sum(float (&v)[N], float (*part)[Room][kBnSum
 }
 static_assert(kBnSumWarps == 16, "four lanes read four warps' sums each");
 
-template <int Room>
-__device__ __forceinline__ void bn_sum_init(float (*part)[Room][kBnSumWarps]) {
-    if (blockDim.x > 32) {
-        for (int i = threadIdx.x; i < 2 * Room * kBnSumWarps; i += blockDim.x) (&part[0][0][0])[i] = 0.f;
-        __syncthreads();
+template <int Lay, int Room>
+__device__ __forceinline__ void bn_sum_init(BnSums<Room, Lay>& part) {
+    if ((Lay & kBnTwo) != 0 || blockDim.x > 32) {
+        for (int i = threadIdx.x; i < static_cast<int>(sizeof(part) / 4); i += blockDim.x) (&part[0][0][0])[i] = 0.f;
+        bn_barrier<Lay>();
     }
 }
 
-// ----------------------------------------------------------------------------- rows of more than 4096 channels
-// Sixteen channels a thread, one by one, a row at a time: as it comes, without anything in flight ahead (half the memory's rate; the layer's rows end at 4096).
-// gate of a chunk
-template <typename X>
-__device__ __forceinline__ void bn_gate(const BnParams& q, long long row, int c, float (&g)[8]) {
-    if (q.gate_mode == kBnGateNone || q.gate_mode == kBnGateToken) {
-        const float s = q.gate_mode == kBnGateToken ? bn_token_gate<X>(q, row) : 1.f;
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = s;
-    } else {
-        bn_load_either<X>(q.gate, q.gate32, q.gate_mode == kBnGateElement ? row * q.gate_ld : 0, q.hidden, c, g);
-    }
-}
-
-template <typename X, typename R>
-__global__ void __launch_bounds__(kBnMaxThreads) block_norm_wide_kernel(const BnParams q) {
-    __shared__ __align__(16) float part[2][2][kBnSumWarps];
-    constexpr int C = 2;
-    bn_sum_init(part);
-    int turn = 0;
-    const float inv_h = 1.f / static_cast<float>(q.hidden);
-    for (long long row = blockIdx.x; row < q.tokens; row += gridDim.x) {
-        float r[C][8], u[C][8];
-        #pragma unroll
-        for (int c = 0; c < C; ++c) bn_load<R>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, c, r[c]);
-        if (q.y != nullptr) {
-            float sum[1] = {0.f};
-            #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                bn_load<X>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, c, u[c]);
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) sum[0] += u[c][j] * u[c][j];
-            }
-            float i1 = 1.f;
-            if (q.post_w != nullptr) {
-                bn_sum<1>(sum, part, turn);
-                i1 = rsqrtf(sum[0] * inv_h + q.eps);
-            }
-            #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                float g[8], w[8];
-                bn_gate<X>(q, row, c, g);
-                if (q.post_w != nullptr) {
-                    bn_load_either<X>(q.post_w, q.weight32, 0, q.hidden, c, w);
-                    #pragma unroll
-                    for (int j = 0; j < 8; ++j) u[c][j] = u[c][j] * i1 * (w[j] + q.offset);
-                }
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) r[c][j] += q.scale * (u[c][j] * g[j]);
-                bn_store<R>(static_cast<R*>(q.residual_out) + row * q.residual_out_ld, q.hidden, c, r[c]);
-            }
-        }
-        if (q.pre_w != nullptr) {
-            float sum[1] = {0.f};
-            #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) sum[0] += r[c][j] * r[c][j];
-            }
-            bn_sum<1>(sum, part, turn);
-            const float i2 = rsqrtf(sum[0] * inv_h + q.eps);
-            #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                float w[8];
-                bn_load_either<X>(q.pre_w, q.weight32, 0, q.hidden, c, w);
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) r[c][j] = r[c][j] * i2 * (w[j] + q.offset);
-                bn_store<X>(static_cast<X*>(q.normed) + row * q.normed_ld, q.hidden, c, r[c]);
-            }
-        }
-    }
-}
-
-// Rows are dealt to the CTAs in turn; a thread sums over the CTA's rows what the gradients of its channels' weights are made of and leaves it in
-// `partial`, which `block_norm_sums_kernel` adds up: always in the same order.
-template <typename X, typename R>
-__global__ void __launch_bounds__(kBnMaxThreads) block_norm_backward_wide_kernel(const BnParams q) {
-    __shared__ __align__(16) float part[2][2][kBnSumWarps];
-    constexpr int C = 2;
-    bn_sum_init(part);
-    int turn = 0;
-    const float inv_h = 1.f / static_cast<float>(q.hidden);
-    const bool post = q.post_w != nullptr, pre = q.pre_w != nullptr;
-    float acc_pre[C][8] = {}, acc_y[C][8] = {};
-    for (long long row = blockIdx.x; row < q.tokens; row += gridDim.x) {
-        float y[C][8], i1 = 1.f;
-        if (q.y != nullptr) {
-            float sum[1] = {0.f};
-            #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                bn_load<X>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, c, y[c]);
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) sum[0] += y[c][j] * y[c][j];
-            }
-            if (post) {
-                bn_sum<1>(sum, part, turn);
-                i1 = rsqrtf(sum[0] * inv_h + q.eps);
-            }
-        }
-        float d[C][8];                                       // d_r', then dr
-        #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (q.d_residual_out != nullptr) {
-                bn_load<R>(static_cast<const R*>(q.d_residual_out) + row * q.d_residual_out_ld, q.hidden, c, d[c]);
-            } else {
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) d[c][j] = 0.f;
-            }
-        }
-        if (pre) {
-            float n[C][8], dh[C][8], sum[2] = {0.f, 0.f};
-            #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                bn_load<R>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, c, n[c]);
-                bn_load<X>(static_cast<const X*>(q.d_normed) + row * q.d_normed_ld, q.hidden, c, dh[c]);
-                float w[8];
-                if (q.y != nullptr) {
-                    float g[8];
-                    bn_gate<X>(q, row, c, g);
-                    if (post) {
-                        bn_load_either<X>(q.post_w, q.weight32, 0, q.hidden, c, w);
-                        #pragma unroll
-                        for (int j = 0; j < 8; ++j) n[c][j] += q.scale * (y[c][j] * i1 * (w[j] + q.offset) * g[j]);
-                    } else {
-                        #pragma unroll
-                        for (int j = 0; j < 8; ++j) n[c][j] += q.scale * (y[c][j] * g[j]);
-                    }
-                }
-                bn_load_either<X>(q.pre_w, q.weight32, 0, q.hidden, c, w);
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    sum[0] += n[c][j] * n[c][j];
-                    sum[1] += dh[c][j] * (w[j] + q.offset) * n[c][j];
-                }
-            }
-            bn_sum<2>(sum, part, turn);
-            const float i2 = rsqrtf(sum[0] * inv_h + q.eps), mean = sum[1] * i2 * inv_h;
-            #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                float w[8];
-                bn_load_either<X>(q.pre_w, q.weight32, 0, q.hidden, c, w);
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float n2 = n[c][j] * i2;
-                    acc_pre[c][j] += dh[c][j] * n2;
-                    d[c][j] += i2 * (dh[c][j] * (w[j] + q.offset) - n2 * mean);
-                }
-            }
-        }
-        #pragma unroll
-        for (int c = 0; c < C; ++c) bn_store<R>(static_cast<R*>(q.d_residual) + row * q.d_residual_ld, q.hidden, c, d[c]);
-        if (q.y == nullptr) continue;
-        float sum[2] = {0.f, 0.f};
-        #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float g[8], w[8], dg[8];
-            bn_gate<X>(q, row, c, g);
-            if (post) bn_load_either<X>(q.post_w, q.weight32, 0, q.hidden, c, w);
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float n1 = y[c][j] * i1, w1 = post ? w[j] + q.offset : 1.f, dv = q.scale * d[c][j];
-                acc_y[c][j] += d[c][j] * n1 * (q.gate_mode == kBnGateChannel ? 1.f : g[j]);
-                dg[j] = dv * (n1 * w1);
-                d[c][j] = dv * g[j] * w1;
-                sum[0] += d[c][j] * n1;
-                sum[1] += dg[j];
-            }
-            if (q.gate_mode == kBnGateElement) {
-                if (q.gate32) bn_store<float>(static_cast<float*>(q.d_gate) + row * q.d_gate_ld, q.hidden, c, dg);
-                else bn_store<X>(static_cast<X*>(q.d_gate) + row * q.d_gate_ld, q.hidden, c, dg);
-            }
-        }
-        if (post || q.gate_mode == kBnGateToken) bn_sum<2>(sum, part, turn);
-        if (q.gate_mode == kBnGateToken && threadIdx.x == 0) {
-            if (q.gate32) static_cast<float*>(q.d_gate)[row * q.d_gate_ld] = sum[1];
-            else static_cast<X*>(q.d_gate)[row * q.d_gate_ld] = bn_round<X>(sum[1]);
-        }
-        const float mean = sum[0] * inv_h;
-        #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (post) {
-                #pragma unroll
-                for (int j = 0; j < 8; ++j) d[c][j] = i1 * (d[c][j] - y[c][j] * i1 * mean);
-            }
-            bn_store<X>(static_cast<X*>(q.d_y) + row * q.d_y_ld, q.hidden, c, d[c]);
-        }
-    }
-    float* p = q.partial + static_cast<long long>(blockIdx.x) * q.hidden;
-    const long long stride = static_cast<long long>(gridDim.x) * q.hidden;
-    const bool sum_y = post || q.gate_mode == kBnGateChannel;
-    #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        if (pre) bn_store<float>(p, q.hidden, c, acc_pre[c]);
-        if (sum_y) bn_store<float>(pre ? p + stride : p, q.hidden, c, acc_y[c]);
-    }
-}
-
-// ----------------------------------------------------------------------------- rows of up to 4096 channels
+// ----------------------------------------------------------------------------- channels of a thread
 // Two 32-bit numbers in one register pair: one instruction adds or multiplies both.
 __device__ __forceinline__ unsigned long long bn_bits(float2 v) { return *reinterpret_cast<unsigned long long*>(&v); }
 __device__ __forceinline__ float2 bn_pair(unsigned long long b) { return *reinterpret_cast<float2*>(&b); }
@@ -379,30 +179,29 @@ __device__ __forceinline__ Bn8<__half> bn_pack(const float2 (&v)[4], __half) {
 }
 
 // Eight elements on their way: as they will lie in memory, or one to a register, because putting two of them together waits for both.
-template <typename T, bool Vec> struct BnAhead { uint32_t w[Vec || sizeof(T) == 4 ? sizeof(T) * 2 : 8]; };
-template <typename T, bool Vec>
-__device__ __forceinline__ Bn8<T> bn_take(const BnAhead<T, Vec>& a) {
+template <typename T, int Lay> struct BnAhead { uint32_t w[(Lay & kBnWhole) != 0 || sizeof(T) == 4 ? sizeof(T) * 2 : 8]; };
+template <typename T, int Lay>
+__device__ __forceinline__ Bn8<T> bn_take(const BnAhead<T, Lay>& a) {
     Bn8<T> r;
     #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) * 2; ++i) r.w[i] = Vec || sizeof(T) == 4 ? a.w[i] : (a.w[(2 * i) & 7] | a.w[(2 * i + 1) & 7] << 16);
+    for (int i = 0; i < static_cast<int>(sizeof(T)) * 2; ++i) r.w[i] = (Lay & kBnWhole) != 0 || sizeof(T) == 4 ? a.w[i] : (a.w[(2 * i) & 7] | a.w[(2 * i + 1) & 7] << 16);
     return r;
 }
 
-// The eight channels of this thread in a row. `Vec`: eight neighbours, in one access (of 32 bytes for 32-bit elements: two of 16 would each move half of
-// every 32-byte sector). Otherwise channels a CTA's width apart, one by one: neighbouring threads still read neighbours.
-template <typename T, bool Vec>
-__device__ __forceinline__ void bn_fetch(const T* row, int hidden, BnAhead<T, Vec>& r) {
-    if constexpr (Vec) {
-        const T* p = row + static_cast<int>(threadIdx.x) * 8;
+// The eight channels of this thread in a row: in one access (of 32 bytes for 32-bit elements: two of 16 would each move half of every 32-byte sector), or one by one.
+template <typename T, int Lay>
+__device__ __forceinline__ void bn_fetch(const T* row, int hidden, BnAhead<T, Lay>& r) {
+    if constexpr ((Lay & kBnWhole) != 0) {
+        const T* p = row + bn_thread<Lay>() * 8;
         if constexpr (sizeof(T) == 4)
             asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]),
                          "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7]) : "l"(p) : "memory");
         else
             asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "l"(p) : "memory");
     } else {
-        int at = static_cast<int>(threadIdx.x);
+        int at = bn_thread<Lay>();
         #pragma unroll
-        for (int i = 0; i < 8; ++i, at += static_cast<int>(blockDim.x)) {
+        for (int i = 0; i < 8; ++i, at += bn_width<Lay>()) {
             if constexpr (sizeof(T) == 4)
                 asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %2, %3;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "=&r"(r.w[i]) : "l"(row + at), "r"(at), "r"(hidden) : "memory");
             else
@@ -410,18 +209,18 @@ __device__ __forceinline__ void bn_fetch(const T* row, int hidden, BnAhead<T, Ve
         }
     }
 }
-template <typename T, bool Vec>
+template <typename T, int Lay>
 __device__ __forceinline__ void bn_put(T* row, int hidden, const float2 (&v)[4]) {
     const Bn8<T> r = bn_pack(v, T());
-    if constexpr (Vec) {
-        T* p = row + static_cast<int>(threadIdx.x) * 8;
+    if constexpr ((Lay & kBnWhole) != 0) {
+        T* p = row + bn_thread<Lay>() * 8;
         if constexpr (sizeof(T) == 4)
             asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]),
                          "r"(r.w[7]) : "memory");
         else
             asm volatile("st.global.v4.b32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]) : "memory");
     } else {
-        const int at = static_cast<int>(threadIdx.x), width = static_cast<int>(blockDim.x);
+        const int at = bn_thread<Lay>(), width = bn_width<Lay>();
         #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int a = at + 2 * i * width, b = a + width;
@@ -437,32 +236,32 @@ __device__ __forceinline__ void bn_put(T* row, int hidden, const float2 (&v)[4])
 }
 
 // weights and gates of the channels
-template <typename X, bool Vec>
+template <typename X, int Lay>
 __device__ __forceinline__ void bn_weight(const void* w, int is32, int hidden, float2 (&v)[4]) {
-    if (is32) { BnAhead<float, Vec> r; bn_fetch<float, Vec>(static_cast<const float*>(w), hidden, r); bn_unpack(bn_take(r), v); }
-    else { BnAhead<X, Vec> r; bn_fetch<X, Vec>(static_cast<const X*>(w), hidden, r); bn_unpack(bn_take(r), v); }
+    if (is32) { BnAhead<float, Lay> r; bn_fetch<float, Lay>(static_cast<const float*>(w), hidden, r); bn_unpack(bn_take(r), v); }
+    else { BnAhead<X, Lay> r; bn_fetch<X, Lay>(static_cast<const X*>(w), hidden, r); bn_unpack(bn_take(r), v); }
 }
 // scale * (channel's gate) * (offset + w_post): the factor of y
-template <typename X, bool Vec>
+template <typename X, int Lay>
 __device__ __forceinline__ void bn_y_factor(const BnParams& q, float2 (&a)[4]) {
     #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = both(q.scale);
     if (q.post_w != nullptr) {
         float2 w[4];
-        bn_weight<X, Vec>(q.post_w, q.weight32, q.hidden, w);
+        bn_weight<X, Lay>(q.post_w, q.weight32, q.hidden, w);
         #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = make_float2(q.scale * (w[i].x + q.offset), q.scale * (w[i].y + q.offset));
     }
     if (q.gate_mode == kBnGateChannel) {
         float2 g[4];
-        bn_weight<X, Vec>(q.gate, q.gate32, q.hidden, g);
+        bn_weight<X, Lay>(q.gate, q.gate32, q.hidden, g);
         #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = mul2(a[i], g[i]);
     }
 }
-template <typename X, bool Vec>
+template <typename X, int Lay>
 __device__ __forceinline__ void bn_pre_factor(const BnParams& q, float2 (&w)[4]) {
-    bn_weight<X, Vec>(q.pre_w, q.weight32, q.hidden, w);
+    bn_weight<X, Lay>(q.pre_w, q.weight32, q.hidden, w);
     #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = make_float2(w[i].x + q.offset, w[i].y + q.offset);
 }
@@ -488,27 +287,27 @@ __device__ __forceinline__ float bn_gate_value(const BnParams& q, uint32_t bits)
     return q.gate32 ? __uint_as_float(bits) : narrow;
 }
 // an element's gate: of the activations' type or 32 bits, held in room for the latter
-template <typename X, bool Vec>
+template <typename X, int Lay>
 __device__ __forceinline__ void bn_fetch_gate(const BnParams& q, long long row, uint32_t (&r)[8]) {
     if (sizeof(X) == 4 || q.gate32) {
-        BnAhead<float, Vec> f;
-        bn_fetch<float, Vec>(static_cast<const float*>(q.gate) + row * q.gate_ld, q.hidden, f);
+        BnAhead<float, Lay> f;
+        bn_fetch<float, Lay>(static_cast<const float*>(q.gate) + row * q.gate_ld, q.hidden, f);
         #pragma unroll
         for (int i = 0; i < 8; ++i) r[i] = f.w[i];
     } else {
-        BnAhead<X, Vec> h;
-        bn_fetch<X, Vec>(static_cast<const X*>(q.gate) + row * q.gate_ld, q.hidden, h);
+        BnAhead<X, Lay> h;
+        bn_fetch<X, Lay>(static_cast<const X*>(q.gate) + row * q.gate_ld, q.hidden, h);
         #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(h.w) / 4); ++i) r[i] = h.w[i];
     }
 }
-template <typename X, bool Vec>
+template <typename X, int Lay>
 __device__ __forceinline__ void bn_unpack_gate(const BnParams& q, const uint32_t (&r)[8], float2 (&g)[4]) {
     if (sizeof(X) == 4 || q.gate32) {
         #pragma unroll
         for (int i = 0; i < 4; ++i) g[i] = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
     } else {
-        BnAhead<X, Vec> h;
+        BnAhead<X, Lay> h;
         #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(h.w) / 4); ++i) h.w[i] = r[i];
         bn_unpack(bn_take(h), g);
@@ -534,15 +333,18 @@ enum BnKind { kBnPlain = 0 /* no gate, or one that is part of y's factor */, kBn
 // 64 registers a thread, so two CTAs of 512 threads an SM; 16-bit streams 56, so three of 384. 16384 x 4096, 32-bit stream, both norms, channel gate: 127 us (6.3 TB/s); 8192 x
 // 3072 in bf16 37 us (5.4). (One CTA of twice the registers an SM 168 us; sixteen channels a thread 134; rows copied ahead into shared memory by cp.async
 // 160. y one row ahead, bf16 40 us; two rows ahead with a 32-bit stream, which then has no register left, 137.)
-template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec>
-__global__ void __maxnreg__((sizeof(R) == 2 && Vec && Kind != kBnElement ? 56 : 64)) block_norm_kernel(const BnParams q) {
-    __shared__ __align__(16) float part[2][2][kBnSumWarps];
+// Rows over two CTAs wait for the cluster's barrier: 8192 x 8192 bf16 120 us (4.5 TB/s), 32-bit stream 161 (5.0), 4096 x 6144 bf16 48 (64 registers, so two CTAs an SM, 55; one
+// CTA with sixteen channels a thread and nothing in flight ahead 178). Clusters of four are slower: 173, 232 and 76.
+template <typename X, typename R, bool Post, bool Pre, int Kind, int Lay>
+__global__ void __maxnreg__((sizeof(R) == 2 && (Lay & kBnWhole) != 0 && Kind != kBnElement ? 56 : 64)) block_norm_kernel(const BnParams q) {
+    constexpr bool kWhole = (Lay & kBnWhole) != 0, kTwo = (Lay & kBnTwo) != 0;
+    __shared__ __align__(16) BnSums<2, Lay> part;
     const float inv_h = 1.f / static_cast<float>(q.hidden);
-    constexpr bool kFar = Post && Vec && sizeof(R) == 2;      // y two rows ahead: its squares are summed a row before its turn
-    const int step = gridDim.x, tokens = static_cast<int>(q.tokens);
-    const bool on = !Vec || static_cast<int>(threadIdx.x) * 8 < q.hidden;
-    BnAhead<R, Vec> rr;
-    BnAhead<X, Vec> ry, ry_far;
+    constexpr bool kFar = Post && kWhole && sizeof(R) == 2;      // y two rows ahead: its squares are summed a row before its turn
+    const int step = kTwo ? gridDim.x >> 1 : gridDim.x, tokens = static_cast<int>(q.tokens);
+    const bool on = !kWhole || bn_thread<Lay>() * 8 < q.hidden;
+    BnAhead<R, Lay> rr;
+    BnAhead<X, Lay> ry, ry_far;
     uint32_t rg[8];
     float2 a[4], w[4];
     uint32_t gate_bits = 0u;
@@ -557,28 +359,28 @@ __global__ void __maxnreg__((sizeof(R) == 2 && Vec && Kind != kBnElement ? 56 : 
     auto fetch = [&](long long row) {
         if (on) {
             if (kFar) {
-                if (row + step < tokens) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + (row + step) * q.y_ld, q.hidden, ry_far);
+                if (row + step < tokens) bn_fetch<X, Lay>(static_cast<const X*>(q.y) + (row + step) * q.y_ld, q.hidden, ry_far);
             } else if (Kind != kBnStream) {
-                bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry);
+                bn_fetch<X, Lay>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry);
             }
-            bn_fetch<R, Vec>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, rr);
-            if (Kind == kBnElement) bn_fetch_gate<X, Vec>(q, row, rg);
+            bn_fetch<R, Lay>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, rr);
+            if (Kind == kBnElement) bn_fetch_gate<X, Lay>(q, row, rg);
         }
         if (Kind == kBnToken) gate_bits = bn_gate_bits<X>(q, row);
     };
-    int row = blockIdx.x;
-    if (kFar && on) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry);
+    int row = kTwo ? blockIdx.x >> 1 : blockIdx.x;
+    if (kFar && on) bn_fetch<X, Lay>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry);
     fetch(row);
     if (on) {
-        if (Kind != kBnStream) bn_y_factor<X, Vec>(q, a);
-        if (Pre) bn_pre_factor<X, Vec>(q, w);
+        if (Kind != kBnStream) bn_y_factor<X, Lay>(q, a);
+        if (Pre) bn_pre_factor<X, Lay>(q, w);
     }
-    bn_sum_init(part);
+    bn_sum_init<Lay, 2>(part);
     int turn = 0;
     float i1 = 1.f;
     if (Post) {
         float sum[1] = {bn_square(bn_take(ry))};
-        bn_sum<1>(sum, part, turn);
+        bn_sum<1, Lay, 2>(sum, part, turn);
         i1 = rsqrtf(sum[0] * inv_h + q.eps);
     }
     while (true) {
@@ -586,7 +388,7 @@ __global__ void __maxnreg__((sizeof(R) == 2 && Vec && Kind != kBnElement ? 56 : 
         float2 r[4], v[4], g[4];
         bn_unpack(bn_take(rr), r);
         if (Kind != kBnStream) bn_unpack(bn_take(ry), v);
-        if (Kind == kBnElement) bn_unpack_gate<X, Vec>(q, rg, g);
+        if (Kind == kBnElement) bn_unpack_gate<X, Lay>(q, rg, g);
         const float f = Kind == kBnToken ? i1 * bn_gate_value<X>(q, gate_bits) : i1;
         if (kFar) ry = ry_far;
         if (more) fetch(row + step);
@@ -597,27 +399,27 @@ __global__ void __maxnreg__((sizeof(R) == 2 && Vec && Kind != kBnElement ? 56 : 
                 if (Kind == kBnElement) v[i] = mul2(v[i], g[i]);
                 r[i] = fma2(v[i], a[i], r[i]);
             }
-            if (on) bn_put<R, Vec>(static_cast<R*>(q.residual_out) + row * q.residual_out_ld, q.hidden, r);
+            if (on) bn_put<R, Lay>(static_cast<R*>(q.residual_out) + row * q.residual_out_ld, q.hidden, r);
         }
         if (Pre) {
             // the sum of the next row's squares goes with this row's
             float sum[2] = {bn_square(r), 0.f};
             if (Post) {
                 sum[1] = bn_square(bn_take(ry));
-                bn_sum<2>(sum, part, turn);
+                bn_sum<2, Lay, 2>(sum, part, turn);
                 i1 = rsqrtf(sum[1] * inv_h + q.eps);
             } else {
                 float only[1] = {sum[0]};
-                bn_sum<1>(only, part, turn);
+                bn_sum<1, Lay, 2>(only, part, turn);
                 sum[0] = only[0];
             }
             const float2 i2 = both(rsqrtf(sum[0] * inv_h + q.eps));
             #pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = mul2(mul2(r[i], i2), w[i]);
-            if (on) bn_put<X, Vec>(static_cast<X*>(q.normed) + row * q.normed_ld, q.hidden, r);
+            if (on) bn_put<X, Lay>(static_cast<X*>(q.normed) + row * q.normed_ld, q.hidden, r);
         } else if (Post) {
             float sum[1] = {bn_square(bn_take(ry))};
-            bn_sum<1>(sum, part, turn);
+            bn_sum<1, Lay, 2>(sum, part, turn);
             i1 = rsqrtf(sum[0] * inv_h + q.eps);
         }
         if (!more) return;
@@ -629,20 +431,23 @@ __global__ void __maxnreg__((sizeof(R) == 2 && Vec && Kind != kBnElement ? 56 : 
 // `block_norm_sums_kernel` adds up: always in the same order. Some 400 instructions a warp and row, so the issue slots are half full; what is left is the wait for a row's
 // exchange, and registers bound what can go on meanwhile: 128 a thread, a row being worked on and a row on its way, y two rows ahead (its sum of squares goes
 // with the exchange of the row before). 8192 x 4096, 32-bit stream, both norms: 97 us (6.2 TB/s); y one row ahead 131.
-// Where a CTA of 128 registers a thread leaves an SM's registers half used and no second one fits (more than 256 threads, up to 384: hidden 2056 to 3072), it takes two rows
+// Where a CTA of 128 registers a thread leaves an SM's registers half used and no second one fits (more than 256 threads, up to 384: hidden 2056 to 3072, and 4104 to 6144 over two CTAs), it takes two rows
 // at a time through one exchange, with 168: 8192 x 3072 in bf16 59 us instead of 67, only the stream's norm 53 instead of 64, 32-bit stream 74 instead of 81. (With 256 threads
 // two CTAs of one row win, 42 us against 46 for 8192 x 2048; with an element's gate, or 32-bit
 // activations, two rows do not fit the registers.)
-template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec, int Rows>
+// Rows over two CTAs: 8192 x 8192 bf16 254 us (3.2 TB/s), 32-bit stream 276 (4.4), 4096 x 6144 bf16, two rows at a time, 85 (one at a time 111; clusters of four 172).
+template <typename X, typename R, bool Post, bool Pre, int Kind, int Lay, int Rows>
 __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1) block_norm_backward_kernel(const BnParams q) {
     constexpr bool kY = Kind != kBnStream, kSumV = Post || Kind == kBnToken;
     constexpr int kSums = (kSumV ? 8 : 2) * Rows;
-    __shared__ __align__(16) float part[2][kSums][kBnSumWarps];
+    constexpr bool kWhole = (Lay & kBnWhole) != 0, kTwo = (Lay & kBnTwo) != 0;
+    __shared__ __align__(16) BnSums<kSums, Lay> part;
+    const int team = kTwo ? blockIdx.x >> 1 : blockIdx.x, teams = kTwo ? gridDim.x >> 1 : gridDim.x;
     const float inv_h = 1.f / static_cast<float>(q.hidden);
-    const int step = gridDim.x * Rows, tokens = static_cast<int>(q.tokens);
-    const bool on = !Vec || static_cast<int>(threadIdx.x) * 8 < q.hidden, sum_y = Post || q.gate_mode == kBnGateChannel, has_d = q.d_residual_out != nullptr;
-    BnAhead<R, Vec> rd[Rows], rr[Rows];                      // on their way
-    BnAhead<X, Vec> ry_ahead[Rows], rh[Rows];
+    const int step = teams * Rows, tokens = static_cast<int>(q.tokens);
+    const bool on = !kWhole || bn_thread<Lay>() * 8 < q.hidden, sum_y = Post || q.gate_mode == kBnGateChannel, has_d = q.d_residual_out != nullptr;
+    BnAhead<R, Lay> rd[Rows], rr[Rows];                      // on their way
+    BnAhead<X, Lay> ry_ahead[Rows], rh[Rows];
     Bn8<X> ry[Rows];                                         // norm of y: the next rows'
     uint32_t rg[Rows][8], gate_bits[Rows];
     float2 a[4], w[4], acc_pre[4], acc_y[4];
@@ -662,7 +467,7 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
         #pragma unroll
         for (int n = 0; n < Rows; ++n) {
             const long long row = first + n;
-            if (kY && on && row < tokens) bn_fetch<X, Vec>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry_ahead[n]);
+            if (kY && on && row < tokens) bn_fetch<X, Lay>(static_cast<const X*>(q.y) + row * q.y_ld, q.hidden, ry_ahead[n]);
             else bn_clear(ry_ahead[n].w);
         }
     };
@@ -679,16 +484,16 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
             }
             if (on) {
                 if (Pre) {
-                    bn_fetch<R, Vec>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, rr[n]);
-                    bn_fetch<X, Vec>(static_cast<const X*>(q.d_normed) + row * q.d_normed_ld, q.hidden, rh[n]);
+                    bn_fetch<R, Lay>(static_cast<const R*>(q.residual) + row * q.residual_ld, q.hidden, rr[n]);
+                    bn_fetch<X, Lay>(static_cast<const X*>(q.d_normed) + row * q.d_normed_ld, q.hidden, rh[n]);
                 }
-                if (has_d) bn_fetch<R, Vec>(static_cast<const R*>(q.d_residual_out) + row * q.d_residual_out_ld, q.hidden, rd[n]);
-                if (Kind == kBnElement) bn_fetch_gate<X, Vec>(q, row, rg[n]);
+                if (has_d) bn_fetch<R, Lay>(static_cast<const R*>(q.d_residual_out) + row * q.d_residual_out_ld, q.hidden, rd[n]);
+                if (Kind == kBnElement) bn_fetch_gate<X, Lay>(q, row, rg[n]);
             }
             if (Kind == kBnToken) gate_bits[n] = bn_gate_bits<X>(q, row);
         }
     };
-    int first = blockIdx.x * Rows;
+    int first = team * Rows;
     grid_dependency_wait();
     grid_launch_dependents();                                // (the sums' kernel waits for this one's end by itself)
     if (Post) {
@@ -698,10 +503,10 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
     }
     fetch(first);
     if (on) {
-        if (kY) bn_y_factor<X, Vec>(q, a);
-        if (Pre) bn_pre_factor<X, Vec>(q, w);
+        if (kY) bn_y_factor<X, Lay>(q, a);
+        if (Pre) bn_pre_factor<X, Lay>(q, w);
     }
-    bn_sum_init<kSums>(part);
+    bn_sum_init<Lay, kSums>(part);
     int turn = 0;
     float i1[Rows];
     #pragma unroll
@@ -710,7 +515,7 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
         float sum[Rows];
         #pragma unroll
         for (int n = 0; n < Rows; ++n) sum[n] = bn_square(ry[n]);
-        bn_sum<Rows, kSums>(sum, part, turn);
+        bn_sum<Rows, Lay, kSums>(sum, part, turn);
         #pragma unroll
         for (int n = 0; n < Rows; ++n) i1[n] = rsqrtf(sum[n] * inv_h + q.eps);
     }
@@ -740,7 +545,7 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
             #pragma unroll
             for (int k = 0; k < 5; ++k) t[k] = both(0.f);
             if (kY) bn_unpack(cy[n], v);
-            if (Kind == kBnElement) bn_unpack_gate<X, Vec>(q, cg[n], g);
+            if (Kind == kBnElement) bn_unpack_gate<X, Lay>(q, cg[n], g);
             if (Pre) bn_unpack(ch[n], dh);
             if (kSumV) bn_unpack(cd[n], d);
             #pragma unroll
@@ -770,7 +575,7 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
                 to[6] = to[7] = 0.f;
             }
         }
-        if (kSumV || Pre) bn_sum<kSums, kSums>(sum, part, turn);
+        if (kSumV || Pre) bn_sum<kSums, Lay, kSums>(sum, part, turn);
         float gate_back[Rows];
         #pragma unroll
         for (int n = 0; n < Rows; ++n) {
@@ -792,14 +597,14 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
                     d[i] = fma2(h2, w[i], fma2(r[n][i], both(-k), d[i]));
                 }
             }
-            if (on && there) bn_put<R, Vec>(static_cast<R*>(q.d_residual) + row * q.d_residual_ld, q.hidden, d);
+            if (on && there) bn_put<R, Lay>(static_cast<R*>(q.d_residual) + row * q.d_residual_ld, q.hidden, d);
             if (kY) {
                 const float2 y_up = both(i1[n] * gate[n]), y_back = both(-i1[n] * i1[n] * gate[n] * inv_h * vd);
                 float2 y[4];
                 bn_unpack(cy[n], y);
                 if (Kind == kBnElement) {
                     float2 g[4], dg[4];
-                    bn_unpack_gate<X, Vec>(q, cg[n], g);
+                    bn_unpack_gate<X, Lay>(q, cg[n], g);
                     #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         dg[i] = mul2(mul2(Post ? mul2(y[i], both(i1[n])) : y[i], a[i]), d[i]);
@@ -807,8 +612,8 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
                     }
                     if (on && there) {
                         const long long at = row * q.d_gate_ld;
-                        if (sizeof(X) == 4 || q.gate32) bn_put<float, Vec>(static_cast<float*>(q.d_gate) + at, q.hidden, dg);
-                        else bn_put<X, Vec>(static_cast<X*>(q.d_gate) + at, q.hidden, dg);
+                        if (sizeof(X) == 4 || q.gate32) bn_put<float, Lay>(static_cast<float*>(q.d_gate) + at, q.hidden, dg);
+                        else bn_put<X, Lay>(static_cast<X*>(q.d_gate) + at, q.hidden, dg);
                     }
                 }
                 #pragma unroll
@@ -817,11 +622,11 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
                     acc_y[i] = fma2(dy, y[i], acc_y[i]);
                     d[i] = Post ? fma2(y[i], y_back, mul2(dy, a[i])) : mul2(dy, a[i]);
                 }
-                if (on && there) bn_put<X, Vec>(static_cast<X*>(q.d_y) + row * q.d_y_ld, q.hidden, d);
+                if (on && there) bn_put<X, Lay>(static_cast<X*>(q.d_y) + row * q.d_y_ld, q.hidden, d);
             }
             if (Post) i1[n] = rsqrtf(of[5] * inv_h + q.eps);
         }
-        if (Kind == kBnToken && threadIdx.x < Rows && first + static_cast<int>(threadIdx.x) < tokens) {
+        if (Kind == kBnToken && (!kTwo || (blockIdx.x & 1u) == 0u) && threadIdx.x < Rows && first + static_cast<int>(threadIdx.x) < tokens) {
             const long long at = (first + static_cast<int>(threadIdx.x)) * q.d_gate_ld;
             const float of = Rows == 2 && threadIdx.x == 1 ? gate_back[Rows - 1] : gate_back[0];
             if (sizeof(X) == 4 || q.gate32) static_cast<float*>(q.d_gate)[at] = of;
@@ -831,9 +636,9 @@ __global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1)
         first += step;
     }
     if (!on) return;
-    float* p = q.partial + static_cast<long long>(blockIdx.x) * q.hidden;
-    if (Pre) bn_put<float, Vec>(p, q.hidden, acc_pre);
-    if (sum_y) bn_put<float, Vec>(Pre ? p + static_cast<long long>(gridDim.x) * q.hidden : p, q.hidden, acc_y);
+    float* p = q.partial + static_cast<long long>(team) * q.hidden;
+    if (Pre) bn_put<float, Lay>(p, q.hidden, acc_pre);
+    if (sum_y) bn_put<float, Lay>(Pre ? p + static_cast<long long>(teams) * q.hidden : p, q.hidden, acc_y);
 }
 
 // Column sums of the CTAs' partial sums: a block takes 32 channels of one of the two, a thread every 128th row of four channels, a few loads that are all on their way at
@@ -885,15 +690,11 @@ __global__ void __launch_bounds__(kBnSumThreads) block_norm_sums_kernel(const Bn
 }
 
 // ----------------------------------------------------------------------------- launches
-template <auto Kernel>
-int bn_start(const BnParams& q, int grid, cudaStream_t stream) {
-    Kernel<<<grid, bn_threads(q.hidden), 0, stream>>>(q);
-    MM_CUDA(cudaGetLastError());
-    return MM_OK;
-}
-template <auto Kernel>
-int bn_start_behind(const BnParams& q, int grid, cudaStream_t stream) {
-    MM_CUDA(launch_behind(Kernel, grid, bn_threads(q.hidden), stream, q));
+// `teams`: CTAs, or pairs of them, that rows are dealt to
+template <auto Kernel, int Lay>
+int bn_start(const BnParams& q, int teams, cudaStream_t stream) {
+    if constexpr ((Lay & kBnTwo) != 0) MM_CUDA(launch_clusters(Kernel, 2u * teams, 2, bn_threads(q.hidden), stream, q));
+    else MM_CUDA(launch_behind(Kernel, teams, bn_threads(q.hidden), stream, q));
     return MM_OK;
 }
 
@@ -910,32 +711,32 @@ int bn_per_sm(int threads, int* per) {
     return MM_OK;
 }
 
-template <typename X, typename R, bool Post, bool Pre, int Kind, bool Vec>
+template <typename X, typename R, bool Post, bool Pre, int Kind, int Lay>
 int bn_launch_kind(const BnParams& q, const BnLaunch& how, cudaStream_t stream) {
     if (how.backward) {
-        if constexpr (Vec && Kind != kBnElement && sizeof(X) == 2) {
+        if constexpr ((Lay & kBnWhole) != 0 && Kind != kBnElement && sizeof(X) == 2) {
             const int threads = bn_threads(q.hidden);
-            if (threads > kBnMaxThreads / 2 && threads <= kBnPairThreads && q.tokens >= 2ll * how.ctas)
-                return bn_start_behind<block_norm_backward_kernel<X, R, Post, Pre, Kind, true, 2>>(q, how.ctas, stream);
+            if (threads > kBnMaxThreads / 2 && threads <= kBnPairThreads && q.tokens >= 2ll * how.teams)
+                return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Lay, 2>, Lay>(q, how.teams, stream);
         }
-        return bn_start_behind<block_norm_backward_kernel<X, R, Post, Pre, Kind, Vec, 1>>(q, how.ctas, stream);
+        return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Lay, 1>, Lay>(q, how.teams, stream);
     }
     int per = 0;
-    const int st = bn_per_sm<block_norm_kernel<X, R, Post, Pre, Kind, Vec>>(bn_threads(q.hidden), &per);
+    const int st = bn_per_sm<block_norm_kernel<X, R, Post, Pre, Kind, Lay>>(bn_threads(q.hidden), &per);
     if (st != MM_OK) return st;
-    const long long most = static_cast<long long>(per) * how.sms;
-    return bn_start_behind<block_norm_kernel<X, R, Post, Pre, Kind, Vec>>(q, static_cast<int>(q.tokens < most ? q.tokens : most), stream);
+    const long long most = static_cast<long long>(per) * how.sms / ((Lay & kBnTwo) != 0 ? 2 : 1);
+    return bn_start<block_norm_kernel<X, R, Post, Pre, Kind, Lay>, Lay>(q, static_cast<int>(q.tokens < most ? q.tokens : most), stream);
 }
 
-template <typename X, typename R, bool Vec>
+template <typename X, typename R, int Lay>
 int bn_launch_rows(const BnParams& q, const BnLaunch& how, cudaStream_t stream) {
     const bool post = q.post_w != nullptr, pre = q.pre_w != nullptr;
-    if (q.y == nullptr) return bn_launch_kind<X, R, false, true, kBnStream, Vec>(q, how, stream);
+    if (q.y == nullptr) return bn_launch_kind<X, R, false, true, kBnStream, Lay>(q, how, stream);
     auto by_kind = [&](auto p, auto n) {
         constexpr bool kPost = decltype(p)::value, kPre = decltype(n)::value;
-        if (q.gate_mode == kBnGateToken) return bn_launch_kind<X, R, kPost, kPre, kBnToken, Vec>(q, how, stream);
-        if (q.gate_mode == kBnGateElement) return bn_launch_kind<X, R, kPost, kPre, kBnElement, Vec>(q, how, stream);
-        return bn_launch_kind<X, R, kPost, kPre, kBnPlain, Vec>(q, how, stream);
+        if (q.gate_mode == kBnGateToken) return bn_launch_kind<X, R, kPost, kPre, kBnToken, Lay>(q, how, stream);
+        if (q.gate_mode == kBnGateElement) return bn_launch_kind<X, R, kPost, kPre, kBnElement, Lay>(q, how, stream);
+        return bn_launch_kind<X, R, kPost, kPre, kBnPlain, Lay>(q, how, stream);
     };
     using std::false_type;
     using std::true_type;
@@ -943,12 +744,11 @@ int bn_launch_rows(const BnParams& q, const BnLaunch& how, cudaStream_t stream) 
                 : (pre ? by_kind(false_type{}, true_type{}) : by_kind(false_type{}, false_type{}));
 }
 
-template <typename X, typename R>
+// Two: rows of more than 4096 channels (compiled in files of their own)
+template <typename X, typename R, bool Two>
 int bn_launch(const BnParams& q, const BnLaunch& how, cudaStream_t stream) {
-    if (q.hidden <= kBnHeldHidden) return how.aligned ? bn_launch_rows<X, R, true>(q, how, stream) : bn_launch_rows<X, R, false>(q, how, stream);
-    if (how.backward) return bn_start<block_norm_backward_wide_kernel<X, R>>(q, how.ctas, stream);
-    const long long most = 2ll * how.sms;
-    return bn_start<block_norm_wide_kernel<X, R>>(q, static_cast<int>(q.tokens < most ? q.tokens : most), stream);
+    constexpr int two = Two ? kBnTwo : 0;
+    return how.aligned ? bn_launch_rows<X, R, two | kBnWhole>(q, how, stream) : bn_launch_rows<X, R, two>(q, how, stream);
 }
 
 template <typename X>

@@ -8,7 +8,7 @@ namespace mm {
 constexpr int kBnMaxHidden = 8192;
 constexpr int kBnMaxThreads = 512;
 constexpr int kBnPairThreads = 384;
-constexpr int kBnHeldHidden = 8 * kBnMaxThreads;             // up to here a thread holds eight channels of a row
+constexpr int kBnOneHidden = 8 * kBnMaxThreads;              // channels that one CTA holds of a row; wider rows belong to two
 enum BnGate { kBnGateNone = 0, kBnGateChannel = 1, kBnGateToken = 2, kBnGateElement = 3 };
 
 struct BnParams {
@@ -31,27 +31,30 @@ struct BnSumsParams {
     float scale, offset;
 };
 
-// `aligned`: rows start on 16 bytes (32-bit ones on 32) and are made of whole groups of eight channels. `ctas`: of a backward pass, with its partial sums.
+// `aligned`: rows start on 16 bytes (32-bit ones on 32) and are made of whole groups of eight channels. `teams`: of a backward pass, with its partial sums.
 struct BnLaunch {
     bool backward, stream32, aligned;
-    int sms, ctas;
+    int sms, teams;
 };
 int launch_block_norm_bf16(const BnParams& q, const BnLaunch& how, cudaStream_t stream);
+int launch_block_norm_wide_bf16(const BnParams& q, const BnLaunch& how, cudaStream_t stream);
 int launch_block_norm_fp16(const BnParams& q, const BnLaunch& how, cudaStream_t stream);
+int launch_block_norm_wide_fp16(const BnParams& q, const BnLaunch& how, cudaStream_t stream);
 int launch_block_norm_fp32(const BnParams& q, const BnLaunch& how, cudaStream_t stream);
+int launch_block_norm_wide_fp32(const BnParams& q, const BnLaunch& how, cudaStream_t stream);
 int launch_block_norm_sums_bf16(const BnSumsParams& q, cudaStream_t stream);
 int launch_block_norm_sums_fp16(const BnSumsParams& q, cudaStream_t stream);
 int launch_block_norm_sums_fp32(const BnSumsParams& q, cudaStream_t stream);
 
-// Threads of a CTA, and CTAs of a backward pass: each leaves a row of partial sums, so the workspace goes by them, and as many as a B200 with its 148 SMs holds
-// at a time (128 registers a thread) leave it.
+// Threads of a CTA, and teams (CTAs, or pairs of them) of a backward pass: each leaves a row of partial sums, so the workspace goes by them, and as many as a B200 with its
+// 148 SMs holds at a time (128 registers a thread) leave it.
 inline int bn_threads(int hidden) {
-    const int per = hidden <= kBnHeldHidden ? 8 : 16;
+    const int per = hidden <= kBnOneHidden ? 8 : 16;
     return ((hidden + per - 1) / per + 31) / 32 * 32;
 }
-inline long long bn_backward_ctas(long long tokens, int hidden) {
+inline long long bn_backward_teams(long long tokens, int hidden) {
     const int fit = 512 / bn_threads(hidden);
-    const long long most = 148ll * (fit < 1 ? 1 : (fit > 8 ? 8 : fit));
+    const long long most = hidden > kBnOneHidden ? 74 : 148ll * (fit < 1 ? 1 : (fit > 8 ? 8 : fit));
     return tokens < most ? tokens : most;
 }
 

@@ -17,16 +17,16 @@ cudaError_t launch_behind(void (*kernel)(P), unsigned grid, unsigned threads, cu
     return cudaLaunchKernelEx(&cfg, kernel, params);
 }
 
-// One cluster of `ctas` CTAs (at most eight), as early.
+// Clusters of `size` CTAs (at most eight), as early.
 template <typename P>
-cudaError_t launch_cluster(void (*kernel)(P), unsigned ctas, unsigned threads, cudaStream_t stream, const P& params) {
+cudaError_t launch_clusters(void (*kernel)(P), unsigned grid, unsigned size, unsigned threads, cudaStream_t stream, const P& params) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.x = size; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(threads); cfg.stream = stream;
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(threads); cfg.stream = stream;
     cfg.attrs = attr; cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, params);
 }

@@ -769,7 +769,7 @@ int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
         if (op == kRtBalance && q.T <= kRtSmallTokens && static_cast<long long>(q.S) * q.E <= kRtSmallCells && q.S <= kRtSmallSequences) {
             // (sequences: all the CTAs there can be, because each takes its pieces of them one after the other)
             const int want = q.S > 1 ? q.T : (q.T + kRtSmallWarps - 1) / kRtSmallWarps, ctas = want < 1 ? 1 : (want < kRtSmallCtas ? want : kRtSmallCtas);
-            MM_CUDA(launch_cluster(balance_small_kernel<L, V, Mode>, ctas, kRtSmallWarps * 32, stream, shared_out(ctas)));
+            MM_CUDA(launch_clusters(balance_small_kernel<L, V, Mode>, ctas, ctas, kRtSmallWarps * 32, stream, shared_out(ctas)));
             return MM_OK;
         }
     }

@@ -97,6 +97,21 @@ def test_rows_in_pairs(tokens, hidden):
         assert all(a is None or torch.equal(a, b) for a, b in zip(mm.block_norm_backward(d_stream, d_normed, **x), mm.block_norm_backward(d_stream, d_normed, **x)))
 
 
+@pytest.mark.parametrize('hidden', [4097, 4104, 5120, 8190, 8192])
+@pytest.mark.parametrize('tokens', [73, 75, 149, 400])
+def test_rows_of_two_ctas(tokens, hidden):
+    """Rows of more than 4096 channels, around the numbers of pairs of CTAs that a GPU holds: results, and the same ones in every call."""
+    for i, kind in enumerate([dict(gate='token'), dict(gate='channel', post=False), dict(pre=False), dict(gate='element'), dict(y=False, post=False), dict()]):
+        types = {**TYPES[(i + tokens + hidden) % len(TYPES)], 'stream': None}
+        x, d_stream, d_normed = _inputs(tokens, hidden, **types, **kind, seed=i)
+        out, grads = mm.block_norm(**x), mm.block_norm_backward(d_stream, d_normed, **x)
+        _check_forward(x, out)
+        _check_gradients(x, d_stream, d_normed, grads)
+        for _ in range(3):                     # one behind the other
+            again, grads_again = mm.block_norm(**x), mm.block_norm_backward(d_stream, d_normed, **x)
+        assert all(a is None or torch.equal(a, b) for a, b in zip((*out, *grads), (*again, *grads_again)))
+
+
 def test_one_gradient_only():
     x, d_stream, d_normed = _inputs(40, 512, gate='token')
     grads = mm.block_norm_backward(None, d_normed, **x)
