@@ -175,6 +175,44 @@ def test_strided_rows(hidden, pad, gate):
     _check_gradients(x, d_stream, d_normed, grads)
 
 
+@pytest.mark.parametrize('tokens, hidden, pad, start', [(5, 9, 0, 0), (2600, 1001, 0, 0), (2600, 1001, 2, 0), (1300, 2047, 5, 0), (700, 3002, 0, 0), (700, 3002, 1, 1), (400, 4089, 0, 0), (400, 4091, 0, 0),
+                                                        (300, 5003, 0, 0), (300, 5003, 4, 3), (160, 8185, 3, 0), (160, 8187, 0, 0), (4000, 67, 0, 0), (4000, 67, 6, 5), (5000, 8, 1, 0), (3000, 5, 0, 0)])
+def test_rows_that_start_anywhere(tokens, hidden, pad, start):
+    """Rows whose starts lie on no boundary, or the first of which lies on one, more of them than are worked on at a time; NaN between and behind them, which has to stay."""
+    ld = hidden + pad
+
+    def among_nan(t):
+        if t is None or t.dim() == 1 or t.shape[1] == 1:
+            return None, t
+        buf = torch.full((start + tokens * ld + 8,), float('nan'), dtype=t.dtype, device='cuda')
+        rows = buf[start:start + tokens * ld].view(tokens, ld)[:, :hidden]
+        rows.copy_(t)
+        return buf, rows
+    for i, kind in enumerate([dict(), dict(gate='token', pre=False), dict(gate='element'), dict(y=False, post=False), dict(gate='channel', post=False), dict(gate='token')]):
+        types = {**TYPES[(i + tokens + pad) % len(TYPES)]}
+        if not kind.get('y', True):
+            types['stream'] = None
+        x, d_stream, d_normed = _inputs(tokens, hidden, **types, **kind, seed=i)
+        s = {name: among_nan(t)[1] for name, t in x.items()}
+        bufs = [among_nan(torch.zeros_like(x[name])) if x[name] is not None else (None, None) for name in ('residual', 'y')]
+        buf_n, normed = among_nan(torch.zeros_like(d_normed)) if d_normed is not None else (None, None)
+        out = mm.block_norm(**s, residual_out=bufs[0][1] if x['y'] is not None else None, normed=normed)
+        _check_forward(x, out)
+        for buf, rows in ((bufs[0][0] if x['y'] is not None else None, out[0]), (buf_n, out[1])):
+            if buf is not None:
+                rows.zero_()
+                assert int(torch.isnan(buf).sum()) == buf.numel() - tokens * hidden
+        grads = mm.block_norm_backward(among_nan(d_stream)[1], among_nan(d_normed)[1], **s)
+        _check_gradients(x, d_stream, d_normed, grads)
+        again = mm.block_norm_backward(among_nan(d_stream)[1], among_nan(d_normed)[1], **s)
+        assert all(a is None or torch.equal(a, b) for a, b in zip(grads, again))
+        if x['y'] is not None and pad == 0 and start == 0:       # in place
+            stream, y = x['residual'].clone(), x['y'].clone()
+            once = mm.block_norm(**x)
+            twice = mm.block_norm(**{**x, 'residual': stream, 'y': y}, residual_out=stream, normed=y if x['pre_weight'] is not None else None)
+            assert torch.equal(once[0], twice[0]) and (once[1] is None or torch.equal(once[1], twice[1]))
+
+
 def test_rows_far_apart():
     """Element offsets beyond 32 bits."""
     hidden, ld = 256, 2 ** 31 // 2 + 8
