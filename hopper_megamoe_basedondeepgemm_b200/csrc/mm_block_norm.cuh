@@ -441,10 +441,11 @@ __global__ void __maxnreg__((sizeof(R) == 2 && (Lay & kBnWhole) != 0 && Kind != 
 // Where a CTA of 128 registers a thread leaves an SM's registers half used and no second one fits (more than 256 threads, up to 384: hidden 2056 to 3072, and 4104 to 6144 over two CTAs), it takes two rows
 // at a time through one exchange, with 168: 8192 x 3072 in bf16 59 us instead of 67, only the stream's norm 53 instead of 64, 32-bit stream 74 instead of 81. (With 256 threads
 // two CTAs of one row win, 42 us against 46 for 8192 x 2048; with an element's gate, or 32-bit
-// activations, two rows do not fit the registers.)
+// activations, two rows do not fit the registers.) With an element's gate one row takes those 168: 128 are too few, and a register that is put away while its load is on its way
+// waits for it (8192 x 3072 bf16 82 us instead of 94, 8192 x 3001 134 instead of 370; odd rows without such a gate are faster with 128, 114 against 141).
 // Rows over two CTAs: 8192 x 8192 bf16 254 us (3.2 TB/s), 32-bit stream 276 (4.4), 4096 x 6144 bf16, two rows at a time, 85 (one at a time 111; clusters of four 172).
-template <typename X, typename R, bool Post, bool Pre, int Kind, int Lay, int Rows>
-__global__ void __launch_bounds__(Rows == 2 ? kBnPairThreads : kBnMaxThreads, 1) block_norm_backward_kernel(const BnParams q) {
+template <typename X, typename R, bool Post, bool Pre, int Kind, int Lay, int Rows, int Most>
+__global__ void __launch_bounds__(Most, 1) block_norm_backward_kernel(const BnParams q) {
     constexpr bool kY = Kind != kBnStream, kSumV = Post || Kind == kBnToken;
     constexpr int kSums = (kSumV ? 8 : 2) * Rows;
     constexpr bool kWhole = (Lay & kBnWhole) != 0, kTwo = (Lay & kBnTwo) != 0;
@@ -721,12 +722,15 @@ int bn_per_sm(int threads, int* per) {
 template <typename X, typename R, bool Post, bool Pre, int Kind, int Lay>
 int bn_launch_kind(const BnParams& q, const BnLaunch& how, cudaStream_t stream) {
     if (how.backward) {
-        if constexpr ((Lay & kBnWhole) != 0 && Kind != kBnElement && sizeof(X) == 2) {
-            const int threads = bn_threads(q.hidden);
-            if (threads > kBnMaxThreads / 2 && threads <= kBnPairThreads && q.tokens >= 2ll * how.teams)
-                return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Lay, 2>, Lay>(q, how.teams, stream);
+        constexpr bool kPairs = (Lay & kBnWhole) != 0 && Kind != kBnElement && sizeof(X) == 2, kMore = Kind == kBnElement;
+        const int threads = bn_threads(q.hidden);
+        if (threads > kBnMaxThreads / 2 && threads <= kBnPairThreads) {
+            if constexpr (kPairs) {
+                if (q.tokens >= 2ll * how.teams) return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Lay, 2, kBnPairThreads>, Lay>(q, how.teams, stream);
+            }
+            if constexpr (kMore) return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Lay, 1, kBnPairThreads>, Lay>(q, how.teams, stream);
         }
-        return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Lay, 1>, Lay>(q, how.teams, stream);
+        return bn_start<block_norm_backward_kernel<X, R, Post, Pre, Kind, Lay, 1, kBnMaxThreads>, Lay>(q, how.teams, stream);
     }
     int per = 0;
     const int st = bn_per_sm<block_norm_kernel<X, R, Post, Pre, Kind, Lay>>(bn_threads(q.hidden), &per);
