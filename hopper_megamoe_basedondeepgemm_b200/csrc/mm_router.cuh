@@ -471,14 +471,13 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lo = rt_share(q, blockIdx.x), hi = rt_share(q, blockIdx.x + 1);
-    grid_launch_dependents();                // (what was ahead of `balance_zero_kernel` has ended)
     for (int e = threadIdx.x; e < V * 32; e += blockDim.x) hist[e] = 0;
     __syncthreads();
-    bool zeroed = false;
+    grid_dependency_wait();                  // (for the cleared sums, and for the logits and routes of kernels ahead of `balance_zero_kernel`: only a grid that waits sees what others wrote)
+    grid_launch_dependents();
     const double z = rt_balance_tokens<L, V, Mode, kRtWarps>(
         q, lo, hi, [&](int, int e) { atomicAdd(hist + e, 1); },
         [&](int s, const float (&acc)[V], int n) {
-            if (!zeroed) { grid_dependency_wait(); zeroed = true; }          // (the sums are zero now)
             #pragma unroll
             for (int j = 0; j < V; ++j) warp_sum[warp][j * 32 + lane] = acc[j];
             if (lane == 0) warp_tokens[warp] = n;
@@ -499,7 +498,6 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
             }
             __syncthreads();
         });
-    if (!zeroed) grid_dependency_wait();
     if (lane == 0) warp_z[warp] = z;
     __syncthreads();
     if (threadIdx.x == 0) {
