@@ -70,6 +70,9 @@ __device__ __forceinline__ float rt_exp(float v) { return rt_exp2(v * kRtLog2e);
 // sigmoid(v), and 1 - sigmoid(v) without the difference of near numbers
 __device__ __forceinline__ float rt_sigmoid(float v) { return rt_rcp(1.f + rt_exp(-v)); }
 __device__ __forceinline__ float rt_sigmoid_rest(float v) { return rt_rcp(1.f + rt_exp(v)); }
+// Scores of which only the ratio counts. Where all of a token's sigmoids are below 2^-24 each is its exponential, as far as 32 bits tell, and is taken relative to the largest one:
+// from a logit of -87 on the sigmoid by itself is 0 in 32 bits. Tokens whose logits are all below kRtLowest have scores of 0 in 64 bits, too, and count as such.
+constexpr float kRtLowSum = 0x1p-24f, kRtLow = -17.f, kRtLowest = -709.78f;
 
 template <typename L, int V>
 __device__ __forceinline__ void rt_fetch(const RtParams& q, int row, int lane, float (&l)[V]) {
@@ -242,7 +245,12 @@ __global__ void __launch_bounds__(kRtWarps * 32) route_kernel(const RtParams q) 
             const float top = rt_max(logit);
             if (chosen) s = rt_exp(logit - top);
         }
-        const float total = rt_sum(s);
+        float total = rt_sum(s);
+        if (Mode == 1 && total < kRtLowSum) {
+            const float top = rt_max(logit);
+            s = chosen && top >= kRtLowest ? rt_exp(logit - top) : 0.f;
+            total = rt_sum(s);
+        }
         const long long to = static_cast<long long>(row) * q.K;
         if (chosen) {
             q.idx[to + rank] = at;
@@ -283,7 +291,7 @@ __device__ __forceinline__ bool rt_scores_try(const float (&l)[V], RtScores<V>& 
     }
     float sum = 0.f, sig_sum = 0.f;
     // mode 1: exp(l) by itself, where it neither overflows nor loses the largest of them, gives both the softmax and the sigmoid
-    const bool plain = Mode == 1 && fabsf(top) <= 40.f;
+    const bool plain = Mode == 1 && top >= kRtLow && top <= 40.f;
     const float base = plain ? 0.f : top, shift = base * kRtLog2e;
     #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -298,6 +306,9 @@ __device__ __forceinline__ bool rt_scores_try(const float (&l)[V], RtScores<V>& 
             if (plain) {
                 s.rest[j] = rt_rcp(1.f + s.exp[j]);
                 s.sig[j] = s.exp[j] * s.rest[j];
+            } else if (top < kRtLow) {
+                s.sig[j] = top >= kRtLowest ? s.exp[j] : 0.f;
+                s.rest[j] = 1.f;
             } else {
                 s.sig[j] = rt_sigmoid(l[j]);
                 if (Rest) s.rest[j] = rt_sigmoid_rest(l[j]);
@@ -719,7 +730,12 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) router_backward_k
                 const float top = rt_max(mine);
                 if (mine > rt_off()) w = rt_exp(mine - top);
             }
-            const float total = rt_sum(w);
+            float total = rt_sum(w);
+            if (Mode == 1 && total < kRtLowSum) {                        // (then `rest` is 1 to 32 bits)
+                const float top = rt_max(mine);
+                w = mine > rt_off() && top >= kRtLowest ? rt_exp(mine - top) : 0.f;
+                total = rt_sum(w);
+            }
             w = total > 0.f ? w * rt_rcp(total) : 0.f;
             const float inner = rt_sum(w * dw);
             const float dk = w * (dw - inner) * rest;

@@ -18,8 +18,8 @@ def route_tokens(logits: torch.Tensor, topk: int, score_mode: int = 0, expert_bi
     """`(topk_idx int64, topk_weights fp32)`, both `[tokens, topk]`, of bf16, fp16 or fp32 logits `[tokens, experts]`.
 
     score_mode 0: the largest logits; weights are the softmax over the selected ones. 1: the largest `sigmoid(logit) + expert_bias` (fp32
-    `[experts]`, optional), compared as in 64 bits; weights are the sigmoids over their sum. Both times `route_scale`. Experts come in descending
-    order, equal ones lower index first. A logit of -inf or NaN switches an expert off for the token, a bias of -inf or NaN for all. Slots for which no expert is left,
+    `[experts]`, optional), compared as in 64 bits; weights are the sigmoids over their sum, also where these are smaller than 32 bits hold (and 0 where they are 0 in
+    64: all selected logits below -709). Both times `route_scale`. Experts come in descending order, equal ones lower index first. A logit of -inf or NaN switches an expert off for the token, a bias of -inf or NaN for all. Slots for which no expert is left,
     and tokens whose `valid` (bool or uint8 `[tokens]`) is 0, get index -1 and weight 0: the layer's masked slots. `topk_idx` / `topk_weights` may
     be given, e.g. `sym_buffer.topk_idx[:tokens]`, apart from everything that the call reads. At most 1024 experts and 32 routes per token.
     """
