@@ -33,10 +33,11 @@ bool share_memory(const Rows& a, const Rows& b) {
     const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
     const uintptr_t ea = pa + (a.n - 1) * a.ld + a.width, eb = pb + (b.n - 1) * b.ld + b.width;
     if (ea <= pb || eb <= pa) return false;
-    if (a.ld != b.ld || a.ld == 0) return true;
-    const int64_t d = pa > pb ? static_cast<int64_t>((pa - pb) % a.ld) : static_cast<int64_t>((pb - pa) % a.ld);
+    const int64_t ld = a.n == 1 ? b.ld : a.ld;                              // (a single one may lie between the others' rows)
+    if ((b.n != 1 && b.ld != ld) || ld == 0) return true;
+    const int64_t d = pa > pb ? static_cast<int64_t>((pa - pb) % ld) : static_cast<int64_t>((pb - pa) % ld);
     const int64_t first = pa > pb ? b.width : a.width, second = pa > pb ? a.width : b.width;       // columns of one buffer lie beside each other
-    return !(d >= first && a.ld - d >= second);
+    return !(d >= first && ld - d >= second);
 }
 
 // An output may be the very rows of an input that is read by the thread which writes them, and nothing else of any tensor of the call.
@@ -208,21 +209,25 @@ int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_gr
     }
     cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
     const int64_t teams = mm::bn_backward_teams(t, a->hidden);
+    const Rows none = {nullptr, 0, 0, 0};
+    // gradients of rows, gradients of channels, working memory; what is read
+    Rows rows[14] = {rows_of(g->d_residual, g->d_residual_stride, t, a->hidden, a->stream_dtype), rows_of(g->d_y, g->d_y_stride, t, a->hidden, a->dtype),
+                     element ? rows_of(g->d_gate, g->d_gate_stride, t, a->hidden, a->gate_dtype) : (token ? rows_of(g->d_gate, g->d_gate_stride, t, 1, a->gate_dtype) : none),
+                     channel ? rows_of(g->d_gate, 0, 1, a->hidden, a->gate_dtype) : none, rows_of(g->d_pre_weight, 0, 1, a->hidden, a->weight_dtype),
+                     rows_of(g->d_post_weight, 0, 1, a->hidden, a->weight_dtype), t > 0 && sums > 0 ? Rows{g->workspace, 0, mm_block_norm_workspace_bytes(t, a->hidden), 1} : none,
+                     rows_of(g->d_residual_out, g->d_residual_out_stride, t, a->hidden, a->stream_dtype), rows_of(g->d_normed, g->d_normed_stride, t, a->hidden, a->dtype),
+                     rows_of(a->residual, a->residual_stride, t, a->hidden, a->stream_dtype), rows_of(a->y, a->y_stride, t, a->hidden, a->dtype),
+                     element ? rows_of(a->gate, a->gate_stride, t, a->hidden, a->gate_dtype) : (token ? rows_of(a->gate, a->gate_stride, t, 1, a->gate_dtype) : rows_of(a->gate, 0, 1, a->hidden, a->gate_dtype)),
+                     rows_of(a->pre_weight, 0, 1, a->hidden, a->weight_dtype), rows_of(a->post_weight, 0, 1, a->hidden, a->weight_dtype)};
+    constexpr int kOutputs = 7;
+    if (t == 1) for (Rows& r : rows) r.ld = 0;
+    for (int i = 0; i < kOutputs; ++i) {
+        if (i < 3 && t > 1 && rows[i].p != nullptr && rows[i].ld < rows[i].width) return MM_ERR_INVALID_ARGUMENT;
+        for (int k = i + 1; k < 14; ++k)         // written apart from everything else
+            if (share_memory(rows[i], rows[k])) return MM_ERR_INVALID_ARGUMENT;
+    }
     if (t > 0) {
-        const Rows none = {nullptr, 0, 0, 0};
-        Rows rows[10] = {rows_of(g->d_residual, g->d_residual_stride, t, a->hidden, a->stream_dtype), rows_of(g->d_y, g->d_y_stride, t, a->hidden, a->dtype),
-                         element ? rows_of(g->d_gate, g->d_gate_stride, t, a->hidden, a->gate_dtype) : (token ? rows_of(g->d_gate, g->d_gate_stride, t, 1, a->gate_dtype) : none),
-                         rows_of(g->d_residual_out, g->d_residual_out_stride, t, a->hidden, a->stream_dtype), rows_of(g->d_normed, g->d_normed_stride, t, a->hidden, a->dtype),
-                         rows_of(a->residual, a->residual_stride, t, a->hidden, a->stream_dtype), rows_of(a->y, a->y_stride, t, a->hidden, a->dtype),
-                         element ? rows_of(a->gate, a->gate_stride, t, a->hidden, a->gate_dtype) : (token ? rows_of(a->gate, a->gate_stride, t, 1, a->gate_dtype) : rows_of(a->gate, 0, 1, a->hidden, a->gate_dtype)),
-                         rows_of(a->pre_weight, 0, 1, a->hidden, a->weight_dtype), rows_of(a->post_weight, 0, 1, a->hidden, a->weight_dtype)};
-        if (t == 1) for (Rows& r : rows) r.ld = 0;
-        for (int i = 0; i < 3; ++i) {
-            if (t > 1 && rows[i].p != nullptr && rows[i].ld < rows[i].width) return MM_ERR_INVALID_ARGUMENT;
-            for (int k = 0; k < 10; ++k)         // gradients are written apart from everything else
-                if (k != i && share_memory(rows[i], rows[k])) return MM_ERR_INVALID_ARGUMENT;
-        }
-        if (token) rows[2].p = rows[7].p = nullptr;
+        const Rows eights[10] = {rows[0], rows[1], rows[7], rows[8], rows[9], rows[10], rows[12], rows[13], token ? none : rows[2], token ? none : rows[11]};   // (a token's gate is read one by one)
         mm::BnParams q = norm_params(a);
         q.d_residual_out = g->d_residual_out; q.d_residual_out_ld = g->d_residual_out_stride;
         q.d_normed = g->d_normed; q.d_normed_ld = g->d_normed_stride;
@@ -230,7 +235,7 @@ int mm_block_norm_backward(const mm_block_norm_args_t* a, const mm_block_norm_gr
         q.d_y = g->d_y; q.d_y_ld = g->d_y_stride;
         q.d_gate = g->d_gate; q.d_gate_ld = g->d_gate_stride;
         q.partial = static_cast<float*>(g->workspace);
-        st = launch_norm(a->dtype, q, {true, a->stream_dtype == MM_DTYPE_FP32, norm_rows_aligned(a->hidden, rows, 10), 0, static_cast<int>(teams)}, stream);
+        st = launch_norm(a->dtype, q, {true, a->stream_dtype == MM_DTYPE_FP32, norm_rows_aligned(a->hidden, eights, 10), 0, static_cast<int>(teams)}, stream);
         if (st != MM_OK) return st;
     }
     if (sums > 0) {

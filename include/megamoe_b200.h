@@ -272,7 +272,7 @@ typedef struct mm_block_norm_args {
     float scale, eps, weight_offset; /* eps > 0 */
 } mm_block_norm_args_t;
 
-/* The gradients' side of mm_block_norm_backward. No output shares memory with anything else of the call. */
+/* The gradients' side of mm_block_norm_backward. Outputs and the workspace that share memory with each other or with an input are refused. */
 typedef struct mm_block_norm_grads {
     const void* d_residual_out;      /* stream_dtype [tokens][hidden], or NULL: zero */
     const void* d_normed;            /* dtype [tokens][hidden]; NULL if pre_weight is */
