@@ -16,7 +16,7 @@ BINDING_SOURCE = 'mm_block_binding.cpp'
 _ABI = os.path.join('..', '..', 'include', 'megamoe_b200.h')
 SOURCES = {
     'mm_abi.cu': ['mm_kernel.cuh', 'mm_frontend.cuh', 'mm_frontend_route.h', 'mm_device_attribute.h', 'mm_ptx.cuh', 'mm_prep.cuh', 'mm_batch.cuh',
-                  'mm_decode.cuh', 'mm_error.h', _ABI],
+                  'mm_decode.cuh', 'mm_error.h', 'mm_launch.h', _ABI],
     'mm_block.cu': ['mm_block_norm.h', 'mm_router.h', 'mm_error.h', _ABI],
     **{f'mm_block_norm_{w}{t}.cu': ['mm_block_norm.cuh', 'mm_block_norm.h', 'mm_launch.h', 'mm_ptx.cuh', 'mm_error.h', _ABI] for w in ('', 'wide_') for t in ('bf16', 'fp16', 'fp32')},
     **{f'mm_router_{t}.cu': ['mm_router.cuh', 'mm_router.h', 'mm_launch.h', 'mm_ptx.cuh', 'mm_error.h', _ABI] for t in ('bf16', 'fp16', 'fp32')},

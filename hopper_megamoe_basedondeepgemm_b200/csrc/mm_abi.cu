@@ -13,6 +13,7 @@
 #include "mm_decode.cuh"
 #include "mm_device_attribute.h"
 #include "mm_error.h"
+#include "mm_launch.h"
 
 namespace mm {
 
@@ -668,8 +669,7 @@ int mm_transform_weights(const void* w_packed, const void* sf, int32_t sf_is_fp3
     q.unit_bytes = mm::kUnitWBytes + q.planes * 512;
     const long long units = static_cast<long long>(num_groups) * (n / 128) * (k / 256);
     if (units > 0x7FFFFFFFll) return MM_ERR_UNSUPPORTED;
-    mm::pretile_weights_kernel<<<static_cast<unsigned>(units), 256, 0, static_cast<cudaStream_t>(stream)>>>(q);
-    MM_CUDA(cudaGetLastError());
+    MM_CUDA(mm::launch_plain(mm::pretile_weights_kernel, static_cast<unsigned>(units), 256, static_cast<cudaStream_t>(stream), q));
     return MM_OK;
 }
 
@@ -681,13 +681,9 @@ int mm_cast_rows_to_fp4(const void* x, int32_t x_is_bf16, int32_t m, int32_t k, 
     const long long threads = static_cast<long long>(m) * (k / 8);
     const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (x_is_bf16)
-        mm::cast_rows_fp4_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), m, k, gran_k, use_ue8m0,
-                                                                      static_cast<uint8_t*>(packed_out), sf_out);
-    else
-        mm::cast_rows_fp4_kernel<float><<<blocks, 256, 0, s>>>(static_cast<const float*>(x), m, k, gran_k, use_ue8m0,
-                                                              static_cast<uint8_t*>(packed_out), sf_out);
-    MM_CUDA(cudaGetLastError());
+    uint8_t* out = static_cast<uint8_t*>(packed_out);
+    if (x_is_bf16) MM_CUDA(mm::launch_plain(mm::cast_rows_fp4_kernel<__nv_bfloat16>, blocks, 256, s, static_cast<const __nv_bfloat16*>(x), m, k, gran_k, use_ue8m0, out, sf_out));
+    else MM_CUDA(mm::launch_plain(mm::cast_rows_fp4_kernel<float>, blocks, 256, s, static_cast<const float*>(x), m, k, gran_k, use_ue8m0, out, sf_out));
     return MM_OK;
 }
 
@@ -700,11 +696,10 @@ int mm_tensor_absmax(const void* x, int32_t x_is_bf16, int64_t n, float* absmax_
     const long long per = x_is_bf16 ? 8 : 4;
     long long blocks = (n / per + 255) / 256;
     blocks = blocks < 1 ? 1 : (blocks > 1184 ? 1184 : blocks);                               // eight blocks per SM at most
-    if (x_is_bf16)
-        mm::absmax_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), n, reinterpret_cast<uint32_t*>(absmax_out));
-    else
-        mm::absmax_kernel<float><<<static_cast<unsigned>(blocks), 256, 0, s>>>(static_cast<const float*>(x), n, reinterpret_cast<uint32_t*>(absmax_out));
-    MM_CUDA(cudaGetLastError());
+    const unsigned grid = static_cast<unsigned>(blocks);
+    uint32_t* out = reinterpret_cast<uint32_t*>(absmax_out);
+    if (x_is_bf16) MM_CUDA(mm::launch_plain(mm::absmax_kernel<__nv_bfloat16>, grid, 256, s, static_cast<const __nv_bfloat16*>(x), n, out));
+    else MM_CUDA(mm::launch_plain(mm::absmax_kernel<float>, grid, 256, s, static_cast<const float*>(x), n, out));
     return MM_OK;
 }
 

@@ -17,6 +17,14 @@ cudaError_t launch_behind(void (*kernel)(P), unsigned grid, unsigned threads, cu
     return cudaLaunchKernelEx(&cfg, kernel, params);
 }
 
+// A launch that begins when the kernel ahead of it has ended. Like those above it says how it went by itself: `cudaGetLastError` would report what an earlier call left.
+template <typename... P, typename... A>
+cudaError_t launch_plain(void (*kernel)(P...), unsigned grid, unsigned threads, cudaStream_t stream, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(threads); cfg.stream = stream;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Clusters of `size` CTAs (at most eight), as early.
 template <typename P>
 cudaError_t launch_clusters(void (*kernel)(P), unsigned grid, unsigned size, unsigned threads, cudaStream_t stream, const P& params) {

@@ -800,16 +800,14 @@ int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
         MM_CUDA(launch_behind(balance_kernel<L, V, Mode>, b.z_parts, kRtWarps * 32, stream, b));
         const long long cells = static_cast<long long>(q.S) * q.E;
         if (cells > kRtEndCells) {
-            MM_CUDA(cudaGetLastError());
             const long long want = cells / 2048;
-            balance_end_kernel<L><<<static_cast<int>(want < kRtBalanceCtas ? want : kRtBalanceCtas), kRtWarps * 32, 0, stream>>>(b);
+            MM_CUDA(launch_plain(balance_end_kernel<L>, static_cast<unsigned>(want < kRtBalanceCtas ? want : kRtBalanceCtas), kRtWarps * 32, stream, b));
         }
     } else if (op == kRtRoute) {
         MM_CUDA(launch_behind(route_kernel<L, V, Mode>, blocks < sms * 8 ? blocks : sms * 8, kRtWarps * 32, stream, q));
     } else {
         MM_CUDA(launch_behind(router_backward_kernel<L, V, Mode>, grid, kRtWarps * 32, stream, shared_out(grid * kRtWarps)));
     }
-    MM_CUDA(cudaGetLastError());
     return MM_OK;
 }
 
