@@ -3,7 +3,9 @@
 Between two blocks a program adds a block's output to the residual stream and normalises the sum for the next one; some models normalise the output
 too, gate it (a shared expert's gate per token, a learned scale per channel) or scale it. `block_norm` is all of that in one pass over the rows:
 what it leaves in `normed` is what `mega_moe_from_hidden` and `fe_forward` read, and the layer's `y` goes back through it. One token or a prefill
-chunk, in place where the program wants it. `block_norm_backward` is its gradient. Neither is recorded by autograd.
+chunk, in place where the program wants it. `block_norm_backward` is its gradient. Neither is recorded by autograd: `block_norm` refuses tensors that require a gradient while
+gradients are enabled (a training step calls the pair from a `torch.autograd.Function`, or on detached tensors). `block_norm_backward` takes them; its results have no
+further derivative.
 """
 from typing import NamedTuple, Optional, Tuple
 

@@ -3,6 +3,8 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -43,6 +45,22 @@ Tensor empty(at::IntArrayRef shape, ScalarType type, const Tensor& like) { retur
 // a tensor of the caller's that has been written: autograd is to know (inference tensors keep no count)
 void written(const Tensor* t) {
     if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+// Nothing here is recorded by autograd: an input that asks for a gradient would not get it, an output that asks for one would be written behind autograd's back.
+void no_tangent(const char* call, const Tensor* t, const char* name) {
+    TORCH_CHECK(t == nullptr || !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t->_fw_grad(0).defined(), call, " is not recorded by autograd, and ", name,
+                " carries a forward-mode derivative");
+}
+void not_recorded(const char* call, const Tensor* t, const char* name, const char* backward) {
+    if (t == nullptr) return;
+    TORCH_CHECK(!c10::GradMode::is_enabled() || !t->requires_grad(), call, " is not recorded by autograd, and ", name, " requires a gradient: call it under torch.no_grad(), with "
+                "detached tensors, or in a torch.autograd.Function whose backward pass calls ", backward);
+    no_tangent(call, t, name);
+}
+void not_written(const char* call, const Tensor* t, const char* name) {
+    TORCH_CHECK(t == nullptr || !c10::GradMode::is_enabled() || !t->requires_grad(), call, " is not recorded by autograd, and would write ", name,
+                ", which requires a gradient: call it under torch.no_grad(), or give a detached tensor");
+    no_tangent(call, t, name);
 }
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
 PyObject* wrap_or_none(const Tensor& t) {
@@ -142,6 +160,13 @@ PyObject* block_norm(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     const Tensor& residual = tensor(arg[0], "residual");
     const Tensor* y = optional_tensor(arg[1], "y");
     const Tensor *out = optional_tensor(arg[8], "residual_out"), *normed = optional_tensor(arg[9], "normed");
+    not_recorded("block_norm", &residual, "residual", "block_norm_backward");
+    not_recorded("block_norm", y, "y", "block_norm_backward");
+    not_recorded("block_norm", optional_tensor(arg[2], "pre_weight"), "pre_weight", "block_norm_backward");
+    not_recorded("block_norm", optional_tensor(arg[3], "post_weight"), "post_weight", "block_norm_backward");
+    not_recorded("block_norm", optional_tensor(arg[4], "gate"), "gate", "block_norm_backward");
+    not_written("block_norm", out, "residual_out");
+    not_written("block_norm", normed, "normed");
     const ScalarType type = y != nullptr ? y->scalar_type() : (normed != nullptr ? normed->scalar_type() : residual.scalar_type());
     Block b = block_inputs(arg + 2, type, residual, y);
     const int64_t tokens = b.a.tokens, hidden = b.a.hidden;
@@ -176,6 +201,11 @@ PyObject* block_norm_backward(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     const Tensor *d_out = optional_tensor(arg[0], "d_residual_out"), *d_normed = optional_tensor(arg[1], "d_normed");
     const Tensor& residual = tensor(arg[2], "residual");
     const Tensor* y = optional_tensor(arg[3], "y");
+    no_tangent("block_norm_backward", d_out, "d_residual_out");
+    no_tangent("block_norm_backward", d_normed, "d_normed");
+    no_tangent("block_norm_backward", &residual, "residual");
+    no_tangent("block_norm_backward", y, "y");
+    for (int i = 4; i < 7; ++i) no_tangent("block_norm_backward", optional_tensor(arg[i], "weights and gate"), "a weight or the gate");
     TORCH_CHECK((d_normed != nullptr) == (arg[4] != Py_None), "d_normed goes with pre_weight");
     TORCH_CHECK(d_normed != nullptr || d_out != nullptr, "the gradient of at least one output must be given");
     const ScalarType type = y != nullptr ? y->scalar_type() : (d_normed != nullptr ? d_normed->scalar_type() : residual.scalar_type());
@@ -253,9 +283,11 @@ PyObject* route_tokens(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK(n == 8, "route_tokens: arguments");
     const Tensor& logits = tensor(arg[0], "logits");
-    mm_router_args_t a = router_inputs(logits, whole(arg[1], "topk"), arg[2]);
-    const Tensor *bias = optional_tensor(arg[3], "expert_bias"), *valid = optional_tensor(arg[4], "valid");
+    const Tensor *bias = optional_tensor(arg[3], "expert_bias"), *valid = optional_tensor(arg[4], "valid");      // (neither has a gradient)
     const Tensor *idx = optional_tensor(arg[6], "topk_idx"), *weights = optional_tensor(arg[7], "topk_weights");
+    not_recorded("route_tokens", &logits, "logits", "router_backward");
+    not_written("route_tokens", weights, "topk_weights");
+    mm_router_args_t a = router_inputs(logits, whole(arg[1], "topk"), arg[2]);
     a.route_scale = static_cast<float>(number(arg[5], "route_scale"));
     const int64_t shape[2] = {a.tokens, a.topk};
     const float* bias_ptr = nullptr;
@@ -285,6 +317,7 @@ PyObject* balance_loss(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK(n == 6, "balance_loss: arguments");
     const Tensor &logits = tensor(arg[0], "logits"), &idx = tensor(arg[1], "topk_idx");
+    not_recorded("balance_loss", &logits, "logits", "router_backward");
     mm_router_args_t a = router_inputs(logits, topk_of(idx), arg[2]);
     a.topk_idx = static_cast<int64_t*>(plain(idx, "topk_idx", {a.tokens, a.topk}, at::kLong, logits));
     mm_balance_args_t b;
@@ -314,6 +347,10 @@ PyObject* router_backward(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     TORCH_CHECK(n == 12, "router_backward: arguments");
     const Tensor &logits = tensor(arg[0], "logits"), &idx = tensor(arg[1], "topk_idx");
+    no_tangent("router_backward", &logits, "logits");
+    no_tangent("router_backward", optional_tensor(arg[3], "d_topk_weights"), "d_topk_weights");
+    if (THPVariable_Check(arg[10])) no_tangent("router_backward", &THPVariable_Unpack(arg[10]), "d_loss");
+    not_written("router_backward", optional_tensor(arg[11], "d_logits"), "d_logits");
     mm_router_args_t a = router_inputs(logits, topk_of(idx), arg[2]);
     const int64_t shape[2] = {a.tokens, a.topk};
     a.topk_idx = static_cast<int64_t*>(plain(idx, "topk_idx", shape, at::kLong, logits));

@@ -3,7 +3,9 @@
 `fe_forward` and `mega_moe_from_hidden` route from bf16 hidden states inside the library. A program that has logits of its own (a 32-bit router, noise
 on the scores, experts that are switched off, padding) gets the same top-k and weights from `route_tokens`, into the buffer's views if it likes;
 in training `balance_loss` adds up how the experts are used, and `router_backward` is the logits' gradient of both in one pass. Nothing here is
-recorded by autograd.
+recorded by autograd: `route_tokens` and `balance_loss` refuse logits that require a gradient while gradients are enabled (a training step calls them from a
+`torch.autograd.Function`, or on detached logits, and hands what `router_backward` returns to `logits.backward`). `router_backward` takes such logits; its result has no
+further derivative.
 """
 from typing import Optional, Tuple, Union
 
