@@ -1,6 +1,7 @@
 """Ahead-of-time build of the CUDA library for sm_100a (in-tree shared object, no JIT cache)."""
 import importlib.util
 import os
+import runpy
 import shutil
 import subprocess
 import sysconfig
@@ -74,28 +75,43 @@ def build(force: bool = False, verbose: bool = False, check: bool = False) -> st
     return path
 
 
+def _compiler() -> str:
+    """The system's compiler, whatever CXX names: a binding with a C++ library of its own in it would not share torch's."""
+    return '/usr/bin/g++' if os.path.exists('/usr/bin/g++') else 'g++'
+
+
+def built_for(torch_dir: str) -> str:
+    """What a binding is good for besides its sources, as it carries it in itself: the torch and the Python whose headers it was compiled with."""
+    torch = runpy.run_path(os.path.join(torch_dir, 'version.py'))
+    return f'for torch {torch["__version__"]} {torch.get("git_version")}, {sysconfig.get_config_var("SOABI")}.'
+
+
+def binding_fits(torch_dir: str) -> bool:
+    with open(BINDING_PATH, 'rb') as f:
+        return built_for(torch_dir).encode() in f.read()
+
+
 def _build_binding(force: bool) -> str:
     """Compile the Python binding against the installed torch and the library next to it; returns what the compiler printed. A host that has no torch or no Python.h
     gets the library without it."""
     inputs = [os.path.join(CSRC, BINDING_SOURCE), os.path.join(CSRC, _ABI)]
-    if not force and not _stale(BINDING_PATH, inputs):
-        return ''
-    # (the system's compiler, whatever CXX names: a binding with a C++ library of its own in it would not share torch's)
-    cxx = '/usr/bin/g++' if os.path.exists('/usr/bin/g++') else 'g++'
     torch_spec = importlib.util.find_spec('torch')
     torch_dir = os.path.dirname(torch_spec.origin) if torch_spec is not None else ''
+    if not force and not _stale(BINDING_PATH, inputs) and torch_spec is not None and binding_fits(torch_dir):
+        return ''
+    cxx = _compiler()
     include = [os.path.join(torch_dir, 'include'), os.path.join(torch_dir, 'include', 'torch', 'csrc', 'api', 'include'), '/usr/local/cuda/include',
                sysconfig.get_paths()['include']]
     needs = [('torch', os.path.join(include[0], 'ATen')), ("Python's header", os.path.join(include[3], 'Python.h')), ('a C++ compiler', shutil.which(cxx) or '')]
     missing = [what for what, path in needs if not os.path.exists(path)]
     if missing:
-        # the library is complete without it; a binding of older sources must not stay
+        # the library is complete without it; a binding of older sources, or for another torch, must not stay
         if os.path.exists(BINDING_PATH):
             os.remove(BINDING_PATH)
         text = f'{os.path.basename(BINDING_PATH)} is not built, for want of {" and ".join(missing)}: the operators around the layer are to be had through the C ABI only'
         warnings.warn(text)
         return text + '\n'
-    return _run([[cxx, '-O2', '-std=c++17', '-shared', '-fPIC', '-fvisibility=hidden', '-o', BINDING_PATH] + [f'-I{i}' for i in include] +
+    return _run([[cxx, '-O2', '-std=c++17', '-shared', '-fPIC', '-fvisibility=hidden', f'-DMM_BUILT_FOR="{built_for(torch_dir)}"', '-o', BINDING_PATH] + [f'-I{i}' for i in include] +
                  [inputs[0], f'-L{PKG_DIR}', f'-l:{LIB_NAME}', f'-L{os.path.join(torch_dir, "lib")}', '-lc10', '-lc10_cuda', '-ltorch_cpu', '-ltorch_cuda',
                   '-ltorch_python', '-Wl,-rpath,$ORIGIN']])
 

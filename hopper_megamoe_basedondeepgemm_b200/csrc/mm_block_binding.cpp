@@ -399,4 +399,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "mm_block_binding", nullptr, -1, me
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_mm_block_binding(void) { return PyModule_Create(&module); }
+// `built_for`: the torch and the Python that it was compiled against, which the package looks for in the file before it loads it
+PyMODINIT_FUNC PyInit_mm_block_binding(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m != nullptr && PyModule_AddStringConstant(m, "built_for", MM_BUILT_FOR) != 0) { Py_DECREF(m); return nullptr; }
+    return m;
+}

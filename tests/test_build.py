@@ -70,3 +70,68 @@ def test_library_without_python_headers(tree, tmp_path):
         assert b.build() == str(tmp_path / 'lib.so')
     assert os.path.exists(tmp_path / 'lib.so') and not os.path.exists(tmp_path / 'bind.so')
     assert any('Python' in str(w.message) for w in seen)
+
+
+FAKE_BINDING = """#!{python}
+import os, sys
+with open({log!r}, 'a') as f:
+    f.write('binding\\n')
+with open(sys.argv[sys.argv.index('-o') + 1], 'w') as f:
+    f.write(' '.join(sys.argv))
+"""
+
+
+@pytest.fixture
+def versions(tree, tmp_path):
+    """A torch of a version that can be set, and a compiler that leaves its command in what it makes."""
+    (tmp_path / 'g++').write_text(FAKE_BINDING.format(python=sys.executable, log=str(tmp_path / 'log')))
+    torch_dir = tmp_path / 'torch'
+    (torch_dir / 'include' / 'ATen').mkdir(parents=True)
+    (torch_dir / '__init__.py').write_text('')
+    import importlib.util
+    find = importlib.util.find_spec
+    spec = importlib.util.spec_from_file_location('torch', str(torch_dir / '__init__.py'))
+    tree.patch.setattr(importlib.util, 'find_spec', lambda name, *a: spec if name == 'torch' else find(name, *a))
+
+    def set_version(v):
+        (torch_dir / 'version.py').write_text(f'__version__ = {v!r}\ngit_version = "abc"\n')
+        tree.age(torch_dir / 'version.py')
+    set_version('2.0')
+    return set_version
+
+
+def test_binding_goes_with_torch_and_python(tree, versions, tmp_path):
+    """Built again for another torch or Python although its sources are older; not without a reason."""
+    assert 'binding' in tree.built()
+    assert tree.built() == []
+    versions('2.1')
+    assert tree.built() == ['binding'] and tree.built() == []
+    assert b.binding_fits(str(tmp_path / 'torch'))
+    get = sysconfig.get_config_var
+    tree.patch.setattr(sysconfig, 'get_config_var', lambda name: 'cpython-399' if name == 'SOABI' else get(name))
+    assert not b.binding_fits(str(tmp_path / 'torch'))
+    assert tree.built() == ['binding'] and tree.built() == []
+
+
+def test_a_binding_that_fits_stays_without_headers(tree, versions, tmp_path):
+    assert 'binding' in tree.built()
+    paths = dict(sysconfig.get_paths(), include=str(tmp_path / 'nowhere'))
+    tree.patch.setattr(sysconfig, 'get_paths', lambda *a, **k: paths)
+    with warnings.catch_warnings():
+        warnings.simplefilter('error')
+        assert tree.built() == []
+    assert os.path.exists(tmp_path / 'bind.so')
+    versions('2.1')                            # and goes where it does not fit and cannot be built
+    with pytest.warns(UserWarning):
+        assert tree.built() == []
+    assert not os.path.exists(tmp_path / 'bind.so')
+
+
+def test_the_package_does_not_load_a_binding_for_another_torch(monkeypatch, tmp_path):
+    from hopper_megamoe_basedondeepgemm_b200 import _binding
+    other = tmp_path / 'mm_block_binding.so'
+    other.write_bytes(b'for torch 1.0 abc, cpython-27.')
+    monkeypatch.setattr(b, 'BINDING_PATH', str(other))
+    monkeypatch.setattr(_binding, 'BINDING_PATH', str(other))
+    with pytest.raises(RuntimeError, match='another torch'):
+        _binding._Binding().block_norm
