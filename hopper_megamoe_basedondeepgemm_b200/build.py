@@ -5,6 +5,7 @@ import runpy
 import shutil
 import subprocess
 import sysconfig
+import time
 import warnings
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -36,40 +37,74 @@ def _stale(path: str, files) -> bool:
     return any(os.path.getmtime(f) > t for f in files)
 
 
-def _run(cmds):
-    """Run the commands side by side; returns what they printed, raises if one failed."""
-    running = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for c in cmds]
-    out = [p.communicate()[0] for p in running]
-    for p, text in zip(running, out):
-        if p.returncode != 0:
-            raise RuntimeError(f'{p.args[0]} failed:\n{text}')
+def _record(path: str) -> str:
+    """Where it says by which commands a file was made."""
+    return os.path.join(OBJ_DIR, os.path.basename(path) + '.cmd')
+
+
+def _named(*commands) -> str:
+    """Commands as they count: wherever the package lies, and whatever they print."""
+    return '\n'.join(' '.join(c.replace(PKG_DIR, '.') for c in command if c not in ('-Xptxas', '-v')) for command in commands)
+
+
+def _recorded(path: str):
+    if not os.path.exists(_record(path)):
+        return None
+    with open(_record(path)) as f:
+        return f.read()
+
+
+def _run(cmds, start, names=None):
+    """Run the commands side by side, each with the file that it makes behind `-o`; returns what they printed, raises if one failed. A file is made under another name and takes its own
+    when it is complete: what a compiler leaves that was stopped is not taken for it. Its time is `start`, so a source that changes meanwhile is newer."""
+    running = []
+    for c in cmds:
+        at = c.index('-o') + 1
+        part = f'{c[at]}.{os.getpid()}.part'
+        running.append((c, c[at], part, subprocess.Popen(c[:at] + [part] + c[at + 1:], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    out, failed = [], ''
+    for c, path, part, p in running:
+        out.append(p.communicate()[0])
+        if p.returncode == 0:
+            os.utime(part, (start, start))
+            os.replace(part, path)
+            with open(_record(path), 'w') as f:
+                f.write(names or _named(c))
+        else:
+            failed = failed or f'{c[0]} failed:\n{out[-1]}'
+            if os.path.exists(part):
+                os.remove(part)
+    if failed:
+        raise RuntimeError(failed)
     return ''.join(out)
 
 
 def build(force: bool = False, verbose: bool = False, check: bool = False) -> str:
     """Compile `csrc/*.cu` into `libmegamoe_b200.so` next to this file (`check`: the test build with the cross-check
-    engine, `libmegamoe_b200_check.so`); returns its path. Sources whose object file is up to date are not compiled again."""
+    engine, `libmegamoe_b200_check.so`); returns its path. Sources whose object file is up to date, and was made by the same command, are not compiled again."""
+    start = time.time()
     path = CHECK_LIB_PATH if check else LIB_PATH
-    inputs = [os.path.join(CSRC, f) for s in SOURCES for f in [s] + SOURCES[s]]
-    if not force and not _stale(path, inputs):
-        if not check:
-            _build_binding(False)
-        return path
     nvcc = os.environ.get('NVCC', '/usr/local/cuda/bin/nvcc')
-    os.makedirs(OBJ_DIR, exist_ok=True)
-    objects, cmds = [], []
+    cmds, inputs = {}, {}                    # by object file
     for source, headers in SOURCES.items():
         own = check and source in CHECK_SOURCES
         obj = os.path.join(OBJ_DIR, source[:-3] + ('_check.o' if own else '.o'))
-        objects.append(obj)
-        if force or _stale(obj, [os.path.join(CSRC, f) for f in [source] + headers]):
-            cmds.append([nvcc] + (['-Xptxas', '-v'] if verbose else []) +
-                        ['-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo', '-O3', '-std=c++17', '-Xcompiler', '-fPIC', '-c', '-o', obj] +
-                        (['-DMM_WITH_CHECK_ENGINE'] if own else []) + [os.path.join(CSRC, source)])
-    text = _run(cmds)
-    _run([[nvcc, '-gencode', 'arch=compute_100a,code=sm_100a', '-shared', '-Xcompiler', '-fPIC', '-o', path] + objects])
+        inputs[obj] = [os.path.join(CSRC, f) for f in [source] + headers]
+        cmds[obj] = [nvcc] + (['-Xptxas', '-v'] if verbose else []) + \
+            ['-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo', '-O3', '-std=c++17', '-Xcompiler', '-fPIC', '-c', '-o', obj] + \
+            (['-DMM_WITH_CHECK_ENGINE'] if own else []) + [os.path.join(CSRC, source)]
+    link = [nvcc, '-gencode', 'arch=compute_100a,code=sm_100a', '-shared', '-Xcompiler', '-fPIC', '-o', path] + list(cmds)
+    names = _named(*cmds.values(), link)
+    # (a library that came without its record is taken as it is)
+    if not force and not _stale(path, [f for files in inputs.values() for f in files]) and _recorded(path) in (None, names):
+        if not check:
+            _build_binding(False, start)
+        return path
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    text = _run([c for obj, c in cmds.items() if force or _stale(obj, inputs[obj]) or _recorded(obj) != _named(c)], start)
+    text += _run([link], start, names)
     if not check:
-        text += _build_binding(force)
+        text += _build_binding(force, start)
     if verbose:
         print(text)
     return path
@@ -91,7 +126,7 @@ def binding_fits(torch_dir: str) -> bool:
         return built_for(torch_dir).encode() in f.read()
 
 
-def _build_binding(force: bool) -> str:
+def _build_binding(force: bool, start: float) -> str:
     """Compile the Python binding against the installed torch and the library next to it; returns what the compiler printed. A host that has no torch or no Python.h
     gets the library without it."""
     inputs = [os.path.join(CSRC, BINDING_SOURCE), os.path.join(CSRC, _ABI)]
@@ -111,9 +146,10 @@ def _build_binding(force: bool) -> str:
         text = f'{os.path.basename(BINDING_PATH)} is not built, for want of {" and ".join(missing)}: the operators around the layer are to be had through the C ABI only'
         warnings.warn(text)
         return text + '\n'
+    os.makedirs(OBJ_DIR, exist_ok=True)
     return _run([[cxx, '-O2', '-std=c++17', '-shared', '-fPIC', '-fvisibility=hidden', f'-DMM_BUILT_FOR="{built_for(torch_dir)}"', '-o', BINDING_PATH] + [f'-I{i}' for i in include] +
                  [inputs[0], f'-L{PKG_DIR}', f'-l:{LIB_NAME}', f'-L{os.path.join(torch_dir, "lib")}', '-lc10', '-lc10_cuda', '-ltorch_cpu', '-ltorch_cuda',
-                  '-ltorch_python', '-Wl,-rpath,$ORIGIN']])
+                  '-ltorch_python', '-Wl,-rpath,$ORIGIN']], start)
 
 
 if __name__ == '__main__':

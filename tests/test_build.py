@@ -135,3 +135,51 @@ def test_the_package_does_not_load_a_binding_for_another_torch(monkeypatch, tmp_
     monkeypatch.setattr(_binding, 'BINDING_PATH', str(other))
     with pytest.raises(RuntimeError, match='another torch'):
         _binding._Binding().block_norm
+
+
+LIBRARY = ['nvcc a', 'nvcc b', 'nvcc lib']
+
+
+def test_only_what_changed_is_compiled(tree, tmp_path, versions):
+    assert tree.built() == ['binding'] + LIBRARY and tree.built() == []
+    (tmp_path / 'csrc' / 'a.h').write_text('x')
+    os.utime(tmp_path / 'csrc' / 'a.h', (2e9, 2e9))
+    assert tree.built() == ['nvcc a', 'nvcc lib']
+    tree.age(tmp_path / 'csrc' / 'a.h')
+    assert tree.built() == []
+    assert tree.built(force=True, verbose=True) == ['binding'] + LIBRARY and tree.built() == []
+    assert tree.built(check=True) == ['nvcc a_check', 'nvcc lib_check'] and tree.built(check=True) == []
+
+
+def test_what_a_stopped_compiler_leaves_is_not_taken(tree, tmp_path, versions):
+    """Its file is newer than the source, and not complete."""
+    (tmp_path / 'break').write_text('')
+    with pytest.raises(RuntimeError):
+        tree.built()
+    assert not os.path.exists(tmp_path / 'obj' / 'a.o') and not os.path.exists(tmp_path / 'lib.so')
+    (tmp_path / 'break').unlink()
+    assert tree.built() == ['binding'] + LIBRARY
+    assert not [f for _, _, files in os.walk(tmp_path) for f in files if f.endswith('.part')]
+
+
+def test_other_commands_make_other_files(tree, tmp_path, versions, monkeypatch):
+    """Another compiler: all again. The same tree in another place: nothing. A library that came without objects and records is taken as it is."""
+    tree.built()
+    (tmp_path / 'nvcc2').write_text((tmp_path / 'nvcc').read_text())
+    (tmp_path / 'nvcc2').chmod(0o755)
+    monkeypatch.setenv('NVCC', str(tmp_path / 'nvcc2'))
+    assert tree.built() == LIBRARY and tree.built() == []
+    for f in os.listdir(tmp_path / 'obj'):
+        os.unlink(tmp_path / 'obj' / f)
+    assert tree.built() == []
+    os.unlink(tmp_path / 'lib.so')
+    assert tree.built() == LIBRARY
+
+
+def test_a_source_that_changes_while_it_is_compiled(tree, tmp_path, versions):
+    """What is made of it is older than it."""
+    fake = (tmp_path / 'nvcc').read_text()
+    (tmp_path / 'nvcc').write_text(fake + f"if out.split('/')[-1].startswith('a.o'):\n    os.utime({str(tmp_path / 'csrc' / 'a.cu')!r})\n")
+    assert 'nvcc a' in tree.built()
+    (tmp_path / 'nvcc').write_text(fake)
+    assert tree.built() == ['nvcc a', 'nvcc lib'] and tree.built() == []
