@@ -28,7 +28,8 @@ def block_norm(residual: torch.Tensor, y: Optional[torch.Tensor] = None, *, pre_
     the gate are of that type or fp32. `gate`: `[hidden]`, `[tokens, 1]`, `[tokens, hidden]` or none. Rows may be strided; hidden is at most 8192.
     Without `y` the stream is only normalised, and returned as it is; without `pre_weight` there is no `normed` (None). `residual_out` may be
     `residual` and `normed` may be `y` or `residual` (the same rows); any other overlap is refused. `normed` has the type of `y` (without `y`:
-    that of the given `normed`, or of the stream). Sums of squares are kept in 32 bits, which hold values up to about 1e17.
+    that of the given `normed`, or of the stream). Sums of squares are kept in 32 bits, which hold values up to about 1e17;
+    `eps` is at least 2^-126, so that squares too small for 32 bits vanish beside it.
     """
     return binding.block_norm(residual, y, pre_weight, post_weight, gate, scale, eps, weight_offset, residual_out, normed)
 

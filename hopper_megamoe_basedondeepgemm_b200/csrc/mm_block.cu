@@ -1,5 +1,6 @@
 // C ABI of the operators around the layer: a block's norms, routing from logits, the balance loss. Argument checks and launches; no torch types, no exceptions.
 #include <cuda_runtime.h>
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 
@@ -59,7 +60,8 @@ int norm_check(const mm_block_norm_args_t* a) {
         if ((a->gate_mode != MM_GATE_NONE) != (a->gate != nullptr) || (a->gate != nullptr && a->y == nullptr)) return MM_ERR_INVALID_ARGUMENT;
         if (a->y == nullptr && (a->post_weight != nullptr || a->pre_weight == nullptr)) return MM_ERR_INVALID_ARGUMENT;
     }
-    if (!(a->eps > 0.f) || !std::isfinite(a->eps) || !std::isfinite(a->scale) || !std::isfinite(a->weight_offset)) return MM_ERR_INVALID_ARGUMENT;
+    // (a subnormal eps would stand beside squares that 32 bits no longer hold)
+    if (!(a->eps >= FLT_MIN) || !std::isfinite(a->eps) || !std::isfinite(a->scale) || !std::isfinite(a->weight_offset)) return MM_ERR_INVALID_ARGUMENT;
     return MM_OK;
 }
 

@@ -269,7 +269,7 @@ typedef struct mm_block_norm_args {
     int32_t dtype;                   /* enum mm_dtype, of y and normed */
     int32_t stream_dtype, weight_dtype, gate_dtype;      /* each `dtype` or MM_DTYPE_FP32 */
     int32_t gate_mode;
-    float scale, eps, weight_offset; /* eps > 0 */
+    float scale, eps, weight_offset; /* eps at least 2^-126 */
 } mm_block_norm_args_t;
 
 /* The gradients' side of mm_block_norm_backward. Outputs and the workspace that share memory with each other or with an input are refused. */

@@ -1,4 +1,5 @@
-"""`mm_block_norm_backward` refuses outputs that share memory with anything else of the call, weights' and gates' gradients and the workspace among them."""
+"""More of what the C ABI of the norms refuses: `mm_block_norm_backward` outputs that share memory with anything else of the call, weights' and gates' gradients and the workspace
+among them, and an eps that 32 bits hold only in part."""
 import ctypes
 
 import pytest
@@ -41,3 +42,16 @@ def test_calls_that_pass_the_checks(norm, grads):
     if torch.cuda.is_available():
         pytest.skip('the addresses are not real')
     assert _call(norm, grads) == 3
+
+
+@pytest.mark.parametrize('eps', [2.0 ** -127, 1e-40, 2.0 ** -149])
+def test_subnormal_eps_is_refused(eps):
+    """Beside such an eps the squares of small rows count, and 32 bits do not hold them."""
+    assert _lib.load().mm_block_norm(ctypes.byref(_norm(eps=eps)), None) == INVALID
+    assert _call(dict(eps=eps), {}) == INVALID
+
+
+def test_smallest_eps():
+    if torch.cuda.is_available():
+        pytest.skip('the addresses are not real')
+    assert _lib.load().mm_block_norm(ctypes.byref(_norm(eps=2.0 ** -126)), None) == 3 and _call(dict(eps=2.0 ** -126), {}) == 3

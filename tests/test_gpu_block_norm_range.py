@@ -50,3 +50,12 @@ def test_small_rows_and_small_eps(tokens, hidden, types, size, eps):
             if x[name] is not None:
                 x[name][tokens // 2:tokens // 2 + 2] = 0
         _check_gradients(x, d_stream, d_normed, mm.block_norm_backward(d_stream, d_normed, **x, eps=eps), eps=eps)
+
+
+@pytest.mark.parametrize('size', [1.0, 1e-17, 1e-19, 1e-21, 0.0])
+def test_smallest_eps(size):
+    """Rows around the root of the smallest eps: squares below what 32 bits hold are nothing beside it."""
+    for kind in (dict(), dict(gate='token')):
+        x, _, _ = _scaled(20, 512, size, 1.0, dtype=FP32, **kind)
+        x['post_weight'] = x['post_weight'] * size                         # the stream stays that small
+        _check_forward(x, mm.block_norm(**x, eps=2.0 ** -126), eps=2.0 ** -126)
