@@ -29,8 +29,8 @@
 
 namespace mm {
 
-// Sums of probabilities over tokens are kept as multiples of 2^-36 in 64 bits: additions of whole numbers, whose order changes nothing. 2^27 tokens fit.
-constexpr float kRtFixed = 68719476736.0f;
+// Sums of probabilities over tokens are kept as whole numbers of 64 bits, whose additions' order changes nothing: multiples of `q.step`, 2^-63 of the next power of two above
+// the number of tokens.
 constexpr int kRtFlushRows = 64;             // rows that a warp sums in 32 bits before they go into the 64-bit sum
 
 template <typename L> __device__ __forceinline__ float rt_float(L v);
@@ -354,7 +354,6 @@ __device__ __forceinline__ void rt_block_sum(double (&v)[N], double (*part)[N]) 
 __device__ __forceinline__ double rt_balance_cells(const RtParams& q, long long first, long long stride) {
     constexpr int kBatch = 6;                // cells in flight
     const long long cells = static_cast<long long>(q.S) * q.E;
-    const float inv_fixed = 1.f / kRtFixed;
     double balance = 0.0;
     for (long long i0 = first; i0 < cells; i0 += kBatch * stride) {
         unsigned long long sum[kBatch];
@@ -370,7 +369,7 @@ __device__ __forceinline__ double rt_balance_cells(const RtParams& q, long long 
         for (int b = 0; b < kBatch; ++b) {
             const long long i = i0 + b * stride;
             if (i >= cells) break;
-            const float inv = n[b] > 0 ? 1.f / static_cast<float>(n[b]) : 0.f, mean = static_cast<float>(sum[b]) * inv_fixed * inv;
+            const float inv = n[b] > 0 ? 1.f / static_cast<float>(n[b]) : 0.f, mean = static_cast<float>(sum[b]) * q.step * inv;
             q.mean[i] = mean;
             q.counts[i] = count[b];
             balance += static_cast<double>(static_cast<float>(count[b]) * inv) * static_cast<double>(mean);
@@ -482,6 +481,7 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lo = rt_share(q, blockIdx.x), hi = rt_share(q, blockIdx.x + 1);
+    const float per_one = 1.f / q.step;
     for (int e = threadIdx.x; e < V * 32; e += blockDim.x) hist[e] = 0;
     __syncthreads();
     grid_dependency_wait();                  // (for the cleared sums, and for the logits and routes of kernels ahead of `balance_zero_kernel`: only a grid that waits sees what others wrote)
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
             for (int e = threadIdx.x; e < q.E; e += blockDim.x) {
                 unsigned long long sum = 0ull;
                 #pragma unroll
-                for (int w = 0; w < kRtWarps; ++w) sum += __float2ull_rn(warp_sum[w][e] * kRtFixed);
+                for (int w = 0; w < kRtWarps; ++w) sum += __float2ull_rn(warp_sum[w][e] * per_one);
                 const long long to = static_cast<long long>(s) * q.E + e;
                 if (sum != 0ull) atomicAdd(q.sums + to, sum);
                 if (hist[e] != 0) { atomicAdd(q.sum_counts + to, hist[e]); hist[e] = 0; }
@@ -795,6 +795,8 @@ int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
         const int ctas = grid < most ? grid : most;
         RtParams b = shared_out(ctas);
         b.z_parts = ctas;
+        b.step = 0x1p-63f;
+        while (b.step * 0x1p63f < static_cast<float>(q.T)) b.step *= 2.f;    // (T as a float may be 2^-24 less: the sums have a bit to spare)
         const long long zero = (b.zero_words + 1023) / 1024;
         MM_CUDA(launch_behind(balance_zero_kernel<L>, static_cast<int>(zero < sms ? zero : sms), 256, stream, b));
         MM_CUDA(launch_behind(balance_kernel<L, V, Mode>, b.z_parts, kRtWarps * 32, stream, b));

@@ -24,6 +24,7 @@ struct RtParams {
     int T, E, K, S, mode;
     int share, shares_more;                  // tokens of a CTA or warp, and how many of the first ones have one more
     float route_scale, balance_coef, z_coef, d_loss;
+    float step;                              // of the sums of probabilities
     const float* d_loss_ptr;                 // device scalar, or nullptr: d_loss
     const float* d_weights;                  // [T][K] or nullptr
     int* counts;                             // [S][E]
