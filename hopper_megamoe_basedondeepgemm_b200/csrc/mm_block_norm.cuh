@@ -18,7 +18,7 @@
 // the rows, of dr n1 (token's or element's gate), times the other's factor. Rows are multiplied by their root before anything else: powers of i1 and i2 by
 // themselves leave the range of 32 bits for streams from 10^12 on, and for rows of zeros with an eps below 10^-25.
 //
-// A row belongs to one CTA, or from 4096 channels on to two (a cluster), eight channels to a thread. Bound by memory: the bytes of the rows, in and out. CTAs stay and walk over the rows; a
+// A row belongs to one CTA, or with more than 4096 channels to two (a cluster), eight channels to a thread. Bound by memory: the bytes of the rows, in and out. CTAs stay and walk over the rows; a
 // thread asks for its part of the next row before it works on the one it has, and while a row's sums are exchanged, the sum of squares of the next row's
 // y goes with them: one barrier a row.
 #pragma once
@@ -341,8 +341,9 @@ enum BnKind { kBnPlain = 0 /* no gate, or one that is part of y's factor */, kBn
 // 64 registers a thread, so two CTAs of 512 threads an SM; 16-bit streams 56, so three of 384. 16384 x 4096, 32-bit stream, both norms, channel gate: 127 us (6.3 TB/s); 8192 x
 // 3072 in bf16 37 us (5.4). (One CTA of twice the registers an SM 168 us; sixteen channels a thread 134; rows copied ahead into shared memory by cp.async
 // 160. y one row ahead, bf16 40 us; two rows ahead with a 32-bit stream, which then has no register left, 137.)
-// Rows over two CTAs wait for the cluster's barrier: 8192 x 8192 bf16 120 us (4.5 TB/s), 32-bit stream 161 (5.0), 4096 x 6144 bf16 48 (64 registers, so two CTAs an SM, 55; one
-// CTA with sixteen channels a thread and nothing in flight ahead 178). Clusters of four are slower: 173, 232 and 76.
+// Rows over two CTAs wait for the cluster's barrier (and for the stores that its release orders): 8192 x 8192 bf16 121 us (4.4 TB/s), 32-bit stream 158 (5.1), 32-bit activations
+// 191 (5.6), 4096 x 6144 bf16 47 (64 registers, so two CTAs an SM, 55; one CTA with sixteen channels a thread and nothing in flight ahead 178). Clusters of four are slower: 173,
+// 232 with a 32-bit stream, and 76.
 template <typename X, typename R, bool Post, bool Pre, int Kind, int Lay>
 __global__ void __maxnreg__((sizeof(R) == 2 && (Lay & kBnWhole) != 0 && Kind != kBnElement ? 56 : 64)) block_norm_kernel(const BnParams q) {
     constexpr bool kWhole = (Lay & kBnWhole) != 0, kTwo = (Lay & kBnTwo) != 0;
@@ -436,15 +437,15 @@ __global__ void __maxnreg__((sizeof(R) == 2 && (Lay & kBnWhole) != 0 && Kind != 
 }
 
 // Rows are dealt to the CTAs in turn; a thread sums what the gradients of its channels' weights are made of over the CTA's rows and leaves it in `partial`, which
-// `block_norm_sums_kernel` adds up: always in the same order. Some 400 instructions a warp and row, so the issue slots are half full; what is left is the wait for a row's
+// `block_norm_sums_kernel` adds up: always in the same order. Some 330 instructions a warp and row, so the issue slots are half full; what is left is the wait for a row's
 // exchange, and registers bound what can go on meanwhile: 128 a thread, a row being worked on and a row on its way, y two rows ahead (its sum of squares goes
-// with the exchange of the row before). 8192 x 4096, 32-bit stream, both norms: 97 us (6.2 TB/s); y one row ahead 131.
+// with the exchange of the row before). 8192 x 4096, 32-bit stream, both norms: 100 us (6.0 TB/s); y one row ahead 131.
 // Where a CTA of 128 registers a thread leaves an SM's registers half used and no second one fits (more than 256 threads, up to 384: hidden 2056 to 3072, and 4104 to 6144 over two CTAs), it takes two rows
-// at a time through one exchange, with 168: 8192 x 3072 in bf16 59 us instead of 67, only the stream's norm 53 instead of 64, 32-bit stream 74 instead of 81. (With 256 threads
-// two CTAs of one row win, 42 us against 46 for 8192 x 2048; with an element's gate, or 32-bit
+// at a time through one exchange, with 168: 8192 x 3072 in bf16 62 us (one row at a time 67), with a token's gate 64, with a 32-bit stream 78 (81). (With 256 threads
+// two CTAs of one row win, 44 us against 46 for 8192 x 2048; with an element's gate, or 32-bit
 // activations, two rows do not fit the registers.) With an element's gate one row takes those 168: 128 are too few, and a register that is put away while its load is on its way
 // waits for it (8192 x 3072 bf16 82 us instead of 94, 8192 x 3001 134 instead of 370; odd rows without such a gate are faster with 128, 114 against 141).
-// Rows over two CTAs: 8192 x 8192 bf16 254 us (3.2 TB/s), 32-bit stream 276 (4.4), 4096 x 6144 bf16, two rows at a time, 85 (one at a time 111; clusters of four 172).
+// Rows over two CTAs: 8192 x 8192 bf16 259 us (3.1 TB/s), 32-bit stream 277 (4.4), 4096 x 6144 bf16, two rows at a time, 87 (one at a time 111; clusters of four 172).
 template <typename X, typename R, bool Post, bool Pre, int Kind, int Lay, int Rows, int Most>
 __global__ void __launch_bounds__(Most, 1) block_norm_backward_kernel(const BnParams q) {
     constexpr bool kY = Kind != kBnStream, kSumV = Post || Kind == kBnToken;

@@ -12,8 +12,8 @@
 //             over the selected slots; of the square 2 lse softmax_e.
 //
 // One warp holds a token's logits in registers, expert j * 32 + lane in slot j of a lane: neighbouring lanes read neighbouring experts wherever a row starts,
-// and the order of slots and lanes is that of the experts. Bound by instructions more than by memory: 680 a token to route one over 384 experts,
-// 250 for its balance loss, 420 for its gradient, against 4 bytes an expert.
+// and the order of slots and lanes is that of the experts. More instructions than memory, against 4 bytes an expert: 690 a token to route one over 384 experts and 406 for
+// the gradient, which bound both (64 % of the issue slots); 245 for the balance loss, which its CTAs' barriers and common sums bound (37 %).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -521,8 +521,8 @@ __global__ void __launch_bounds__(kRtWarps * 32, rt_ctas<V>()) balance_kernel(co
 }
 
 // Few tokens: one cluster, whose CTAs keep their sums in shared memory and add up each other's: one launch, nothing in memory but the results. A call from Python takes
-// 2.5 us less of the host than with two launches (with the gradient 12.9 and 15.4 us a pass). On the GPU 16 tokens of 48 experts take 4.7 us (6.4), 64 5.4 (6.4), 256 6.5
-// (6.4), 400 7.2 (6.4): the border is where that costs more than it gives.
+// 2.5 us less of the host than with two launches (with the gradient 12.9 and 15.4 us a pass). On the GPU 16 tokens of 48 experts take 3.2 us, 256 5.4, 384 5.9, and by the two
+// launches 385 take 5.9; of 384 experts 4.2, 5.9, 6.5 and 6.2, in five sequences 6.6, 7.8, 8.5 and 9.2: the border is where the GPU begins to lose.
 template <typename T>
 __device__ __forceinline__ T rt_of_cta(const T* p, uint32_t rank) {      // the same variable of another CTA of the cluster
     static_assert(sizeof(T) == 4 || sizeof(T) == 8);
@@ -789,8 +789,8 @@ int rt_launch_kernel(RtOp op, const RtParams& q, int sms, cudaStream_t stream) {
     }
     if (op == kRtBalance) {
         // one sequence: two CTAs an SM at most, because what each CTA adds to the same sums and counts costs more than its share of the tokens (16384 tokens of 48 experts
-        // 10.0 us, with five an SM 11.8); several sequences: all that fit, because a CTA takes its pieces of sequences one after the other (12000 tokens of 128
-        // experts in 37 sequences 16.2 us, with two an SM 18.0)
+        // with the gradient 15.4 us, with five an SM 17.0); several sequences: all that fit, because a CTA takes its pieces of sequences one after the other (12000 tokens of 128
+        // experts in 37 sequences 23.5 us, with two an SM 24.6)
         const int most = q.cu == nullptr && 2 * sms < kRtBalanceCtas ? 2 * sms : kRtBalanceCtas;
         const int ctas = grid < most ? grid : most;
         RtParams b = shared_out(ctas);

@@ -31,9 +31,10 @@ def route_tokens(logits: torch.Tensor, topk: int, score_mode: int = 0, expert_bi
 class BalanceLoss:
     """What `balance_loss` returns, and `router_backward` takes.
 
-    losses      fp32 [3]: balance_coef * balance + z_coef * z, balance, z
+    losses      fp32 [3]: balance_coef * balance + z_coef * z, balance, z (no graph: `router_backward` has their gradient)
     counts      int32 [sequences, experts]: routing slots per expert
-    mean_probs  fp32 [sequences, experts]: mean probability of the expert over the sequence's routed tokens
+    mean_probs  fp32 [sequences, experts]: mean probability of the expert over the sequence's routed tokens (summed in steps of 2^-63 of the next power of two above the number
+                of tokens)
     tokens      int32 [sequences]: tokens with a route
     """
     __slots__ = ('losses', 'counts', 'mean_probs', 'tokens', 'cu_seqlens', 'balance_coef', 'z_coef', 'score_mode')
