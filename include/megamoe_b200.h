@@ -315,7 +315,8 @@ typedef struct mm_balance_args {
 } mm_balance_args_t;
 
 /* The topk experts with the largest keys (logits; or sigmoid + expert_bias, compared as in 64 bits), ties to the lower expert, and their
- * weights: what mm_fe_forward and mm_frontend_launch work out from hidden states, from logits that the caller has. Tokens whose `valid` is
+ * weights: what mm_fe_forward and mm_frontend_launch work out from hidden states (there with sigmoids in 32 bits), from logits that the caller has. Weights of
+ * sigmoids are their ratio also where 32 bits do not hold them, and 0 where 64 do not (all selected logits below -709). Tokens whose `valid` is
  * 0, and slots for which no expert is left, get -1 and weight 0. Here and below, outputs (and the workspace) that share memory with each
  * other or with an input are refused. */
 int mm_route_tokens(const mm_router_args_t* args, const float* expert_bias, const uint8_t* valid, void* stream);
